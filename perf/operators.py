@@ -382,7 +382,7 @@ def _run_own(state):
         return packed
     leaves = [state["q"], state["k"], state["v"]] + ([state["table"]] if state["table"] is not None else [])
     grads = torch.autograd.grad(out, leaves, state["grad"])
-    return packed + [x.reshape(-1, *x.shape[-2:]) for x in grads]
+    return packed + [x.reshape(-1, *x.shape[-2:]) for x in grads[:3]] + list(grads[3:])
 
 
 def run(state):
