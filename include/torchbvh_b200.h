@@ -274,6 +274,113 @@ int tbvh_query_knn_share_multicast(int device, const float* node_aabbs, const in
 /* dst[i] = src[i] (int32 -> int64) for i < count, on `stream`. No reference counterpart. */
 int tbvh_widen_indices(int device, const int32_t* src, int64_t* dst, int64_t count, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Block selection and block attention (no reference counterpart: the
+ * reference's multi-head helpers weigh neighbours by inverse distance,
+ * torchbvh/_multihead.py:151-190; these give them learned weights).
+ *
+ * A block is a run of 64 consecutive leaves of a cloud's sorted order. For
+ * every query tbvh_select_blocks takes the num_blocks blocks whose boxes are
+ * nearest; tbvh_attend_blocks is multi-head softmax attention over the points
+ * of those blocks, with an optional learned bias by distance bucket.
+ */
+
+/* Geometry of a selection. points_per_cloud > 0: num_clouds clouds of that
+ * size with queries_per_cloud queries each, tables NULL. Else ragged: the
+ * table of tbvh_block_table, on the host and on the device. */
+typedef struct tbvh_block_geometry {
+  int device;
+  int dim;                        /* 2 or 3 */
+  int num_blocks;                 /* blocks per query, 1..32 */
+  int backward;                   /* 1: the plan also serves the backward pass */
+  int64_t num_clouds;
+  int64_t points_per_cloud;
+  int64_t queries_per_cloud;
+  const int64_t* table_host;      /* [num_clouds][7] */
+  const int64_t* table_dev;
+  const float* node_aabbs;        /* of tbvh_build */
+  const int64_t* sorted_indices;  /* of tbvh_build */
+  const float* query_points;      /* [total_queries][dim]; read by tbvh_select_blocks only */
+  const int64_t* order;           /* of tbvh_sort_queries; NULL: the given order; read by the same only */
+  void* plan;                     /* tbvh_block_plan_size() bytes, kept with the selection */
+  size_t plan_bytes;
+} tbvh_block_geometry;
+
+/* Host only: fills table_out[num_clouds][7] (first point, points, first node
+ * row, first query, queries, first tile, first block of each cloud) from host
+ * offsets of num_clouds + 1 entries. Queries per cloud may be zero. */
+int tbvh_block_table(int64_t num_clouds, const int64_t* point_offsets, const int64_t* query_offsets,
+                     int64_t* table_out);
+
+/* Bytes of the plan buffer of this selection (0 for a bad geometry); reads the
+ * sizes of `g` only. */
+size_t tbvh_block_plan_size(const tbvh_block_geometry* g);
+
+/* The num_blocks nearest blocks of every query: out_blocks int64
+ * [total_queries][num_blocks] (block of the query's cloud), out_distances
+ * float32, ascending by (squared box distance, block). The distance is
+ * sum over axes of max(lo - q, max(q - hi, 0))^2 in float32, each operation
+ * rounded, x first. Slots past the cloud's blocks, and every slot of a query
+ * whose distances are not below FLT_MAX (infinite, NaN), hold -1 and FLT_MAX.
+ * Fills the plan, which keeps what attention needs of the queries. */
+int tbvh_select_blocks(const tbvh_block_geometry* g, int64_t* out_blocks, float* out_distances, void* stream);
+
+enum { TBVH_F32 = 0, TBVH_F16 = 1, TBVH_BF16 = 2 };
+
+/* Features of one attention call: queries [total_queries][heads][channels],
+ * keys and values [total_points][kv_heads][channels], contiguous, in the
+ * caller's point and query order. heads is a multiple of kv_heads; channels
+ * 1..128. Bias: table [heads][num_buckets] float32 and num_buckets - 1 edges;
+ * the bucket of a pair is the number of edges not above its squared distance
+ * (float32, each operation rounded, x first). num_buckets 0: no bias, else
+ * 1..64. */
+typedef struct tbvh_attend_features {
+  int dtype;
+  int heads;
+  int kv_heads;
+  int channels;
+  float scale;
+  int num_buckets;
+  const void* queries;
+  const void* keys;
+  const void* values;
+  const float* bias_table;
+  const float* bias_edges;
+} tbvh_attend_features;
+
+/* out [total_queries][heads][channels] of the features' type; for the backward
+ * pass lse [total_queries][heads] float32, the base-2 logarithm of each row's
+ * sum of exponentials, and out_exact, out before its rounding to 16 bits (both
+ * may be NULL: not kept). A row without a key (no block, or all logits
+ * -infinity) is 0. */
+size_t tbvh_attend_blocks_workspace_size(const tbvh_block_geometry* g, const tbvh_attend_features* f);
+int tbvh_attend_blocks(const tbvh_block_geometry* g, const tbvh_attend_features* f, void* out, float* lse,
+                       float* out_exact, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients from grad_out (shape and type of out). out_exact: used in place of
+ * out where given; without it the table's gradient is only as exact as out's
+ * rounding. grad_queries and grad_table
+ * may be NULL; grad_keys and grad_values are both given or both NULL. Needs a
+ * plan made with backward = 1 when grad_keys is given. Sums run in a fixed
+ * order: equal inputs give equal bits. */
+size_t tbvh_attend_blocks_backward_workspace_size(const tbvh_block_geometry* g, const tbvh_attend_features* f);
+int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_features* f, const void* out,
+                                const float* out_exact, const float* lse, const void* grad_out, void* grad_queries,
+                                void* grad_keys, void* grad_values, float* grad_table, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/* Learned bias of neighbour lists by distance bucket:
+ * out[r][h][j] = table[h][number of edges not above d2[r][h][j]] for rows x
+ * heads x k values; per_head 0: d2 is [rows][k], shared by the heads. The
+ * backward entry sums grad_out into grad_table [heads][num_buckets] in a fixed
+ * order. num_buckets 1..64. */
+int tbvh_distance_bias(int device, const float* squared_distances, int64_t rows, int heads, int64_t k, int per_head,
+                       const float* table, const float* edges, int num_buckets, float* out, void* stream);
+size_t tbvh_distance_bias_backward_workspace_size(int64_t rows, int heads, int64_t k, int num_buckets);
+int tbvh_distance_bias_backward(int device, const float* squared_distances, int64_t rows, int heads, int64_t k,
+                                int per_head, const float* edges, int num_buckets, const float* grad_out,
+                                float* grad_table, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

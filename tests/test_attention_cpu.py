@@ -1,0 +1,284 @@
+"""Refusals and host logic of block selection, block attention and the distance
+bias: everything that is checked before any device work."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import torchbvh_b200 as torchbvh
+from torchbvh_b200 import _native
+from torchbvh_b200._attention import BlockSelection
+
+VOID = ctypes.c_void_p
+
+
+def _int64(*values):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+# ---- Python ---------------------------------------------------------------------------------
+
+def test_exports():
+    for name in ("BlockSelection", "select_blocks", "attend_blocks", "distance_bias"):
+        assert name in torchbvh.__all__ and hasattr(torchbvh, name)
+    assert callable(torchbvh.BVH.select_blocks)
+
+
+@pytest.mark.parametrize("n", [0, -1, 33, 2.0, "4"])
+def test_select_rejects_bad_block_counts(n):
+    with pytest.raises(ValueError, match="num_blocks must be 1 to 32"):
+        torchbvh.select_blocks(torchbvh.BVHHandle({}), torch.zeros(4, 3), n)
+
+
+def test_select_rejects_what_is_no_handle():
+    with pytest.raises(TypeError, match="must be a BVHHandle returned by build_bvh"):
+        torchbvh.select_blocks({}, torch.zeros(4, 3), 4)
+
+
+def _handle(n=100, dim=3):
+    return torchbvh.BVHHandle({"node_aabbs": torch.zeros(4, 2 * dim), "sorted_indices": torch.zeros(n, dtype=torch.int64),
+                               "num_leaves": n, "dim": dim})
+
+
+def _batched(b=2, n=100, dim=3):
+    return torchbvh.BatchedBVHHandle({"node_aabbs": torch.zeros(b, 4, 2 * dim), "num_leaves": n, "dim": dim,
+                                      "batch_size": b, "sorted_indices": torch.zeros(b, n, dtype=torch.int64)})
+
+
+def test_select_rejects_bad_queries():
+    with pytest.raises(ValueError, match=r"select_blocks: query_points must have shape \(M, D\)"):
+        torchbvh.select_blocks(_handle(), torch.zeros(2, 4, 3), 4)
+    with pytest.raises(ValueError, match=r"must have shape \(B, M, D\)"):
+        torchbvh.select_blocks(_batched(), torch.zeros(4, 3), 4)
+    with pytest.raises(ValueError, match="last dimension must match BVH dim"):
+        torchbvh.select_blocks(_handle(), torch.zeros(4, 2), 4)
+    with pytest.raises(ValueError, match="query_points must be a CUDA tensor"):
+        torchbvh.select_blocks(_handle(), torch.zeros(4, 3), 4)
+    with pytest.raises(TypeError, match="query_offsets requires a RaggedBVHHandle"):
+        torchbvh.select_blocks(_handle(), torch.zeros(4, 3), 4, query_offsets=torch.tensor([0, 4]))
+    with pytest.raises(ValueError, match="query_offsets is required"):
+        torchbvh.select_blocks(torchbvh.RaggedBVHHandle({}, []), torch.zeros(4, 3), 4)
+
+
+def test_select_rejects_a_destroyed_handle():
+    handle = _handle()
+    torchbvh.destroy_bvh(handle)
+    with pytest.raises(RuntimeError, match="BVH handle has been destroyed"):
+        torchbvh.select_blocks(handle, torch.zeros(4, 3), 4)
+
+
+def _selection(query_shape=(5,), key_shape=(100,), backward=1):
+    fields = {"block_indices": torch.zeros(*query_shape, 4, dtype=torch.int64), "num_blocks": 4}
+    return BlockSelection(fields, _native.BlockGeometry(backward=backward), (), key_shape, query_shape)
+
+
+def _qkv(h=2, kv=2, c=8, dtype=torch.float32, m=5, n=100):
+    return torch.zeros(m, h, c, dtype=dtype), torch.zeros(n, kv, c, dtype=dtype), torch.zeros(n, kv, c, dtype=dtype)
+
+
+def test_attend_rejects_what_is_no_selection():
+    with pytest.raises(TypeError, match="must be a BlockSelection"):
+        torchbvh.attend_blocks({}, *_qkv())
+    gone = _selection()
+    torchbvh.destroy_bvh(gone)
+    with pytest.raises(RuntimeError, match="Block selection has been destroyed"):
+        torchbvh.attend_blocks(gone, *_qkv())
+
+
+def test_attend_rejects_bad_shapes():
+    q, k, v = _qkv()
+    attend = lambda *a, **kw: torchbvh.attend_blocks(_selection(), *a, **kw)
+    with pytest.raises(ValueError, match=r"queries must have shape \(5, H, C\)"):
+        attend(q[:4], k, v)
+    with pytest.raises(ValueError, match=r"queries must have shape"):
+        attend(q[None], k, v)
+    with pytest.raises(ValueError, match=r"keys must have shape \(100, Hkv, C\)"):
+        attend(q, k[:99], v)
+    with pytest.raises(ValueError, match="values must have shape"):
+        attend(q, k, v[..., :4])
+    with pytest.raises(ValueError, match="keys and values must have the same heads"):
+        attend(q, k, v[:, :1])
+    with pytest.raises(ValueError, match="query heads must be a multiple of key heads"):
+        attend(*_qkv(h=3, kv=2))
+    with pytest.raises(ValueError, match="query heads must be a multiple of key heads"):
+        attend(*_qkv(h=0, kv=0))
+    for c in (0, 129):
+        with pytest.raises(ValueError, match="channels must be 1 to 128"):
+            attend(*_qkv(c=c))
+    with pytest.raises(ValueError, match="queries must be a CUDA tensor"):
+        attend(q, k, v)
+
+
+@pytest.mark.parametrize("table, edges, text", [
+    (torch.zeros(2, 4), None, "must be given together"),
+    (None, torch.zeros(3), "must be given together"),
+])
+def test_attend_rejects_half_a_bias(table, edges, text, monkeypatch):
+    # Past the device checks, which need no device for what is refused after them.
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    with pytest.raises(ValueError, match=text):
+        torchbvh.attend_blocks(_selection(), *_qkv(), bias_table=table, bias_edges=edges)
+
+
+def test_attend_rejects_bad_types_biases_and_scales(monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    attend = lambda *a, **kw: torchbvh.attend_blocks(_selection(), *a, **kw)
+    with pytest.raises(ValueError, match="share one type"):
+        attend(*_qkv(dtype=torch.float64))
+    q, k, v = _qkv()
+    with pytest.raises(ValueError, match="share one type"):
+        attend(q, k.half(), v)
+    edges = torch.zeros(3)
+    for table, match in ((torch.zeros(3, 4), r"bias_table must have shape \(H, num_buckets\)"),
+                         (torch.zeros(4), r"bias_table must have shape"),
+                         (torch.zeros(2, 0), "1 to 64 buckets"), (torch.zeros(2, 65), "1 to 64 buckets"),
+                         (torch.zeros(2, 5), r"bias_edges must have shape \(num_buckets - 1,\)"),
+                         (torch.zeros(2, 4).double(), "bias_table must be float32")):
+        with pytest.raises(ValueError, match=match):
+            attend(q, k, v, bias_table=table, bias_edges=edges)
+    for scale in (float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="scale must be finite"):
+            attend(q, k, v, scale=scale)
+
+
+def test_attend_refuses_gradients_without_the_backward_lists(monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    monkeypatch.setattr(BlockSelection, "_used_here", lambda self: None)
+    q, k, v = _qkv()
+    with pytest.raises(ValueError, match="backward=True"):
+        torchbvh.attend_blocks(_selection(backward=0), q.requires_grad_(True), k, v)
+
+
+def test_distance_bias_rejects_bad_arguments(monkeypatch):
+    d2, table, edges = torch.zeros(1, 10, 2, 4), torch.zeros(2, 3), torch.zeros(2)
+    with pytest.raises(ValueError, match="squared_distances must be a CUDA tensor"):
+        torchbvh.distance_bias(d2, table, edges)
+    with pytest.raises(ValueError, match="must have shape"):
+        torchbvh.distance_bias(d2[0, 0], table, edges)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    with pytest.raises(ValueError, match="squared_distances must be float32"):
+        torchbvh.distance_bias(d2.half(), table, edges)
+    with pytest.raises(ValueError, match="head dimension must match table"):
+        torchbvh.distance_bias(d2, torch.zeros(3, 3), edges)
+    with pytest.raises(ValueError, match="at least one head"):
+        torchbvh.distance_bias(d2[:, :, 0], torch.zeros(0, 3), edges)
+    with pytest.raises(ValueError, match="edges must have shape"):
+        torchbvh.distance_bias(d2, table, torch.zeros(3))
+
+
+# ---- C ABI ----------------------------------------------------------------------------------
+
+def test_block_table(native_lib):
+    table = list(_native.block_table([0, 64, 65, 1000], [0, 10, 10, 75]))
+    rows = _native.real_node_count
+    assert table == [0, 64, 0, 0, 10, 0, 0,
+                     64, 1, rows(64), 10, 0, 1, 1,
+                     65, 935, rows(64) + rows(1), 10, 65, 1, 2]
+
+
+@pytest.mark.parametrize("points, queries, text", [
+    ((1, 5), (0, 4), "offsets must start at 0"),
+    ((0, 5), (2, 4), "offsets must start at 0"),
+    ((0, 5, 5), (0, 1, 2), "strictly increasing"),
+    ((0, 5, 6), (0, 2, 1), "must not decrease"),
+])
+def test_block_table_rejects(native_lib, points, queries, text):
+    with pytest.raises(RuntimeError, match=text):
+        _native.block_table(list(points), list(queries))
+    assert native_lib.tbvh_block_table(0, None, None, None) == _native.TBVH_ERR_BAD_ARG
+
+
+def _geometry(**kw):
+    base = dict(device=-1, dim=3, num_blocks=4, backward=0, num_clouds=2, points_per_cloud=1000, queries_per_cloud=70)
+    return _native.BlockGeometry(**{**base, **kw})
+
+
+def _features(**kw):
+    base = dict(dtype=0, heads=4, kv_heads=2, channels=32, scale=1.0, num_buckets=0, queries=16, keys=16, values=16)
+    return _native.AttendFeatures(**{**base, **kw})
+
+
+def test_plan_size(native_lib):
+    size = lambda **kw: native_lib.tbvh_block_plan_size(ctypes.byref(_geometry(**kw)))
+    tiles, entries = 2 * 3, 16  # 32-query tiles; 16 blocks a cloud are fewer than 32 x 4
+    assert size() >= tiles * (32 * 4 + 3 * 32 * 4 + 4 + entries * 8)
+    assert size(backward=1) >= size() + 2 * tiles * entries * 8
+    assert size(points_per_cloud=2**20, num_clouds=1) > size(points_per_cloud=2**12, num_clouds=1)
+    assert size(dim=4) == 0 and size(num_blocks=33) == 0 and size(num_clouds=0) == 0
+    # Offsets past 32 bits are counted in 64.
+    assert size(points_per_cloud=2**30, queries_per_cloud=2**30, num_clouds=1, num_blocks=32) > 2**36
+
+
+@pytest.mark.parametrize("change, text", [
+    ({"dim": 4}, "D must be 2 or 3"),
+    ({"num_blocks": 0}, "num_blocks must be 1 to 32"),
+    ({"num_clouds": 0}, "number of clouds"),
+    ({"points_per_cloud": 2**31}, "total point count"),
+    ({"queries_per_cloud": 2**31 - 1}, "total query count"),
+    ({"queries_per_cloud": -1}, "total query count"),
+    ({"points_per_cloud": 0}, "ragged clouds need a host table"),
+    ({}, "NULL input pointer"),
+])
+def test_select_entry_rejects(native_lib, change, text):
+    rc = native_lib.tbvh_select_blocks(ctypes.byref(_geometry(**change)), 16, 16, None)
+    assert rc == _native.TBVH_ERR_BAD_ARG and text in native_lib.tbvh_last_error().decode()
+
+
+def test_select_entry_rejects_a_small_plan_and_a_foreign_table(native_lib):
+    g = _geometry(node_aabbs=16, sorted_indices=16, plan=16, plan_bytes=64)
+    assert native_lib.tbvh_select_blocks(ctypes.byref(g), 16, 16, None) == _native.TBVH_ERR_WORKSPACE
+    table = _native.block_table([0, 64, 65], [0, 10, 10])
+    table[7] = 63  # the second cloud's first point
+    g = _geometry(points_per_cloud=0, table_host=ctypes.cast(table, VOID), table_dev=16)
+    assert native_lib.tbvh_select_blocks(ctypes.byref(g), 16, 16, None) == _native.TBVH_ERR_BAD_ARG
+    assert "not one of tbvh_block_table" in native_lib.tbvh_last_error().decode()
+    assert native_lib.tbvh_select_blocks(None, 16, 16, None) == _native.TBVH_ERR_BAD_ARG
+
+
+@pytest.mark.parametrize("change, text", [
+    ({"dtype": 3}, "float32, float16 or bfloat16"),
+    ({"heads": 3}, "positive multiple"),
+    ({"heads": 0}, "positive multiple"),
+    ({"kv_heads": 0}, "positive multiple"),
+    ({"heads": 130, "kv_heads": 2}, "at most 64 query heads"),
+    ({"channels": 0}, "channels must be 1 to 128"),
+    ({"channels": 129}, "channels must be 1 to 128"),
+    ({"num_buckets": 65}, "1 to 64 buckets"),
+    ({"num_buckets": 4}, "NULL bias pointer"),
+    ({"keys": None}, "NULL input pointer"),
+])
+def test_attend_entries_reject(native_lib, change, text):
+    g, f = _geometry(), _features(**change)
+    for rc in (native_lib.tbvh_attend_blocks(ctypes.byref(g), ctypes.byref(f), 16, None, None, None, 0, None),
+               native_lib.tbvh_attend_blocks_backward(ctypes.byref(g), ctypes.byref(f), 16, None, 16, 16, 16, None, None,
+                                                      None, 16, 2**40, None)):
+        assert rc == _native.TBVH_ERR_BAD_ARG and text in native_lib.tbvh_last_error().decode()
+
+
+def test_backward_entry_rejects(native_lib):
+    g = _geometry(node_aabbs=16, sorted_indices=16, plan=256, plan_bytes=2**40)
+    call = lambda *a: native_lib.tbvh_attend_blocks_backward(ctypes.byref(g), ctypes.byref(_features()), *a)
+    error = lambda: native_lib.tbvh_last_error().decode()
+    assert call(16, None, 16, 16, 16, 16, None, None, 16, 2**40, None) == _native.TBVH_ERR_BAD_ARG
+    assert "both be given" in error()
+    assert call(16, None, 16, 16, 16, 16, 16, None, 16, 2**40, None) == _native.TBVH_ERR_BAD_ARG
+    assert "without the backward lists" in error()
+    assert call(16, None, 16, 16, 16, None, None, 16, 16, 2**40, None) == _native.TBVH_ERR_BAD_ARG
+    assert "needs a bias" in error()
+    assert call(None, None, 16, 16, 16, None, None, None, 16, 2**40, None) == _native.TBVH_ERR_BAD_ARG
+    assert call(16, None, 16, 16, 16, None, None, None, 16, 64, None) == _native.TBVH_ERR_WORKSPACE
+
+
+def test_distance_bias_entries_reject(native_lib):
+    bias, back = native_lib.tbvh_distance_bias, native_lib.tbvh_distance_bias_backward
+    assert bias(-1, 16, 10, 0, 4, 1, 16, 16, 3, 16, None) == _native.TBVH_ERR_BAD_ARG
+    assert bias(-1, 16, 10, 2, 4, 1, 16, 16, 65, 16, None) == _native.TBVH_ERR_BAD_ARG
+    assert bias(-1, 16, -1, 2, 4, 1, 16, 16, 3, 16, None) == _native.TBVH_ERR_BAD_ARG
+    assert bias(-1, None, 10, 2, 4, 1, 16, 16, 3, 16, None) == _native.TBVH_ERR_BAD_ARG
+    assert bias(-1, 16, 10, 2, 4, 1, 16, None, 3, 16, None) == _native.TBVH_ERR_BAD_ARG
+    assert bias(-1, None, 0, 2, 4, 1, None, None, 3, None, None) == _native.TBVH_OK
+    assert back(-1, 16, 10, 2, 4, 1, 16, 3, 16, 16, None, 0, None) == _native.TBVH_ERR_WORKSPACE
+    assert back(-1, 16, 10, 2, 4, 1, 16, 3, None, 16, 16, 2**30, None) == _native.TBVH_ERR_BAD_ARG
+    assert native_lib.tbvh_distance_bias_backward_workspace_size(10, 2, 4, 0) == 0

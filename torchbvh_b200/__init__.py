@@ -9,6 +9,7 @@ behind it is hand-written CUDA for sm_100a in ``libtorchbvh_b200.so``; there
 is no CPU fallback.
 """
 
+from ._attention import BlockSelection, attend_blocks, distance_bias, select_blocks
 from ._bvh_class import BVH
 from ._constants import SUPPORTED_DIMS, SUPPORTED_K
 from ._handles import BVHHandle, BatchedBVHHandle, RaggedBVHHandle, destroy_bvh
@@ -28,6 +29,10 @@ __all__ = [
     "query_displaced_knn",
     "gather_neighbor_values",
     "interpolate_displaced",
+    "BlockSelection",
+    "select_blocks",
+    "attend_blocks",
+    "distance_bias",
     "device_status",
     "SUPPORTED_K",
     "SUPPORTED_DIMS",

@@ -33,6 +33,17 @@ NVCC_FLAGS = [
 ]
 
 
+# Sources compiled without fast math: block selection, block attention and the
+# distance bias define their scores and buckets by plain float32 rounding.
+PRECISE_SOURCES = ("tbvh_select", "tbvh_attend", "tbvh_bias")
+
+
+def _flags_for(src: Path) -> list[str]:
+    if src.stem.startswith(PRECISE_SOURCES):
+        return [f for f in NVCC_FLAGS if f != "--use_fast_math"]
+    return list(NVCC_FLAGS)
+
+
 def _nvcc() -> str:
     cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     candidate = Path(cuda_home) / "bin" / "nvcc"
@@ -65,11 +76,10 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
     nvcc = _nvcc()
     obj_dir = PACKAGE_DIR / "_build"
     obj_dir.mkdir(exist_ok=True)
-    flags = NVCC_FLAGS + list(extra_flags or [])
 
     def compile_one(src: Path) -> Path:
         obj = obj_dir / (src.stem + ".o")
-        cmd = [nvcc, *flags, "-I", str(INCLUDE), "-I", str(CSRC), "-c", str(src), "-o", str(obj)]
+        cmd = [nvcc, *_flags_for(src), *(extra_flags or []), "-I", str(INCLUDE), "-I", str(CSRC), "-c", str(src), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd), flush=True)
         proc = subprocess.run(cmd, capture_output=True, text=True)

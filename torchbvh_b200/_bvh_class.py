@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import torch
 
+from ._attention import select_blocks
 from ._handles import destroy_bvh
 from ._query import build_bvh, query_knn
 from ._validation import _reject_unless
@@ -52,6 +53,12 @@ class BVH:
         """
         return query_knn(self._handle, query_points, k, query_offsets=query_offsets, source_points=source_points,
                          sort_queries=sort_queries, out=out)
+
+    def select_blocks(self, query_points: torch.Tensor, num_blocks: int, *,
+                      query_offsets: torch.Tensor | None = None, backward: bool = True):
+        """Chooses the nearest blocks of 64 points for every query (see
+        ``select_blocks``), for ``attend_blocks``."""
+        return select_blocks(self._handle, query_points, num_blocks, query_offsets=query_offsets, backward=backward)
 
     def destroy(self) -> None:
         destroy_bvh(self._handle)

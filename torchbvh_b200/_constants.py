@@ -3,6 +3,13 @@
 SUPPORTED_K = (4, 8, 16, 32)
 SUPPORTED_DIMS = (2, 3)
 
+# Block selection and attention: leaves of a block, most blocks of a query, most
+# channels of a head, most buckets of a distance bias.
+BLOCK_SIZE = 64
+MAX_SELECTED_BLOCKS = 32
+MAX_BLOCK_CHANNELS = 128
+MAX_BIAS_BUCKETS = 64
+
 # Squared distance at or below which a neighbour counts as an exact hit in
 # interpolate_displaced, and the inverse-distance weight regulariser
 # (torchbvh/_constants.py:3).

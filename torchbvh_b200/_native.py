@@ -49,6 +49,30 @@ _i64 = ctypes.c_int64
 _ptr = ctypes.c_void_p
 _size = ctypes.c_size_t
 
+class BlockGeometry(ctypes.Structure):
+    """``tbvh_block_geometry``."""
+
+    _fields_ = [
+        ("device", _i32), ("dim", _i32), ("num_blocks", _i32), ("backward", _i32),
+        ("num_clouds", _i64), ("points_per_cloud", _i64), ("queries_per_cloud", _i64),
+        ("table_host", _ptr), ("table_dev", _ptr), ("node_aabbs", _ptr), ("sorted_indices", _ptr),
+        ("query_points", _ptr), ("order", _ptr), ("plan", _ptr), ("plan_bytes", _size),
+    ]
+
+
+class AttendFeatures(ctypes.Structure):
+    """``tbvh_attend_features``."""
+
+    _fields_ = [
+        ("dtype", _i32), ("heads", _i32), ("kv_heads", _i32), ("channels", _i32), ("scale", ctypes.c_float),
+        ("num_buckets", _i32), ("queries", _ptr), ("keys", _ptr), ("values", _ptr), ("bias_table", _ptr),
+        ("bias_edges", _ptr),
+    ]
+
+
+_geometry_p = ctypes.POINTER(BlockGeometry)
+_features_p = ctypes.POINTER(AttendFeatures)
+
 _SIGNATURES = {
     "tbvh_last_error": (ctypes.c_char_p, []),
     "tbvh_abi_version": (_i32, []),
@@ -90,6 +114,20 @@ _SIGNATURES = {
         _i32, [_i32, _ptr, _ptr, _i64, _ptr, _i64, _ptr, _i64, _i32, _i32, _ptr, _ptr, _ptr],
     ),
     "tbvh_widen_indices": (_i32, [_i32, _ptr, _ptr, _i64, _ptr]),
+    "tbvh_block_table": (_i32, [_i64, _ptr, _ptr, _ptr]),
+    "tbvh_block_plan_size": (_size, [_geometry_p]),
+    "tbvh_select_blocks": (_i32, [_geometry_p, _ptr, _ptr, _ptr]),
+    "tbvh_attend_blocks_workspace_size": (_size, [_geometry_p, _features_p]),
+    "tbvh_attend_blocks": (_i32, [_geometry_p, _features_p, _ptr, _ptr, _ptr, _ptr, _size, _ptr]),
+    "tbvh_attend_blocks_backward_workspace_size": (_size, [_geometry_p, _features_p]),
+    "tbvh_attend_blocks_backward": (
+        _i32, [_geometry_p, _features_p, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _size, _ptr],
+    ),
+    "tbvh_distance_bias": (_i32, [_i32, _ptr, _i64, _i32, _i64, _i32, _ptr, _ptr, _i32, _ptr, _ptr]),
+    "tbvh_distance_bias_backward_workspace_size": (_size, [_i64, _i32, _i64, _i32]),
+    "tbvh_distance_bias_backward": (
+        _i32, [_i32, _ptr, _i64, _i32, _i64, _i32, _ptr, _i32, _ptr, _ptr, _ptr, _size, _ptr],
+    ),
     "tbvh_query_knn_gather": (
         _i32,
         [_i32, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _ptr, _i32, _i32, _ptr, _ptr, _ptr, _ptr,
@@ -523,6 +561,110 @@ def query_knn_ragged(packed: dict, query_points: torch.Tensor, query_offsets: to
         for h in hooks:
             h("end", device)
     return (indices, distances) if positions is None else (indices, distances, positions)
+
+
+# ---------------------------------------------------------------------------
+# Block selection, block attention, distance bias (no reference counterpart)
+# ---------------------------------------------------------------------------
+
+_FEATURE_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _data(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def block_table(point_offsets: list[int], query_offsets: list[int]):
+    """Host table of a ragged selection: seven int64 a cloud (tbvh_block_table)."""
+    clouds = len(point_offsets) - 1
+    table = (_i64 * (7 * clouds))()
+    points, queries = (_i64 * (clouds + 1))(*point_offsets), (_i64 * (clouds + 1))(*query_offsets)
+    _check(load_library().tbvh_block_table(clouds, ctypes.cast(points, _ptr), ctypes.cast(queries, _ptr),
+                                           ctypes.cast(table, _ptr)))
+    return table
+
+
+def select_blocks(geometry: BlockGeometry, total_queries: int, device: torch.device):
+    """(block_indices, squared_distances, plan) of ``geometry``, whose plan pointer it sets."""
+    lib = load_library()
+    plan_bytes = int(lib.tbvh_block_plan_size(ctypes.byref(geometry)))
+    plan = _workspace(plan_bytes, device)
+    geometry.plan, geometry.plan_bytes = plan.data_ptr(), plan.numel()
+    shape = (total_queries, geometry.num_blocks)
+    blocks = torch.empty(shape, dtype=torch.int64, device=device)
+    distances = torch.empty(shape, dtype=torch.float32, device=device)
+    _check(lib.tbvh_select_blocks(ctypes.byref(geometry), blocks.data_ptr(), distances.data_ptr(), _stream(device)))
+    # Read by the selection alone; nothing keeps them past this call.
+    geometry.query_points = geometry.order = None
+    return blocks, distances, plan
+
+
+def _attend_features(queries, keys, values, table, edges, scale: float) -> AttendFeatures:
+    return AttendFeatures(_FEATURE_TYPES[queries.dtype], queries.size(-2), keys.size(-2), queries.size(-1), scale,
+                          0 if table is None else table.size(1), queries.data_ptr(), keys.data_ptr(),
+                          values.data_ptr(), _data(table), _data(edges))
+
+
+def attend_blocks(geometry: BlockGeometry, queries, keys, values, table, edges, scale: float, keep_lse: bool,
+                  keep_exact: bool):
+    """(out, lse, out before its rounding to 16 bits); the latter two None unless kept."""
+    lib = load_library()
+    device = queries.device
+    features = _attend_features(queries, keys, values, table, edges, scale)
+    out = torch.empty_like(queries)
+    lse = torch.empty(queries.shape[:-1], dtype=torch.float32, device=device) if keep_lse else None
+    exact = torch.empty(queries.shape, dtype=torch.float32, device=device) if keep_exact else None
+    nbytes = int(lib.tbvh_attend_blocks_workspace_size(ctypes.byref(geometry), ctypes.byref(features)))
+    ws = _workspace(nbytes, device) if nbytes > 256 else None
+    _check(lib.tbvh_attend_blocks(ctypes.byref(geometry), ctypes.byref(features), out.data_ptr(), _data(lse),
+                                  _data(exact), _data(ws), nbytes, _stream(device)))
+    return out, lse, exact
+
+
+def attend_blocks_backward(geometry: BlockGeometry, queries, keys, values, table, edges, scale: float, out,
+                           exact, lse, grad_out, need_queries: bool, need_keys: bool, need_table: bool):
+    """(grad_queries, grad_keys, grad_values, grad_table), None where not needed."""
+    lib = load_library()
+    device = queries.device
+    features = _attend_features(queries, keys, values, table, edges, scale)
+    grad_q = torch.empty_like(queries) if need_queries else None
+    grad_k = torch.empty_like(keys) if need_keys else None
+    grad_v = torch.empty_like(values) if need_keys else None
+    grad_t = torch.empty_like(table) if need_table else None
+    ws = _workspace(lib.tbvh_attend_blocks_backward_workspace_size(ctypes.byref(geometry), ctypes.byref(features)),
+                    device)
+    _check(lib.tbvh_attend_blocks_backward(
+        ctypes.byref(geometry), ctypes.byref(features), _data(out), _data(exact), lse.data_ptr(), grad_out.data_ptr(),
+        _data(grad_q), _data(grad_k), _data(grad_v), _data(grad_t), ws.data_ptr(), ws.numel(), _stream(device)))
+    return grad_q, grad_k, grad_v, grad_t
+
+
+def distance_bias(squared_distances: torch.Tensor, heads: int, per_head: bool, table, edges) -> torch.Tensor:
+    """Bias (..., heads, k) of contiguous squared distances (..., heads, k) or (..., k)."""
+    device = squared_distances.device
+    k = int(squared_distances.size(-1))
+    lead = squared_distances.shape[:-2] if per_head else squared_distances.shape[:-1]
+    rows = lead.numel()
+    out = torch.empty((*lead, heads, k), dtype=torch.float32, device=device)
+    _check(load_library().tbvh_distance_bias(
+        device.index, squared_distances.data_ptr(), rows, heads, k, 1 if per_head else 0, table.data_ptr(),
+        edges.data_ptr(), int(table.size(1)), out.data_ptr(), _stream(device)))
+    return out
+
+
+def distance_bias_backward(squared_distances, heads: int, per_head: bool, edges, grad_out) -> torch.Tensor:
+    """Gradient (heads, buckets) of the bias table."""
+    device = squared_distances.device
+    lib = load_library()
+    k = int(squared_distances.size(-1))
+    rows = (squared_distances.shape[:-2] if per_head else squared_distances.shape[:-1]).numel()
+    buckets = int(edges.numel()) + 1
+    grad = torch.empty((heads, buckets), dtype=torch.float32, device=device)
+    ws = _workspace(lib.tbvh_distance_bias_backward_workspace_size(rows, heads, k, buckets), device)
+    _check(lib.tbvh_distance_bias_backward(
+        device.index, squared_distances.data_ptr(), rows, heads, k, 1 if per_head else 0, edges.data_ptr(), buckets,
+        grad_out.data_ptr(), grad.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device)))
+    return grad
 
 
 # ---------------------------------------------------------------------------

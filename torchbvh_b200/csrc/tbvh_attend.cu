@@ -1,0 +1,279 @@
+// C entries of block attention: argument checks, launch plans, and the small
+// kernels around the two backward passes.
+#include <climits>
+
+#include "tbvh_attend_q.cuh"
+#include "tbvh_kernels.h"
+
+namespace tbvh {
+namespace {
+
+// delta[row][head] = <grad_out, out>, and for float16 the largest |grad_out|
+// (float bits order like unsigned numbers; a maximum has no order of its own).
+// One warp a (row, head).
+template <typename T, typename O>
+__global__ void __launch_bounds__(256) k_delta(const T* grad, const O* out, float* delta, unsigned* most, int64_t rows,
+                                               int channels) {
+  __shared__ unsigned s_most[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = int64_t(blockIdx.x) * 8 + warp;
+  unsigned big = 0;
+  if (row < rows) {
+    float sum = 0.0f;
+    for (int i = lane; i < channels; i += 32) {
+      const float x = Frag<T>::to_float(grad[row * channels + i]);
+      sum = fmaf(x, Frag<O>::to_float(out[row * channels + i]), sum);
+      big = max(big, __float_as_uint(fabsf(x)));
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFullMask, sum, d);
+    if (lane == 0) delta[row] = sum;
+  }
+  if (most == nullptr) return;
+  big = __reduce_max_sync(kFullMask, big);
+  if (lane == 0) s_most[warp] = big;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) big = max(big, s_most[w]);
+    atomicMax(most, big);
+  }
+}
+
+template <typename T>
+cudaError_t run_delta(const void* grad, const void* out, const float* exact, float* delta, unsigned* most,
+                      int64_t pairs, int channels, cudaStream_t stream) {
+  const unsigned grid = unsigned((pairs + 7) / 8);
+  const T* g = static_cast<const T*>(grad);
+  if (exact) k_delta<T, float><<<grid, 256, 0, stream>>>(g, exact, delta, most, pairs, channels);
+  else k_delta<T, T><<<grid, 256, 0, stream>>>(g, static_cast<const T*>(out), delta, most, pairs, channels);
+  count_launches(1);
+  return cudaGetLastError();
+}
+
+size_t pad256(size_t v) { return (v + 255) / 256 * 256; }
+
+struct BackwardSizes {
+  size_t delta, most, part, rows;
+  size_t total() const { return delta + most + part + rows; }
+};
+
+BackwardSizes backward_sizes(const BlockSetup& s, const tbvh_attend_features* f) {
+  BackwardSizes b{};
+  b.delta = pad256(size_t(s.total_queries) * f->heads * 4);
+  b.most = 256;
+  if (f->num_buckets > 0) {
+    b.part = pad256(size_t(s.map.num_tiles) * f->heads * f->num_buckets * 4);
+    b.rows = pad256(size_t(kTableRows) * f->heads * f->num_buckets * 8);
+  }
+  return b;
+}
+
+// Splits of the forward pass: enough thread blocks for two an SM when the tiles
+// alone are fewer, never more than a tile can have entries.
+int forward_splits(const BlockSetup& s, const AttendArgs& a) {
+  const int64_t groups = a.heads_cta >= a.group ? (a.kv_heads + a.kv_cta - 1) / a.kv_cta
+                                                : int64_t(a.kv_heads) * ((a.group + a.heads_cta - 1) / a.heads_cta);
+  const int64_t blocks = s.map.num_tiles * groups;
+  if (blocks <= 0 || blocks >= 148) return 1;
+  int64_t want = (296 + blocks - 1) / blocks;
+  if (want > s.plan.capacity) want = s.plan.capacity;
+  return int(want < 1 ? 1 : want > 32 ? 32 : want);
+}
+
+// Heads of a thread block of the query-tile kernels: at most four (eight warps),
+// key and value rows of at most 256 bytes a leaf (two stages of both then take
+// 64 KB, so that two to three blocks share an SM), and what fits an SM at all.
+void plan_heads(AttendArgs& a, int size, bool back) {
+  const int cp = padded_channels(a.channels);
+  int fit = 256 / (cp * size);
+  if (fit < 1) fit = 1;
+  int kv = a.group > 4 ? 1 : 4 / a.group;
+  if (kv > fit) kv = fit;
+  if (kv > a.kv_heads) kv = a.kv_heads;
+  a.kv_cta = kv;
+  a.heads_cta = a.group > 4 ? 4 : kv * a.group;
+  while (a.heads_cta > 1 && query_tile_smem(size, cp, a.kv_cta, a.heads_cta, back, a.buckets > 0, a.buckets).total >
+                                220 * 1024) {
+    if (a.kv_cta > 1) {
+      --a.kv_cta;
+      a.heads_cta = a.kv_cta * a.group;
+    } else {
+      --a.heads_cta;  // part of a group
+    }
+  }
+}
+
+int check_features(const char* op, const tbvh_attend_features* f, bool pointers) {
+  if (f == nullptr) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: features are NULL", op);
+  if (f->dtype != TBVH_F32 && f->dtype != TBVH_F16 && f->dtype != TBVH_BF16)
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: features must be float32, float16 or bfloat16", op);
+  if (f->heads < 1 || f->kv_heads < 1 || f->heads % f->kv_heads != 0 || f->heads > 4096)
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: heads must be a positive multiple of the key/value heads (at most 4096)", op);
+  if (f->heads / f->kv_heads > 64)
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: at most 64 query heads may share a key/value head", op);
+  if (f->channels < 1 || f->channels > 128)
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: channels must be 1 to 128", op);
+  if (f->num_buckets < 0 || f->num_buckets > kMaxBuckets)
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: the bias has 1 to %d buckets", op, kMaxBuckets);
+  if (!pointers) return TBVH_OK;
+  if (f->num_buckets > 0 && (!f->bias_table || (!f->bias_edges && f->num_buckets > 1)))
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL bias pointer", op);
+  if (!f->keys || !f->values) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL input pointer", op);
+  return TBVH_OK;
+}
+
+int element_size(int dtype) { return dtype == TBVH_F32 ? 4 : 2; }
+
+AttendArgs common_args(const tbvh_block_geometry* g, const tbvh_attend_features* f, const BlockSetup& s,
+                       bool back) {
+  AttendArgs a{};
+  a.map = s.map;
+  a.plan = s.plan;
+  a.aabbs = g->node_aabbs;
+  a.sorted = g->sorted_indices;
+  a.dim = g->dim;
+  a.q = f->queries;
+  a.k = f->keys;
+  a.v = f->values;
+  a.heads = f->heads;
+  a.kv_heads = f->kv_heads;
+  a.channels = f->channels;
+  a.group = f->heads / f->kv_heads;
+  a.scale = f->scale;
+  a.table = f->num_buckets > 0 ? f->bias_table : nullptr;
+  a.edges = f->bias_edges;
+  a.buckets = f->num_buckets;
+  a.status = device_status_ptr();
+  a.splits = 1;
+  plan_heads(a, element_size(f->dtype), back);
+  return a;
+}
+
+bool pairs_aligned(int channels, const void* p) { return channels % 2 == 0 && uintptr_t(p) % 4 == 0; }
+
+}  // namespace
+}  // namespace tbvh
+
+extern "C" {
+
+size_t tbvh_attend_blocks_workspace_size(const tbvh_block_geometry* g, const tbvh_attend_features* f) {
+  using namespace tbvh;
+  BlockSetup s;
+  if (measure_blocks("attend_blocks", g, s) || check_features("attend_blocks", f, false)) return 0;
+  const AttendArgs a = common_args(g, f, s, false);
+  const int splits = forward_splits(s, a);
+  if (splits == 1) return 256;
+  return size_t(splits) * s.map.num_tiles * f->heads * kTileQueries * (2 * padded_channels(f->channels) + 2) * 4;
+}
+
+int tbvh_attend_blocks(const tbvh_block_geometry* g, const tbvh_attend_features* f, void* out, float* lse,
+                       float* out_exact, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace tbvh;
+  const char* op = "attend_blocks";
+  int rc = check_features(op, f, true);
+  if (rc) return rc;
+  BlockSetup s;
+  rc = setup_blocks(op, g, s);
+  if (rc) return rc;
+  if (s.total_queries == 0) return TBVH_OK;
+  if (out_exact && f->dtype == TBVH_F32)
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: out_exact is for 16-bit features (out is float32 already)", op);
+  if (!f->queries || !out) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL query or output pointer", op);
+  AttendArgs a = common_args(g, f, s, false);
+  a.splits = forward_splits(s, a);
+  const size_t need = tbvh_attend_blocks_workspace_size(g, f);
+  if (a.splits > 1 && (workspace == nullptr || workspace_bytes < need))
+    return blocks_fail(TBVH_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the required %zu", op,
+                       workspace_bytes, need);
+  a.width = copy_width(size_t(f->channels) * element_size(f->dtype), f->queries, f->keys, f->values);
+  a.wide_out = pairs_aligned(f->channels, out);
+  a.out = out;
+  a.lse = lse;
+  a.out_exact = out_exact;
+  a.part_row = padded_channels(f->channels) * (out_exact ? 2 : 1) + 2;
+  a.part = static_cast<float*>(workspace);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = launch_attend_forward(a, f->dtype, st);
+  if (e == cudaSuccess && a.splits > 1) e = launch_attend_merge(a, f->dtype, st);
+  return e == cudaSuccess ? TBVH_OK : blocks_cuda_fail(e, op);
+}
+
+size_t tbvh_attend_blocks_backward_workspace_size(const tbvh_block_geometry* g, const tbvh_attend_features* f) {
+  using namespace tbvh;
+  BlockSetup s;
+  if (measure_blocks("attend_blocks_backward", g, s) || check_features("attend_blocks_backward", f, false)) return 0;
+  return backward_sizes(s, f).total();
+}
+
+int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_features* f, const void* out,
+                                const float* out_exact, const float* lse, const void* grad_out, void* grad_queries,
+                                void* grad_keys, void* grad_values, float* grad_table, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  using namespace tbvh;
+  const char* op = "attend_blocks_backward";
+  int rc = check_features(op, f, true);
+  if (rc) return rc;
+  BlockSetup s;
+  rc = setup_blocks(op, g, s);
+  if (rc) return rc;
+  if ((grad_keys == nullptr) != (grad_values == nullptr))
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: grad_keys and grad_values must both be given or both be NULL", op);
+  if (grad_keys && !g->backward)
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: the selection was made without the backward lists", op);
+  if (grad_table && f->num_buckets == 0)
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: grad_table needs a bias", op);
+  if (s.total_queries > 0 && (!f->queries || (!out && !out_exact) || !lse || !grad_out))
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL query, output or gradient pointer", op);
+  const BackwardSizes b = backward_sizes(s, f);
+  if (workspace == nullptr || workspace_bytes < b.total())
+    return blocks_fail(TBVH_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the required %zu", op,
+                       workspace_bytes, b.total());
+  AttendArgs a = common_args(g, f, s, true);
+  char* at = static_cast<char*>(workspace);
+  a.delta = reinterpret_cast<float*>(at);
+  at += b.delta;
+  unsigned* most = reinterpret_cast<unsigned*>(at);
+  at += b.most;
+  float* part = reinterpret_cast<float*>(at);
+  at += b.part;
+  double* rows = reinterpret_cast<double*>(at);
+  a.lse_in = lse;
+  a.grad_out = grad_out;
+  a.grad_q = grad_queries;
+  a.grad_k = grad_keys;
+  a.grad_v = grad_values;
+  a.grad_max = f->dtype == TBVH_F16 ? most : nullptr;
+  a.table_part = grad_table ? part : nullptr;
+  const size_t row_bytes = size_t(f->channels) * element_size(f->dtype);
+  a.width = copy_width(row_bytes, f->queries, f->keys, f->values);
+  const int grad_width = copy_width(row_bytes, grad_out, nullptr, nullptr);
+  if (grad_width < a.width) a.width = grad_width;
+  a.wide_out = (!grad_queries || pairs_aligned(f->channels, grad_queries)) &&
+               (!grad_keys || (pairs_aligned(f->channels, grad_keys) && pairs_aligned(f->channels, grad_values)));
+
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  const int values = f->heads * f->num_buckets;
+  if (s.total_queries > 0) {
+    if (a.grad_max) e = cudaMemsetAsync(most, 0, 4, st);
+    const int64_t pairs = s.total_queries * f->heads;
+    if ((pairs + 7) / 8 > INT_MAX) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: too many query rows", op);
+    if (e == cudaSuccess) {
+      if (f->dtype == TBVH_BF16) e = run_delta<__nv_bfloat16>(grad_out, out, out_exact, a.delta, nullptr, pairs, f->channels, st);
+      else if (f->dtype == TBVH_F16) e = run_delta<__half>(grad_out, out, out_exact, a.delta, most, pairs, f->channels, st);
+      else e = run_delta<float>(grad_out, out, out_exact, a.delta, nullptr, pairs, f->channels, st);
+    }
+    if (e == cudaSuccess && (grad_queries || grad_table)) e = launch_attend_grad_q(a, f->dtype, st);
+  }
+  if (e == cudaSuccess && grad_table) {
+    if (s.total_queries == 0) {
+      e = cudaMemsetAsync(grad_table, 0, size_t(values) * 4, st);
+    } else {
+      e = launch_table_sum(part, rows, grad_table, s.map.num_tiles, values, st);
+    }
+  }
+  if (e == cudaSuccess && grad_keys) e = launch_attend_grad_kv(a, f->dtype, st);
+  return e == cudaSuccess ? TBVH_OK : blocks_cuda_fail(e, op);
+}
+
+}  // extern "C"

@@ -1,0 +1,69 @@
+// Forward pass of block attention (tbvh_attend_q.cuh) and the joining of its
+// splits.
+#include "tbvh_attend_q.cuh"
+#include "tbvh_kernels.h"
+
+namespace tbvh {
+
+cudaError_t launch_attend_forward(const AttendArgs& a, int dtype, cudaStream_t stream) {
+  const cudaError_t e = a.out_exact != nullptr ? launch_attend_forward_exact(a, dtype, stream)
+                                               : run_query_tile_by_type<false, false>(a, dtype, stream);
+  if (e == cudaSuccess) count_launches(1);
+  return e;
+}
+
+namespace {
+
+// Joins the splits of one row: with m = max m_s, l = sum l_s 2^(m_s - m) and
+// o = sum o_s 2^(m_s - m) / l. One warp a row.
+template <typename T>
+__global__ void __launch_bounds__(256) k_merge(AttendArgs a, int cp) {
+  const int64_t tile = blockIdx.x;
+  const int head = blockIdx.y, lane = threadIdx.x & 31;
+  for (int q = threadIdx.x >> 5; q < kTileQueries; q += 8) {
+    const int row = a.plan.query_row[tile * kTileQueries + q];
+    if (row < 0) continue;
+    const int64_t slot = (tile * a.heads + head) * kTileQueries + q;
+    const int64_t stride = a.map.num_tiles * a.heads * kTileQueries;
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part[(s * stride + slot) * a.part_row]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, o[4] = {}, fine[4] = {};
+    const bool exact = a.out_exact != nullptr;
+    for (int s = 0; s < a.splits; ++s) {
+      const float* p = a.part + (s * stride + slot) * a.part_row;
+      const float w = exp2_fast(p[0] - base);
+      sum = fmaf(p[1], w, sum);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (lane + 32 * i < cp) {
+          o[i] = fmaf(p[2 + lane + 32 * i], w, o[i]);
+          if (exact) fine[i] = fmaf(p[2 + cp + lane + 32 * i], w, fine[i]);
+        }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T* out = static_cast<T*>(a.out) + (int64_t(row) * a.heads + head) * a.channels;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (lane + 32 * i < a.channels) {
+        out[lane + 32 * i] = Frag<T>::from_float(o[i] * inv);
+        if (exact) a.out_exact[(int64_t(row) * a.heads + head) * a.channels + lane + 32 * i] = (o[i] + fine[i]) * inv;
+      }
+    }
+    if (a.lse != nullptr && lane == 0) a.lse[int64_t(row) * a.heads + head] = sum == 0.0f ? INFINITY : top + log2f(sum);
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_attend_merge(const AttendArgs& a, int dtype, cudaStream_t stream) {
+  const dim3 grid(unsigned(a.map.num_tiles), unsigned(a.heads));
+  const int cp = padded_channels(a.channels);
+  if (dtype == TBVH_BF16) k_merge<__nv_bfloat16><<<grid, 256, 0, stream>>>(a, cp);
+  else if (dtype == TBVH_F16) k_merge<__half><<<grid, 256, 0, stream>>>(a, cp);
+  else k_merge<float><<<grid, 256, 0, stream>>>(a, cp);
+  count_launches(1);
+  return cudaGetLastError();
+}
+
+}  // namespace tbvh

@@ -1,0 +1,631 @@
+// Block selection: for every query the blocks of 64 leaves whose boxes are
+// nearest, and the plan that block attention reads (tbvh_blocks.h).
+//
+// score(q, j) = sum_a max(lo_ja - q_a, max(q_a - hi_ja, 0))^2, each operation
+// rounded in float32 (no contraction), so that any implementation that rounds
+// the same way selects the same blocks. All steps are monotone: a box inside
+// another never scores lower, in float32 too, which is what makes pruning by
+// the inner nodes exact. Ties go to the lower block: keys are (score bits,
+// block) pairs, and a node's key holds its first block, so a node whose score
+// ties the k-th best is entered only if it could still win by index. Coincident
+// clouds, where every block scores the same, therefore end after k blocks.
+//
+// This file is compiled without fast math: scores keep subnormals.
+#include <climits>
+#include <cstdarg>
+#include <cstdio>
+
+#include "tbvh_blocks.h"
+#include "tbvh_kernels.h"
+
+namespace tbvh {
+
+int blocks_fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return record_error(code, buf);
+}
+
+int blocks_cuda_fail(cudaError_t e, const char* op) {
+  return blocks_fail(TBVH_ERR_CUDA, "%s: CUDA error %s (%s)", op, cudaGetErrorName(e), cudaGetErrorString(e));
+}
+
+namespace {
+
+size_t pad256(size_t v) { return (v + 255) / 256 * 256; }
+
+struct PlanSizes {
+  size_t rows, points, count, entries, begin, bcount, list;
+};
+
+PlanSizes plan_sizes(int64_t tiles, int64_t capacity, int64_t blocks, bool backward) {
+  PlanSizes p{};
+  p.rows = pad256(size_t(tiles) * kTileQueries * sizeof(int));
+  p.points = pad256(size_t(tiles) * 3 * kTileQueries * sizeof(float));
+  p.count = pad256(size_t(tiles) * sizeof(int));
+  p.entries = pad256(size_t(tiles) * size_t(capacity) * sizeof(uint2));
+  if (backward) {
+    p.begin = pad256(size_t(blocks + 1) * sizeof(int64_t));
+    p.bcount = pad256(size_t(blocks) * sizeof(int));
+    p.list = p.entries;
+  }
+  return p;
+}
+
+}  // namespace
+
+size_t block_plan_bytes(int64_t tiles, int64_t capacity, int64_t blocks, bool backward) {
+  const PlanSizes p = plan_sizes(tiles, capacity, blocks, backward);
+  return p.rows + p.points + p.count + p.entries + p.begin + p.bcount + 2 * p.list;
+}
+
+// Sizes only: everything but the pointers.
+int measure_blocks(const char* op, const tbvh_block_geometry* g, BlockSetup& s) {
+  s = BlockSetup{};
+  if (g == nullptr) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: geometry is NULL", op);
+  if (g->dim != 2 && g->dim != 3) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: D must be 2 or 3", op);
+  if (g->num_blocks < 1 || g->num_blocks > kMaxSelect)
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: num_blocks must be 1 to %d", op, kMaxSelect);
+  if (g->num_clouds < 1 || g->num_clouds > INT_MAX)
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: number of clouds must be in [1, 2^31)", op);
+  int64_t most_blocks = 0;
+  BlockMap& map = s.map;
+  map.num_clouds = int(g->num_clouds);
+  if (g->points_per_cloud > 0) {
+    if (g->points_per_cloud > INT_MAX || g->num_clouds * g->points_per_cloud > INT_MAX)
+      return blocks_fail(TBVH_ERR_BAD_ARG, "%s: total point count must fit in signed int32", op);
+    if (g->queries_per_cloud < 0 || g->queries_per_cloud > INT_MAX ||
+        g->num_clouds * g->queries_per_cloud > INT_MAX)
+      return blocks_fail(TBVH_ERR_BAD_ARG, "%s: total query count must fit in signed int32", op);
+    map.n = g->points_per_cloud;
+    map.m = g->queries_per_cloud;
+    map.rows = real_node_count(map.n);
+    map.num_tiles = g->num_clouds * tiles_of(map.m);
+    map.num_blocks = g->num_clouds * blocks_of(map.n);
+    most_blocks = blocks_of(map.n);
+    s.total_points = g->num_clouds * map.n;
+    s.total_queries = g->num_clouds * map.m;
+  } else {
+    const auto* t = reinterpret_cast<const BlockCloud*>(g->table_host);
+    if (t == nullptr) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: ragged clouds need a host table", op);
+    BlockCloud want{};
+    for (int64_t b = 0; b < g->num_clouds; ++b) {
+      const BlockCloud& c = t[b];
+      if (c.n < 1 || c.m < 0 || c.n > INT_MAX || c.m > INT_MAX || c.p0 != want.p0 || c.row0 != want.row0 ||
+          c.q0 != want.q0 || c.t0 != want.t0 || c.b0 != want.b0)
+        return blocks_fail(TBVH_ERR_BAD_ARG, "%s: the host table is not one of tbvh_block_table", op);
+      want.p0 += c.n;
+      want.row0 += real_node_count(c.n);
+      want.q0 += c.m;
+      want.t0 += tiles_of(c.m);
+      want.b0 += blocks_of(c.n);
+      if (want.p0 > INT_MAX) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: total point count must fit in signed int32", op);
+      if (want.q0 > INT_MAX) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: total query count must fit in signed int32", op);
+      if (blocks_of(c.n) > most_blocks) most_blocks = blocks_of(c.n);
+    }
+    map.num_tiles = want.t0;
+    map.num_blocks = want.b0;
+    s.total_points = want.p0;
+    s.total_queries = want.q0;
+  }
+  s.plan.capacity = int64_t(kTileQueries) * g->num_blocks;
+  if (s.plan.capacity > most_blocks) s.plan.capacity = most_blocks;
+  return TBVH_OK;
+}
+
+int setup_blocks(const char* op, const tbvh_block_geometry* g, BlockSetup& s) {
+  int rc = measure_blocks(op, g, s);
+  if (rc) return rc;
+  if (g->points_per_cloud <= 0) {
+    if (g->table_dev == nullptr) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: ragged clouds need a device table", op);
+    s.map.table = reinterpret_cast<const BlockCloud*>(g->table_dev);
+  }
+  if (!g->node_aabbs || !g->sorted_indices)
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL input pointer", op);
+  const PlanSizes p = plan_sizes(s.map.num_tiles, s.plan.capacity, s.map.num_blocks, g->backward != 0);
+  const size_t need = block_plan_bytes(s.map.num_tiles, s.plan.capacity, s.map.num_blocks, g->backward != 0);
+  if (g->plan == nullptr || g->plan_bytes < need)
+    return blocks_fail(TBVH_ERR_WORKSPACE, "%s: plan of %zu bytes is smaller than the required %zu", op, g->plan_bytes,
+                       need);
+  char* at = static_cast<char*>(g->plan);
+  s.plan.query_row = reinterpret_cast<int*>(at);
+  at += p.rows;
+  s.plan.query_point = reinterpret_cast<float*>(at);
+  at += p.points;
+  s.plan.tile_count = reinterpret_cast<int*>(at);
+  at += p.count;
+  s.plan.entries = reinterpret_cast<uint2*>(at);
+  at += p.entries;
+  if (g->backward) {
+    s.plan.block_begin = reinterpret_cast<int64_t*>(at);
+    at += p.begin;
+    s.plan.block_count = reinterpret_cast<int*>(at);
+    at += p.bcount;
+    s.plan.list = reinterpret_cast<uint2*>(at);
+    at += p.list;
+    s.plan.unsorted = reinterpret_cast<uint2*>(at);
+  }
+  if (g->device >= 0) {
+    int cur = -1;
+    if (cudaGetDevice(&cur) != cudaSuccess || cur != g->device) {
+      const cudaError_t e = cudaSetDevice(g->device);
+      if (e != cudaSuccess) return blocks_cuda_fail(e, op);
+    }
+  }
+  return TBVH_OK;
+}
+
+namespace {
+
+struct SelectArgs {
+  BlockMap map;
+  BlockPlan plan;
+  const float* aabbs;
+  const float* queries;
+  const int64_t* order;  // nullable
+  int64_t* out_blocks;
+  float* out_dist;
+  int num;
+  unsigned* status;
+};
+
+constexpr int kSelectStack = 44;  // <= 3 more nodes per two levels, 25 levels at most
+
+template <int D>
+struct Box {
+  float lo[D], hi[D];
+};
+
+template <int D>
+__device__ __forceinline__ Box<D> load_box(const float* rows, int64_t row) {
+  Box<D> b;
+  const float2* p = reinterpret_cast<const float2*>(rows + row * (2 * D));
+  if constexpr (D == 3) {
+    const float2 u = __ldg(p), v = __ldg(p + 1), w = __ldg(p + 2);
+    b.lo[0] = u.x; b.lo[1] = u.y; b.lo[2] = v.x;
+    b.hi[0] = v.y; b.hi[1] = w.x; b.hi[2] = w.y;
+  } else {
+    const float2 u = __ldg(p), v = __ldg(p + 1);
+    b.lo[0] = u.x; b.lo[1] = u.y;
+    b.hi[0] = v.x; b.hi[1] = v.y;
+  }
+  return b;
+}
+
+template <int D>
+__device__ __forceinline__ float box_score(const float* q, const Box<D>& b) {
+  float s = 0.0f;
+#pragma unroll
+  for (int a = 0; a < D; ++a) {
+    const float gap = fmaxf(__fsub_rn(b.lo[a], q[a]), fmaxf(__fsub_rn(q[a], b.hi[a]), 0.0f));
+    const float sq = __fmul_rn(gap, gap);
+    s = a == 0 ? sq : __fadd_rn(s, sq);
+  }
+  return s;
+}
+
+__device__ __forceinline__ uint64_t score_key(float s, uint32_t block) {
+  return (uint64_t(__float_as_uint(s)) << 32) | block;
+}
+
+// One warp a tile. The warp walks the tree as a packet, two levels a step: the
+// (up to four) grandchildren of a node are scored by every lane, those that
+// some lane admits are pushed, the one nearest to most lanes last. A popped
+// node is scored again against the meanwhile lower k-th keys.
+template <int D, int CAP>
+__global__ void __launch_bounds__(32) k_select(SelectArgs a) {
+  __shared__ uint32_t s_stack[kSelectStack];
+  __shared__ int64_t s_row[32];
+  __shared__ uint64_t s_keys[32 * CAP];
+  __shared__ int64_t s_query[32];
+  const int lane = threadIdx.x;
+  const int64_t tile = blockIdx.x;
+  const BlockCloud c = a.map.of_tile(tile);
+  const int64_t pos = (tile - c.t0) * kTileQueries + lane;
+  const int leaf_level = ceil_log2_i64(c.n);
+  const int last = leaf_level > kBlockLevels ? leaf_level - kBlockLevels : 0;  // level of the blocks
+
+  // First node row of every level: exclusive sum of the level counts.
+  {
+    const int64_t count = lane <= leaf_level ? level_count(c.n, leaf_level, lane) : 0;
+    int64_t x = count;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t y = __shfl_up_sync(kFullMask, x, d);
+      if (lane >= d) x += y;
+    }
+    s_row[lane] = c.row0 + x - count;
+  }
+
+  bool active = pos < c.m;
+  int64_t query = -1;
+  if (active) {
+    const int64_t local = a.order ? a.order[c.q0 + pos] : pos;
+    if (local < 0 || local >= c.m) {
+      if (a.status) atomicOr(a.status, kDevErrBadIndex);
+      active = false;
+    } else {
+      query = c.q0 + local;
+    }
+  }
+  s_query[lane] = query;
+  a.plan.query_row[tile * kTileQueries + lane] = int(query);
+  float q[D];
+  bool searching = active;
+#pragma unroll
+  for (int x = 0; x < D; ++x) {
+    q[x] = active ? a.queries[query * D + x] : 0.0f;
+    searching = searching && q[x] == q[x];  // a NaN query selects nothing
+  }
+#pragma unroll
+  for (int x = 0; x < 3; ++x)
+    a.plan.query_point[(tile * 3 + x) * kTileQueries + lane] = x < D ? q[x < D ? x : 0] : 0.0f;
+  // Ascending keys; the first CAP - num slots hold 0 and stay, so the last slot
+  // is the num-th best. Admission: key < last slot.
+  const uint64_t empty = uint64_t(__float_as_uint(kFar)) << 32;
+  uint64_t key[CAP];
+#pragma unroll
+  for (int i = 0; i < CAP; ++i) key[i] = i < CAP - a.num ? 0 : empty;
+  if (!searching) {
+#pragma unroll
+    for (int i = 0; i < CAP; ++i) key[i] = empty;
+  }
+  // A lane that does not search admits nothing: its bound is 0.
+  uint64_t bound = searching ? empty : 0;
+  __syncwarp();
+
+  auto insert = [&](uint64_t x) {
+    if (x < bound) {
+#pragma unroll
+      for (int i = CAP - 1; i > 0; --i) key[i] = x < key[i - 1] ? key[i - 1] : (x < key[i] ? x : key[i]);
+      key[0] = x < key[0] ? x : key[0];
+      bound = key[CAP - 1];
+    }
+  };
+
+  int depth = 0;
+  if (last == 0) {
+    insert(score_key(box_score<D>(q, load_box<D>(a.aabbs, s_row[0])), 0));
+  } else {
+    if (lane == 0) s_stack[0] = 0;
+    depth = 1;
+  }
+  __syncwarp();
+  bool fresh = true;  // the root needs no second look
+  while (depth > 0) {
+    --depth;
+    const uint32_t node = s_stack[depth];
+    __syncwarp();
+    const int level = int(node >> 27);
+    const uint32_t j = node & 0x7ffffffu;
+    if (!fresh) {
+      const float s = box_score<D>(q, load_box<D>(a.aabbs, s_row[level] + j));
+      if (!__any_sync(kFullMask, score_key(s, j << (last - level)) < bound)) continue;
+    }
+    fresh = false;
+    const int step = last - level >= 2 ? 2 : 1;
+    const int child_level = level + step;
+    const uint32_t base = j << step;
+    const int64_t there = level_count(c.n, leaf_level, child_level) - base;
+    const int children = there < (1 << step) ? int(there) : (1 << step);
+    float score[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      score[k] = k < children ? box_score<D>(q, load_box<D>(a.aabbs, s_row[child_level] + base + k)) : kFar;
+    if (child_level == last) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < children) insert(score_key(score[k], base + k));
+      continue;
+    }
+    // Every lane votes for its nearest child that it admits.
+    int nearest = -1;
+    float least = kFar;
+    unsigned admitted = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool ok = k < children && score_key(score[k], (base + k) << (last - child_level)) < bound;
+      if (__any_sync(kFullMask, ok)) admitted |= 1u << k;
+      if (ok && score[k] < least) {
+        least = score[k];
+        nearest = k;
+      }
+    }
+    int votes[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      votes[k] = (admitted >> k & 1u) ? __popc(__ballot_sync(kFullMask, nearest == k)) : -1;
+    if (depth + 4 > kSelectStack) {
+      if (a.status && lane == 0) atomicOr(a.status, kDevErrStackOverflow);
+      break;
+    }
+    // Fewest votes first; among equals the higher child first (popped later).
+#pragma unroll
+    for (int round = 0; round < 4; ++round) {
+      int pick = -1;
+#pragma unroll
+      for (int k = 3; k >= 0; --k)
+        if (votes[k] >= 0 && (pick < 0 || votes[k] < (pick == 3 ? votes[3] : pick == 2 ? votes[2] : votes[1]))) pick = k;
+      if (pick >= 0) {
+        if (lane == 0) s_stack[depth] = (uint32_t(child_level) << 27) | (base + pick);
+        ++depth;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k == pick) votes[k] = -1;
+      }
+    }
+    __syncwarp();
+  }
+
+  // Rows of the result, written a row at a time: slot s of lane r by lane s.
+#pragma unroll
+  for (int i = 0; i < CAP; ++i) s_keys[lane * CAP + i] = key[i];
+  __syncwarp();
+  {
+    int r = lane / a.num, slot = lane % a.num;
+    const int dr = 32 / a.num, ds = 32 % a.num;
+    for (int i = lane; i < 32 * a.num; i += 32) {
+      const int64_t row = s_query[r];
+      if (row >= 0) {
+        const uint64_t k = s_keys[r * CAP + CAP - a.num + slot];
+        const bool none = k >= empty;
+        a.out_blocks[row * a.num + slot] = none ? -1 : int64_t(uint32_t(k));
+        a.out_dist[row * a.num + slot] = none ? kFar : __uint_as_float(uint32_t(k >> 32));
+      }
+      r += dr;
+      slot += ds;
+      if (slot >= a.num) {
+        slot -= a.num;
+        ++r;
+      }
+    }
+  }
+
+  // Union of the lanes' blocks in ascending order: each round takes the least
+  // block above the previous one.
+  uint32_t id[CAP];
+#pragma unroll
+  for (int i = 0; i < CAP; ++i) {
+    const bool real = searching && i >= CAP - a.num && key[i] < empty;
+    id[i] = real ? uint32_t(key[i]) + 1 : 0;  // 0: none
+  }
+  uint32_t done = 0;
+  int count = 0;
+  uint2* entries = a.plan.entries + tile * a.plan.capacity;
+  while (count < a.plan.capacity) {
+    uint32_t next = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < CAP; ++i) next = id[i] > done && id[i] < next ? id[i] : next;
+    const uint32_t least = __reduce_min_sync(kFullMask, next);
+    if (least == 0xffffffffu) break;
+    const unsigned mask = __ballot_sync(kFullMask, next == least);
+    if (lane == 0) {
+      entries[count] = make_uint2(least - 1, mask);
+      if (a.plan.block_count) atomicAdd(a.plan.block_count + c.b0 + (least - 1), 1);
+    }
+    ++count;
+    done = least;
+  }
+  if (lane == 0) a.plan.tile_count[tile] = count;
+}
+
+// Exclusive sums of the block counts (one block of threads; 8 values a thread
+// and step), and the counts set to 0 as fill cursors.
+__global__ void __launch_bounds__(1024) k_block_begin(BlockPlan plan, int64_t blocks) {
+  __shared__ int64_t s_warp[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t carry = 0;
+  for (int64_t at = 0; at < blocks; at += 8 * 1024) {
+    int64_t sum = 0;
+    int v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t j = at + tid * 8 + i;
+      v[i] = j < blocks ? plan.block_count[j] : 0;
+      sum += v[i];
+    }
+    int64_t x = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t y = __shfl_up_sync(kFullMask, x, d);
+      if (lane >= d) x += y;
+    }
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    int64_t before = carry, total = 0;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) {
+      if (w < warp) before += s_warp[w];
+      total += s_warp[w];
+    }
+    before += x - sum;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t j = at + tid * 8 + i;
+      if (j < blocks) {
+        plan.block_begin[j] = before;
+        plan.block_count[j] = 0;
+      }
+      before += v[i];
+    }
+    carry += total;
+    __syncthreads();
+  }
+  if (tid == 0) plan.block_begin[blocks] = carry;
+}
+
+// Every tile's entries into their blocks' runs, in order of arrival (the next
+// kernel puts them in order). One warp a tile.
+__global__ void __launch_bounds__(128) k_block_fill(BlockMap map, BlockPlan plan) {
+  const int64_t tile = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (tile >= map.num_tiles) return;
+  const BlockCloud c = map.of_tile(tile);
+  const uint2* e = plan.entries + tile * plan.capacity;
+  const int count = plan.tile_count[tile];
+  for (int i = threadIdx.x & 31; i < count; i += 32) {
+    const int64_t block = c.b0 + e[i].x;
+    const int64_t at = plan.block_begin[block] + atomicAdd(plan.block_count + block, 1);
+    plan.unsorted[at] = make_uint2(uint32_t(tile), e[i].y);
+  }
+}
+
+// Every block's run by ascending tile, whatever order it arrived in. Short runs
+// are ranked by comparison in shared memory; long ones by a bitmap over the
+// cloud's tiles, a window at a time: a tile's place is the number of set bits
+// below its own.
+constexpr int kOrderThreads = 128;
+constexpr int kOrderShort = 512;
+constexpr int kOrderWords = 2048;  // bitmap window: 65,536 tiles
+
+__global__ void __launch_bounds__(kOrderThreads) k_block_order(BlockMap map, BlockPlan plan) {
+  __shared__ uint32_t s_tile[kOrderShort];
+  __shared__ uint32_t s_bits[kOrderWords];
+  __shared__ int s_before[kOrderWords];
+  __shared__ int s_warp[kOrderThreads / 32];
+  const int tid = threadIdx.x;
+  const int64_t block = blockIdx.x;
+  const int64_t begin = plan.block_begin[block];
+  const int64_t count = plan.block_begin[block + 1] - begin;
+  const uint2* in = plan.unsorted + begin;
+  uint2* out = plan.list + begin;
+  if (count <= kOrderShort) {
+    for (int i = tid; i < count; i += kOrderThreads) s_tile[i] = in[i].x;
+    __syncthreads();
+    for (int i = tid; i < count; i += kOrderThreads) {
+      const uint32_t mine = s_tile[i];
+      int rank = 0;
+      for (int k = 0; k < count; ++k) rank += s_tile[k] < mine;
+      out[rank] = in[i];
+    }
+    return;
+  }
+  const BlockCloud c = map.of_block(block);
+  const int64_t tiles = tiles_of(c.m);
+  int64_t placed = 0;
+  for (int64_t first = 0; first < tiles; first += kOrderWords * 32) {
+    for (int w = tid; w < kOrderWords; w += kOrderThreads) s_bits[w] = 0;
+    __syncthreads();
+    for (int64_t i = tid; i < count; i += kOrderThreads) {
+      const int64_t t = int64_t(in[i].x) - c.t0 - first;
+      if (t >= 0 && t < kOrderWords * 32) atomicOr(s_bits + (t >> 5), 1u << (t & 31));
+    }
+    __syncthreads();
+    // Exclusive popcount sums; thread t owns words [t * per, (t + 1) * per).
+    constexpr int per = kOrderWords / kOrderThreads;
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < per; ++i) sum += __popc(s_bits[tid * per + i]);
+    int x = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(kFullMask, x, d);
+      if ((tid & 31) >= d) x += y;
+    }
+    if ((tid & 31) == 31) s_warp[tid >> 5] = x;
+    __syncthreads();
+    int before = x - sum, total = 0;
+#pragma unroll
+    for (int w = 0; w < kOrderThreads / 32; ++w) {
+      if (w < (tid >> 5)) before += s_warp[w];
+      total += s_warp[w];
+    }
+#pragma unroll
+    for (int i = 0; i < per; ++i) {
+      s_before[tid * per + i] = before;
+      before += __popc(s_bits[tid * per + i]);
+    }
+    __syncthreads();
+    for (int64_t i = tid; i < count; i += kOrderThreads) {
+      const int64_t t = int64_t(in[i].x) - c.t0 - first;
+      if (t >= 0 && t < kOrderWords * 32)
+        out[placed + s_before[t >> 5] + __popc(s_bits[t >> 5] & ((1u << (t & 31)) - 1))] = in[i];
+    }
+    placed += total;
+    __syncthreads();
+  }
+}
+
+template <int D>
+cudaError_t launch_select(const SelectArgs& a, cudaStream_t stream) {
+  const unsigned grid = unsigned(a.map.num_tiles);
+  if (a.num <= 4) k_select<D, 4><<<grid, 32, 0, stream>>>(a);
+  else if (a.num <= 8) k_select<D, 8><<<grid, 32, 0, stream>>>(a);
+  else if (a.num <= 16) k_select<D, 16><<<grid, 32, 0, stream>>>(a);
+  else k_select<D, 32><<<grid, 32, 0, stream>>>(a);
+  count_launches(1);
+  return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace tbvh
+
+extern "C" {
+
+int tbvh_block_table(int64_t num_clouds, const int64_t* point_offsets, const int64_t* query_offsets,
+                     int64_t* table_out) {
+  const char* op = "block_table";
+  if (num_clouds < 1 || !point_offsets || !query_offsets || !table_out)
+    return tbvh::blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL pointer or no clouds", op);
+  if (point_offsets[0] != 0 || query_offsets[0] != 0)
+    return tbvh::blocks_fail(TBVH_ERR_BAD_ARG, "%s: offsets must start at 0", op);
+  auto* t = reinterpret_cast<tbvh::BlockCloud*>(table_out);
+  tbvh::BlockCloud c{};
+  for (int64_t b = 0; b < num_clouds; ++b) {
+    c.n = point_offsets[b + 1] - point_offsets[b];
+    c.m = query_offsets[b + 1] - query_offsets[b];
+    if (c.n < 1) return tbvh::blocks_fail(TBVH_ERR_BAD_ARG, "%s: offsets must be strictly increasing", op);
+    if (c.m < 0) return tbvh::blocks_fail(TBVH_ERR_BAD_ARG, "%s: query offsets must not decrease", op);
+    t[b] = c;
+    c.p0 += c.n;
+    c.row0 += tbvh::real_node_count(c.n);
+    c.q0 += c.m;
+    c.t0 += tbvh::tiles_of(c.m);
+    c.b0 += tbvh::blocks_of(c.n);
+  }
+  return TBVH_OK;
+}
+
+size_t tbvh_block_plan_size(const tbvh_block_geometry* g) {
+  tbvh::BlockSetup s;
+  if (tbvh::measure_blocks("select_blocks", g, s)) return 0;
+  return tbvh::block_plan_bytes(s.map.num_tiles, s.plan.capacity, s.map.num_blocks, g->backward != 0);
+}
+
+int tbvh_select_blocks(const tbvh_block_geometry* g, int64_t* out_blocks, float* out_distances, void* stream) {
+  using namespace tbvh;
+  const char* op = "select_blocks";
+  BlockSetup s;
+  int rc = setup_blocks(op, g, s);
+  if (rc) return rc;
+  if (s.total_queries > 0 && (!g->query_points || !out_blocks || !out_distances))
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL query or output pointer", op);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  if (s.plan.block_count) e = cudaMemsetAsync(s.plan.block_count, 0, size_t(s.map.num_blocks) * sizeof(int), st);
+  if (e == cudaSuccess && s.map.num_tiles > 0) {
+    SelectArgs a{};
+    a.map = s.map;
+    a.plan = s.plan;
+    a.aabbs = g->node_aabbs;
+    a.queries = g->query_points;
+    a.order = g->order;
+    a.out_blocks = out_blocks;
+    a.out_dist = out_distances;
+    a.num = g->num_blocks;
+    a.status = device_status_ptr();
+    e = g->dim == 3 ? launch_select<3>(a, st) : launch_select<2>(a, st);
+  }
+  if (e == cudaSuccess && s.plan.block_count) {
+    k_block_begin<<<1, 1024, 0, st>>>(s.plan, s.map.num_blocks);
+    if (s.map.num_tiles > 0) k_block_fill<<<unsigned((s.map.num_tiles + 3) / 4), 128, 0, st>>>(s.map, s.plan);
+    k_block_order<<<unsigned(s.map.num_blocks), kOrderThreads, 0, st>>>(s.map, s.plan);
+    count_launches(s.map.num_tiles > 0 ? 3 : 2);
+    e = cudaGetLastError();
+  }
+  return e == cudaSuccess ? TBVH_OK : blocks_cuda_fail(e, op);
+}
+
+}  // extern "C"
