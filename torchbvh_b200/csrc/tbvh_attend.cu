@@ -81,19 +81,15 @@ int forward_splits(const BlockSetup& s, const AttendArgs& a) {
 }
 
 // Heads of a thread block of the query-tile kernels: at most four (eight warps),
-// key and value rows of at most 256 bytes a leaf (two stages of both then take
-// 64 KB, so that two to three blocks share an SM), and what fits an SM at all.
+// fewer where two thread blocks would not share an SM's memory.
 void plan_heads(AttendArgs& a, int size, bool back) {
   const int cp = padded_channels(a.channels);
-  int fit = 256 / (cp * size);
-  if (fit < 1) fit = 1;
   int kv = a.group > 4 ? 1 : 4 / a.group;
-  if (kv > fit) kv = fit;
   if (kv > a.kv_heads) kv = a.kv_heads;
   a.kv_cta = kv;
   a.heads_cta = a.group > 4 ? 4 : kv * a.group;
-  while (a.heads_cta > 1 && query_tile_smem(size, cp, a.kv_cta, a.heads_cta, back, a.buckets > 0, a.buckets).total >
-                                220 * 1024) {
+  while (a.heads_cta > 1 &&
+         query_tile_smem(size, cp, a.kv_cta, a.heads_cta, back, a.buckets > 0, a.buckets).total > 110 * 1024) {
     if (a.kv_cta > 1) {
       --a.kv_cta;
       a.heads_cta = a.kv_cta * a.group;

@@ -279,11 +279,11 @@ inline int copy_width(size_t row_bytes, const void* a, const void* b, const void
 }
 
 // Copies rows rows[0..count) (packed row numbers, negative: zeros) of a tensor
-// [row][heads][channels] into tiles dst[head][row][LD], heads first..first +
-// heads_here. Asynchronous for widths of 4 bytes and more.
+// [row][heads][channels] into tiles dst[head][row][LD], heads_here heads from
+// `first`, `step` apart. Asynchronous for widths of 4 bytes and more.
 template <typename T, int CP, int BYTES>
 __device__ __forceinline__ void copy_rows_w(T* dst, int tile_elems, const T* src, const int* rows, int count,
-                                            int heads, int channels, int first, int heads_here) {
+                                            int heads, int channels, int first, int heads_here, int head_step) {
   constexpr int E = BYTES / int(sizeof(T));
   constexpr int LD = Tile<T, CP>::LD;
   const bool full = channels == CP;
@@ -294,7 +294,7 @@ __device__ __forceinline__ void copy_rows_w(T* dst, int tile_elems, const T* src
     const int row = rows[r];
     const T* p = src + (int64_t(row < 0 ? 0 : row) * heads + first) * channels + at;
     T* d = dst + r * LD + at;
-    for (int h = 0; h < heads_here; ++h, p += channels, d += tile_elems) {
+    for (int h = 0; h < heads_here; ++h, p += int64_t(head_step) * channels, d += tile_elems) {
       if constexpr (BYTES >= 4) cp_async<BYTES>(smem_u32(d), p, row >= 0);
       else *d = row >= 0 ? *p : T(0.0f);
     }
@@ -303,12 +303,12 @@ __device__ __forceinline__ void copy_rows_w(T* dst, int tile_elems, const T* src
 
 template <typename T, int CP>
 __device__ __forceinline__ void copy_rows(T* dst, int tile_elems, const T* src, const int* rows, int count, int heads,
-                                          int channels, int first, int heads_here, int width) {
-  if (width == 16) copy_rows_w<T, CP, 16>(dst, tile_elems, src, rows, count, heads, channels, first, heads_here);
-  else if (width == 8) copy_rows_w<T, CP, 8>(dst, tile_elems, src, rows, count, heads, channels, first, heads_here);
-  else if (width == 4) copy_rows_w<T, CP, 4>(dst, tile_elems, src, rows, count, heads, channels, first, heads_here);
+                                          int channels, int first, int heads_here, int width, int step = 1) {
+  if (width == 16) copy_rows_w<T, CP, 16>(dst, tile_elems, src, rows, count, heads, channels, first, heads_here, step);
+  else if (width == 8) copy_rows_w<T, CP, 8>(dst, tile_elems, src, rows, count, heads, channels, first, heads_here, step);
+  else if (width == 4) copy_rows_w<T, CP, 4>(dst, tile_elems, src, rows, count, heads, channels, first, heads_here, step);
   else if constexpr (sizeof(T) == 2)
-    copy_rows_w<T, CP, 2>(dst, tile_elems, src, rows, count, heads, channels, first, heads_here);
+    copy_rows_w<T, CP, 2>(dst, tile_elems, src, rows, count, heads, channels, first, heads_here, step);
 }
 
 // Zeros in the padding channels of tiles that copies never write.
@@ -321,15 +321,19 @@ __device__ __forceinline__ void clear_padding(T* tiles, int rows, int channels) 
 }
 
 // ---- distance buckets --------------------------------------------------------------------
-// bucket(x) = number of edges not above x. Floats of one cell (same exponent and
-// two top mantissa bits) share a table entry: the count at the cell's lower end;
-// the edges inside the cell are then stepped over. Edges that rise by 25 % or
-// more put at most one edge in a cell.
-constexpr int kBucketCells = 1024;
+// bucket(x) = number of edges not above x. A cell holds the floats of one
+// exponent and three top mantissa bits, counted from the smallest positive edge:
+// 511 cells reach 2^63 times that edge, one takes all that is larger. A cell's
+// entry is the count at its lower end and, where one edge lies inside, that
+// edge: a lookup is one read and one comparison. Only where edges are closer
+// than a cell (12 %) are they stepped over one by one.
+constexpr int kBucketCells = 512;
 
 struct BucketTable {
   float edge[kMaxBuckets];  // ascending; unused and NaN edges at the end as NaN (never counted)
-  uint8_t cell[kBucketCells];
+  uint2 cell[kBucketCells]; // count | crowded << 8, bits of the edge inside (NaN: none)
+  int first;                // cell number of cell[0]
+  int not_positive;         // edges that are zero or negative
 
   // All threads of the block; a barrier must follow.
   __device__ void make(const float* edges, int count) {
@@ -340,30 +344,49 @@ struct BucketTable {
     for (int i = threadIdx.x; i < kMaxBuckets; i += blockDim.x) {
       const float x = raw[i];
       int rank = 0;
-      for (int j = 0; j < kMaxBuckets; ++j) {
+      for (int j = 0; j < count; ++j) {
         const float y = raw[j];
-        const bool before = x != x ? (y == y || j < i) : (y < x || (y == x && j < i));
-        rank += before;
+        rank += y != y ? x != x && j < i : x != x || y < x || (y == x && j < i);
       }
+      if (i >= count) rank = i;  // behind every edge
       edge[rank] = x;
     }
     __syncthreads();
+    if (threadIdx.x == 0) {
+      int n = 0;
+      while (n < count && edge[n] <= 0.0f) ++n;
+      not_positive = n;
+      first = n < count && edge[n] == edge[n] ? int(__float_as_uint(edge[n]) >> 20) - 1 : 0;
+    }
+    __syncthreads();
     for (int i = threadIdx.x; i < kBucketCells; i += blockDim.x) {
-      const float low = __uint_as_float(uint32_t(i) << 21);
-      int lo = 0, hi = kMaxBuckets;  // edges [0, lo) are not above low; NaN edges never are
+      const int n = max(first + i, 0);
+      // Edges up to the cell's lower end; cell 0 starts at 0.
+      const float low = i == 0 ? 0.0f : __uint_as_float(uint32_t(n) << 20);
+      const float high = i + 1 == kBucketCells ? INFINITY : __uint_as_float(uint32_t(n + 1) << 20);
+      int lo = 0, hi = count;
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (edge[mid] <= low) lo = mid + 1; else hi = mid;
       }
-      cell[i] = uint8_t(lo);
+      int inside = 0;
+      while (inside < 2 && lo + inside < count && (edge[lo + inside] < high || i + 1 == kBucketCells) &&
+             edge[lo + inside] == edge[lo + inside])
+        ++inside;
+      cell[i] = make_uint2(uint32_t(lo) | (inside > 1 ? 256u : 0u),
+                           __float_as_uint(inside > 0 ? edge[lo] : nan));
     }
   }
   // x >= 0 or NaN (a NaN counts no edge).
   __device__ __forceinline__ int find(float x) const {
-    if (x != x) return 0;
-    int b = cell[__float_as_uint(x) >> 21];
-    while (b < kMaxBuckets && edge[b] <= x) ++b;
-    return b;
+    const int i = min(max(int(__float_as_uint(x) >> 20) - first, 0), kBucketCells - 1);
+    const uint2 c = cell[i];
+    int b = int(c.x) + (x >= __uint_as_float(c.y) ? 1 : 0);
+    if (b >= 256) {  // several edges in the cell
+      b = int(c.x) - 256;
+      while (b < kMaxBuckets && edge[b] <= x) ++b;
+    }
+    return x == x ? b : 0;
   }
   // Any x.
   __device__ __forceinline__ int find_any(float x) const {
@@ -439,6 +462,16 @@ struct HeadSpan {
     }
   }
 };
+
+// float16: the power of two that brings the largest |grad_out| to [1, 2), so that
+// products of small gradients stay normal numbers; taken out again at the end.
+template <typename T>
+__device__ __forceinline__ float gradient_lift(const AttendArgs& a) {
+  if (a.grad_max == nullptr) return 1.0f;
+  const float most = __uint_as_float(*a.grad_max);
+  if (!(most > 0.0f && most <= FLT_MAX)) return 1.0f;
+  return exp2f(-floorf(log2f(most)));
+}
 
 // Packed key row of leaf `leaf` of a cloud, or -1 past its end.
 __device__ __forceinline__ int key_row(const AttendArgs& a, const BlockCloud& c, int64_t leaf) {

@@ -5,12 +5,12 @@
 //   dV = sum p dO;  dK = scale sum dS Q
 //
 // A thread block serves one block of 64 keys and up to two key/value heads;
-// four warps a head, 16 keys each. It walks the block's list of tiles in
+// four warps a head, 16 keys each. It walks the block's list of queries, 32 a
+// step: only those that selected it, so no score is computed in vain, in
 // ascending order, so the sums run in a fixed order without atomics, and over
-// the query heads that share a key/value head. Queries whose mask bit is clear
-// are copied as zeros: non-finite rows of queries that did not select the block
-// never meet it. Every key row belongs to exactly one block, so every gradient
-// row is written once, also for blocks that nobody selected.
+// the query heads that share a key/value head. Every key row belongs to exactly
+// one block, so every gradient row is written once, also for blocks that nobody
+// selected.
 #pragma once
 
 #include "tbvh_attend.cuh"
@@ -84,14 +84,19 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
   const int k_tile = kBlockLeaves * LD, q_tile = kTileQueries * LD;
   const int stage = a.kv_cta * q_tile;
 
-  const int64_t begin = a.plan.block_begin[block];
-  const int entries = int(a.plan.block_begin[block + 1] - begin);
-  const uint2* list = a.plan.list + begin;
+  const int64_t begin = a.plan.query_begin[block];
+  const int listed = int(a.plan.query_begin[block + 1] - begin);
+  const int chunks = (listed + kTileQueries - 1) / kTileQueries;
+  const uint32_t* list = a.plan.list + begin;
   const int64_t leaf0 = (block - c.b0) * kBlockLeaves;
   const int valid = c.n - leaf0 < kBlockLeaves ? int(c.n - leaf0) : kBlockLeaves;
-  // Steps: every entry once for each query head that shares a key/value head.
+  // Steps: every chunk once for each query head that shares a key/value head.
   const int group = a.group;
-  const int64_t steps = int64_t(entries) * group;
+  const int64_t steps = int64_t(chunks) * group;
+  // As in the query-tile kernel.
+  const bool folded = a.scale >= 0x1p-30f && a.scale <= 0x1p30f;
+  const float unit = folded ? a.scale * kLog2e : 1.0f;
+  const float bias_unit = folded ? 1.0f / a.scale : kLog2e;
 
   if (tid < kBlockLeaves) {
     s_krows[tid] = key_row(a, c, leaf0 + tid);
@@ -103,16 +108,20 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
   int next_row = -1;
   float next_pt[3] = {0.0f, 0.0f, 0.0f};
   auto fetch = [&](int e) {
-    if (tid < kTileQueries && e < entries) {
-      const uint2 entry = list[e];
-      next_row = entry.y >> tid & 1u ? a.plan.query_row[int64_t(entry.x) * kTileQueries + tid] : -1;
-      if (bias)
-        for (int x = 0; x < 3; ++x)
-          next_pt[x] = a.plan.query_point[(int64_t(entry.x) * 3 + x) * kTileQueries + tid];
+    if (tid < kTileQueries && e < chunks) {
+      const int at = e * kTileQueries + tid;
+      next_row = -1;
+      if (at < listed) {
+        const uint32_t slot = list[at];
+        next_row = a.plan.query_row[slot];
+        if (bias)
+          for (int x = 0; x < 3; ++x)
+            next_pt[x] = a.plan.query_point[(int64_t(slot / kTileQueries) * 3 + x) * kTileQueries + slot % kTileQueries];
+      }
     }
   };
   auto put = [&](int e) {
-    if (tid < kTileQueries && e < entries) {
+    if (tid < kTileQueries && e < chunks) {
       const int slot = e & 1;
       s_rows[slot * kTileQueries + tid] = next_row;
       if (bias)
@@ -124,31 +133,40 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
       const int slot = int(step & 1);
       const int* rows = s_rows + (e & 1) * kTileQueries;
       // Query heads kv * group + member, one a key/value head.
-      for (int h = 0; h < kvs; ++h) {
-        const int head = (kv0 + h) * group + member;
-        copy_rows<T, CP>(s_q + slot * stage + h * q_tile, q_tile, static_cast<const T*>(a.q), rows, kTileQueries,
-                         a.heads, a.channels, head, 1, a.width);
-        copy_rows<T, CP>(s_d + slot * stage + h * q_tile, q_tile, static_cast<const T*>(a.grad_out), rows,
-                         kTileQueries, a.heads, a.channels, head, 1, a.width);
-      }
+      copy_rows<T, CP>(s_q + slot * stage, q_tile, static_cast<const T*>(a.q), rows, kTileQueries, a.heads, a.channels,
+                       kv0 * group + member, kvs, a.width, group);
+      copy_rows<T, CP>(s_d + slot * stage, q_tile, static_cast<const T*>(a.grad_out), rows, kTileQueries, a.heads,
+                       a.channels, kv0 * group + member, kvs, a.width, group);
       for (int i = tid; i < kvs * kTileQueries; i += blockDim.x) {
         const int h = i / kTileQueries, q = i % kTileQueries, row = rows[q];
         const int64_t at = int64_t(row < 0 ? 0 : row) * a.heads + (kv0 + h) * group + member;
-        cp_async<4>(smem_u32(s_lse + (slot * a.kv_cta + h) * kTileQueries + q), a.lse_in + at, row >= 0);
+        float* lse = s_lse + (slot * a.kv_cta + h) * kTileQueries + q;
+        // Past the list's end the rows are zeros and the sum is infinite: p = 0.
+        if (row >= 0) cp_async<4>(smem_u32(lse), a.lse_in + at, true);
+        else *lse = INFINITY;
         cp_async<4>(smem_u32(s_delta + (slot * a.kv_cta + h) * kTileQueries + q), a.delta + at, row >= 0);
       }
     }
     cp_commit();
   };
+  // Distance buckets of chunk e, times four: a thread has a key and four neighbouring queries.
   auto sort_pairs = [&](int e) {
-    if (bias && e < entries) {
+    if (bias && e < chunks) {
       const int slot = e & 1;
-      const float* p = s_pts + slot * 3 * kTileQueries;
-      for (int i = tid; i < kTileQueries * kBlockLeaves; i += blockDim.x) {
-        const int q = i % kTileQueries, key = i / kTileQueries;
-        const float d = pair_distance(p[q], p[kTileQueries + q], p[2 * kTileQueries + q], s_kpts[key],
-                                      s_kpts[kBlockLeaves + key], s_kpts[2 * kBlockLeaves + key], a.dim == 3);
-        s_buckets[(slot * kBlockLeaves + key) * BROW + q] = uint8_t(min(s_table.find(d), a.buckets - 1));
+      for (int u = tid; u < kTileQueries * kBlockLeaves / 4; u += blockDim.x) {
+        const int key = u / (kTileQueries / 4), q4 = u % (kTileQueries / 4) * 4;
+        const float kx = s_kpts[key], ky = s_kpts[kBlockLeaves + key], kz = s_kpts[2 * kBlockLeaves + key];
+        const float* p = s_pts + slot * 3 * kTileQueries + q4;
+        const float4 px = *reinterpret_cast<const float4*>(p);
+        const float4 py = *reinterpret_cast<const float4*>(p + kTileQueries);
+        const float4 pz = *reinterpret_cast<const float4*>(p + 2 * kTileQueries);
+        const bool three = a.dim == 3;
+        const uint32_t b0 = s_table.find(pair_distance(px.x, py.x, pz.x, kx, ky, kz, three));
+        const uint32_t b1 = s_table.find(pair_distance(px.y, py.y, pz.y, kx, ky, kz, three));
+        const uint32_t b2 = s_table.find(pair_distance(px.z, py.z, pz.z, kx, ky, kz, three));
+        const uint32_t b3 = s_table.find(pair_distance(px.w, py.w, pz.w, kx, ky, kz, three));
+        *reinterpret_cast<uint32_t*>(s_buckets + (slot * kBlockLeaves + key) * BROW + q4) =
+            (b0 | b1 << 8 | b2 << 16 | b3 << 24) << 2;
       }
     }
   };
@@ -161,8 +179,7 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
   put(0);
   if (bias) {
     for (int i = tid; i < kvs * group * a.buckets; i += blockDim.x)
-      s_bias[(i / a.buckets) * kMaxBuckets + i % a.buckets] = a.table[int64_t(kv0) * group * a.buckets + i] * kLog2e;
-    s_table.make(a.edges, a.buckets - 1);
+      s_bias[(i / a.buckets) * kMaxBuckets + i % a.buckets] = a.table[int64_t(kv0) * group * a.buckets + i] * bias_unit;
   }
   __syncthreads();
   copy_rows<T, CP>(s_k, k_tile, static_cast<const T*>(a.k), s_krows, kBlockLeaves, a.kv_heads, a.channels, kv0, kvs,
@@ -172,6 +189,10 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
   copy(0, 0, 0);
   fetch(1);
   put(1);
+  if (bias) {
+    s_table.make(a.edges, a.buckets - 1);
+    __syncthreads();
+  }
   sort_pairs(0);
   cp_wait<0>();
   __syncthreads();
@@ -181,14 +202,7 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
   const int g = lane >> 2, t = lane & 3;
   const T* k_rows = s_k + kv * k_tile;
   const T* v_rows = s_v + kv * k_tile;
-  const float scale = a.scale * kLog2e;
-  float lift = 1.0f;
-  if constexpr (sizeof(T) == 2) {
-    if (a.grad_max != nullptr) {
-      const float most = __uint_as_float(*a.grad_max);
-      if (most > 0.0f && most <= FLT_MAX) lift = exp2f(-floorf(log2f(most)));
-    }
-  }
+  const float lift = gradient_lift<T>(a);
   typename F::A held_k[HOLD], held_v[HOLD];
   if constexpr (HELD) {
     if (mine) {
@@ -197,7 +211,6 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
     }
   }
   float dk[CP / 8][4] = {}, dv[CP / 8][4] = {};
-  const bool there[2] = {quarter * 16 + g < valid, quarter * 16 + g + 8 < valid};
 
   int e = 0, member = 0;
   for (int64_t step = 0; step < steps; ++step) {
@@ -211,35 +224,58 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
     }
     if (mine) {
       const int slot = int(step & 1);
-      const unsigned mask = list[e].y;
       const T* q_rows = s_q + slot * stage + kv * q_tile;
       const T* d_rows = s_d + slot * stage + kv * q_tile;
       const float* lse = s_lse + (slot * a.kv_cta + kv) * kTileQueries + 2 * t;
       const float* delta = s_delta + (slot * a.kv_cta + kv) * kTileQueries + 2 * t;
-      const float* head_bias = s_bias + (kv * group + member) * kMaxBuckets;
+      const char* head_bias = reinterpret_cast<const char*>(s_bias + (kv * group + member) * kMaxBuckets);
       const uint8_t* near = s_buckets + ((e & 1) * kBlockLeaves + quarter * 16 + g) * BROW + 2 * t;
-      float s[NT][4] = {}, ds[NT][4] = {};
-      multiply_nk<T, CP, NT, HELD>(s, held_k, k_rows, quarter * 16, q_rows, 0, lane);
+      float s[NT][4], ds[NT][4] = {};
+      auto read_bias = [&]() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint32_t lo = *reinterpret_cast<const uint16_t*>(near + n * 8);
+          const uint32_t hi = *reinterpret_cast<const uint16_t*>(near + 8 * BROW + n * 8);
+          s[n][0] = *reinterpret_cast<const float*>(head_bias + (lo & 255));
+          s[n][1] = *reinterpret_cast<const float*>(head_bias + (lo >> 8));
+          s[n][2] = *reinterpret_cast<const float*>(head_bias + (hi & 255));
+          s[n][3] = *reinterpret_cast<const float*>(head_bias + (hi >> 8));
+        }
+      };
+      if (bias && folded) {
+        read_bias();
+        multiply_nk<T, CP, NT, HELD>(s, held_k, k_rows, quarter * 16, q_rows, 0, lane);
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[n][j] = 0.0f;
+        multiply_nk<T, CP, NT, HELD>(s, held_k, k_rows, quarter * 16, q_rows, 0, lane);
+        if (!folded) {
+          float x[NT][4];
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              x[n][j] = s[n][j] * (a.scale * kLog2e);
+              s[n][j] = 0.0f;
+            }
+          if (bias) read_bias();
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[n][j] += x[n][j];
+        }
+      }
       multiply_nk<T, CP, NT, HELD>(ds, held_v, v_rows, quarter * 16, d_rows, 0, lane);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float2 l = *reinterpret_cast<const float2*>(lse + n * 8);
         const float2 d = *reinterpret_cast<const float2*>(delta + n * 8);
-        float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (bias) {
-          const uint16_t lo = *reinterpret_cast<const uint16_t*>(near + n * 8);
-          const uint16_t hi = *reinterpret_cast<const uint16_t*>(near + 8 * BROW + n * 8);
-          b[0] = head_bias[lo & 255];
-          b[1] = head_bias[lo >> 8];
-          b[2] = head_bias[hi & 255];
-          b[3] = head_bias[hi >> 8];
-        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool on = there[i >> 1] && (mask >> (n * 8 + 2 * t + (i & 1)) & 1u);
-          const float p = on ? exp2_fast(fmaf(s[n][i], scale, b[i]) - ((i & 1) ? l.y : l.x)) : 0.0f;
-          s[n][i] = p;
-          ds[n][i] = on ? p * (fmaf(ds[n][i], lift, -((i & 1) ? d.y : d.x) * lift)) : 0.0f;
+        for (int j = 0; j < 4; ++j) {
+          s[n][j] = exp2_fast(fmaf(s[n][j], unit, -((j & 1) ? l.y : l.x)));
+          ds[n][j] = s[n][j] * (lift * (ds[n][j] - ((j & 1) ? d.y : d.x)));
         }
       }
       constexpr int STEPS = kTileQueries / F::STEP;

@@ -8,7 +8,7 @@
 // order: spatial neighbours, whose selections mostly agree. The plan lists for
 // every tile the union of its queries' blocks in ascending order, each with a
 // 32-bit mask of the queries that selected it, and (for the backward pass) for
-// every block its tiles in ascending order with the same masks.
+// every block the queries that selected it, in ascending tile order.
 #pragma once
 
 #include <cstddef>
@@ -72,10 +72,12 @@ struct BlockPlan {
   int* tile_count;        // [tiles] entries of each tile
   uint2* entries;         // [tiles][capacity] (block of the cloud, query mask)
   int64_t capacity;       // most entries a tile can have
-  int64_t* block_begin;   // [blocks + 1] first list element of each block   (backward only from here)
-  int* block_count;       // [blocks] elements, then fill cursors
-  uint2* list;            // (tile, query mask) by block, tiles ascending
-  uint2* unsorted;        // the same in arrival order (scratch)
+  int64_t* query_begin;   // [blocks + 1] first list element of each block   (backward only from here)
+  uint32_t* list;         // by block: query slots (32 * tile + lane), ascending
+  int64_t* entry_begin;   // [blocks + 1] first entry of each block in `unsorted`  (scratch from here)
+  int* entry_count;       // [blocks] entries, then fill cursors
+  int* query_count;       // [blocks] queries
+  uint2* unsorted;        // (tile, query mask) by block, in arrival order
 };
 
 // Host-side description of a selection, checked.
@@ -85,7 +87,6 @@ struct BlockSetup {
   int64_t total_points, total_queries;
 };
 
-size_t block_plan_bytes(int64_t tiles, int64_t capacity, int64_t blocks, bool backward);
 // Checks the sizes and fills everything of `s` but the pointers.
 int measure_blocks(const char* op, const tbvh_block_geometry* g, BlockSetup& s);
 // Checks the struct and fills `s`; on failure sets tbvh_last_error() and returns the status.

@@ -38,10 +38,10 @@ namespace {
 size_t pad256(size_t v) { return (v + 255) / 256 * 256; }
 
 struct PlanSizes {
-  size_t rows, points, count, entries, begin, bcount, list;
+  size_t rows, points, count, entries, begin, counts, list, unsorted;
 };
 
-PlanSizes plan_sizes(int64_t tiles, int64_t capacity, int64_t blocks, bool backward) {
+PlanSizes plan_sizes(int64_t tiles, int64_t capacity, int64_t blocks, int64_t picks, bool backward) {
   PlanSizes p{};
   p.rows = pad256(size_t(tiles) * kTileQueries * sizeof(int));
   p.points = pad256(size_t(tiles) * 3 * kTileQueries * sizeof(float));
@@ -49,18 +49,23 @@ PlanSizes plan_sizes(int64_t tiles, int64_t capacity, int64_t blocks, bool backw
   p.entries = pad256(size_t(tiles) * size_t(capacity) * sizeof(uint2));
   if (backward) {
     p.begin = pad256(size_t(blocks + 1) * sizeof(int64_t));
-    p.bcount = pad256(size_t(blocks) * sizeof(int));
-    p.list = p.entries;
+    p.counts = pad256(size_t(blocks) * sizeof(int));
+    p.list = pad256(size_t(picks) * sizeof(uint32_t));
+    p.unsorted = p.entries;
   }
   return p;
 }
 
-}  // namespace
-
-size_t block_plan_bytes(int64_t tiles, int64_t capacity, int64_t blocks, bool backward) {
-  const PlanSizes p = plan_sizes(tiles, capacity, blocks, backward);
-  return p.rows + p.points + p.count + p.entries + p.begin + p.bcount + 2 * p.list;
+size_t plan_total(const PlanSizes& p) {
+  return p.rows + p.points + p.count + p.entries + 2 * p.begin + 2 * p.counts + p.list + p.unsorted;
 }
+
+PlanSizes plan_sizes(const BlockSetup& s, const tbvh_block_geometry* g) {
+  return plan_sizes(s.map.num_tiles, s.plan.capacity, s.map.num_blocks, s.total_queries * g->num_blocks,
+                    g->backward != 0);
+}
+
+}  // namespace
 
 // Sizes only: everything but the pointers.
 int measure_blocks(const char* op, const tbvh_block_geometry* g, BlockSetup& s) {
@@ -125,8 +130,8 @@ int setup_blocks(const char* op, const tbvh_block_geometry* g, BlockSetup& s) {
   }
   if (!g->node_aabbs || !g->sorted_indices)
     return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL input pointer", op);
-  const PlanSizes p = plan_sizes(s.map.num_tiles, s.plan.capacity, s.map.num_blocks, g->backward != 0);
-  const size_t need = block_plan_bytes(s.map.num_tiles, s.plan.capacity, s.map.num_blocks, g->backward != 0);
+  const PlanSizes p = plan_sizes(s, g);
+  const size_t need = plan_total(p);
   if (g->plan == nullptr || g->plan_bytes < need)
     return blocks_fail(TBVH_ERR_WORKSPACE, "%s: plan of %zu bytes is smaller than the required %zu", op, g->plan_bytes,
                        need);
@@ -140,12 +145,16 @@ int setup_blocks(const char* op, const tbvh_block_geometry* g, BlockSetup& s) {
   s.plan.entries = reinterpret_cast<uint2*>(at);
   at += p.entries;
   if (g->backward) {
-    s.plan.block_begin = reinterpret_cast<int64_t*>(at);
+    s.plan.query_begin = reinterpret_cast<int64_t*>(at);
     at += p.begin;
-    s.plan.block_count = reinterpret_cast<int*>(at);
-    at += p.bcount;
-    s.plan.list = reinterpret_cast<uint2*>(at);
+    s.plan.list = reinterpret_cast<uint32_t*>(at);
     at += p.list;
+    s.plan.entry_begin = reinterpret_cast<int64_t*>(at);
+    at += p.begin;
+    s.plan.entry_count = reinterpret_cast<int*>(at);
+    at += p.counts;
+    s.plan.query_count = reinterpret_cast<int*>(at);
+    at += p.counts;
     s.plan.unsorted = reinterpret_cast<uint2*>(at);
   }
   if (g->device >= 0) {
@@ -404,7 +413,10 @@ __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
     const unsigned mask = __ballot_sync(kFullMask, next == least);
     if (lane == 0) {
       entries[count] = make_uint2(least - 1, mask);
-      if (a.plan.block_count) atomicAdd(a.plan.block_count + c.b0 + (least - 1), 1);
+      if (a.plan.entry_count) {
+        atomicAdd(a.plan.entry_count + c.b0 + (least - 1), 1);
+        atomicAdd(a.plan.query_count + c.b0 + (least - 1), __popc(mask));
+      }
     }
     ++count;
     done = least;
@@ -412,11 +424,14 @@ __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
   if (lane == 0) a.plan.tile_count[tile] = count;
 }
 
-// Exclusive sums of the block counts (one block of threads; 8 values a thread
-// and step), and the counts set to 0 as fill cursors.
+// Exclusive sums of the blocks' counts: of entries (thread block 0, which also
+// sets the counts to 0 as fill cursors) and of queries (thread block 1). Eight
+// values a thread and step.
 __global__ void __launch_bounds__(1024) k_block_begin(BlockPlan plan, int64_t blocks) {
   __shared__ int64_t s_warp[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int* counts = blockIdx.x == 0 ? plan.entry_count : plan.query_count;
+  int64_t* begin = blockIdx.x == 0 ? plan.entry_begin : plan.query_begin;
   int64_t carry = 0;
   for (int64_t at = 0; at < blocks; at += 8 * 1024) {
     int64_t sum = 0;
@@ -424,7 +439,7 @@ __global__ void __launch_bounds__(1024) k_block_begin(BlockPlan plan, int64_t bl
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int64_t j = at + tid * 8 + i;
-      v[i] = j < blocks ? plan.block_count[j] : 0;
+      v[i] = j < blocks ? counts[j] : 0;
       sum += v[i];
     }
     int64_t x = sum;
@@ -446,15 +461,15 @@ __global__ void __launch_bounds__(1024) k_block_begin(BlockPlan plan, int64_t bl
     for (int i = 0; i < 8; ++i) {
       const int64_t j = at + tid * 8 + i;
       if (j < blocks) {
-        plan.block_begin[j] = before;
-        plan.block_count[j] = 0;
+        begin[j] = before;
+        if (blockIdx.x == 0) counts[j] = 0;
       }
       before += v[i];
     }
     carry += total;
     __syncthreads();
   }
-  if (tid == 0) plan.block_begin[blocks] = carry;
+  if (tid == 0) begin[blocks] = carry;
 }
 
 // Every tile's entries into their blocks' runs, in order of arrival (the next
@@ -467,53 +482,60 @@ __global__ void __launch_bounds__(128) k_block_fill(BlockMap map, BlockPlan plan
   const int count = plan.tile_count[tile];
   for (int i = threadIdx.x & 31; i < count; i += 32) {
     const int64_t block = c.b0 + e[i].x;
-    const int64_t at = plan.block_begin[block] + atomicAdd(plan.block_count + block, 1);
+    const int64_t at = plan.entry_begin[block] + atomicAdd(plan.entry_count + block, 1);
     plan.unsorted[at] = make_uint2(uint32_t(tile), e[i].y);
   }
 }
 
-// Every block's run by ascending tile, whatever order it arrived in. Short runs
-// are ranked by comparison in shared memory; long ones by a bitmap over the
-// cloud's tiles, a window at a time: a tile's place is the number of set bits
-// below its own.
+// Every block's queries in ascending order, whatever order its entries arrived
+// in. An entry's first place is the number of queries in entries of lower
+// tiles: by comparison in shared memory for short runs; for long ones by a
+// bitmap of the queries of a window of tiles (a tile's word is its mask), whose
+// words are counted.
 constexpr int kOrderThreads = 128;
 constexpr int kOrderShort = 512;
-constexpr int kOrderWords = 2048;  // bitmap window: 65,536 tiles
+constexpr int kOrderWords = 2048;
+
+__device__ __forceinline__ void write_slots(uint32_t* out, uint32_t tile, uint32_t mask) {
+  for (; mask != 0; mask &= mask - 1) *out++ = tile * kTileQueries + (__ffs(mask) - 1);
+}
 
 __global__ void __launch_bounds__(kOrderThreads) k_block_order(BlockMap map, BlockPlan plan) {
-  __shared__ uint32_t s_tile[kOrderShort];
+  __shared__ uint2 s_entry[kOrderShort];
   __shared__ uint32_t s_bits[kOrderWords];
-  __shared__ int s_before[kOrderWords];
   __shared__ int s_warp[kOrderThreads / 32];
   const int tid = threadIdx.x;
   const int64_t block = blockIdx.x;
-  const int64_t begin = plan.block_begin[block];
-  const int64_t count = plan.block_begin[block + 1] - begin;
+  const int64_t begin = plan.entry_begin[block];
+  const int64_t count = plan.entry_begin[block + 1] - begin;
   const uint2* in = plan.unsorted + begin;
-  uint2* out = plan.list + begin;
+  uint32_t* out = plan.list + plan.query_begin[block];
   if (count <= kOrderShort) {
-    for (int i = tid; i < count; i += kOrderThreads) s_tile[i] = in[i].x;
+    for (int i = tid; i < count; i += kOrderThreads) s_entry[i] = in[i];
     __syncthreads();
     for (int i = tid; i < count; i += kOrderThreads) {
-      const uint32_t mine = s_tile[i];
-      int rank = 0;
-      for (int k = 0; k < count; ++k) rank += s_tile[k] < mine;
-      out[rank] = in[i];
+      const uint2 mine = s_entry[i];
+      int before = 0;
+      for (int k = 0; k < count; ++k) {
+        const uint2 e = s_entry[k];
+        before += e.x < mine.x ? __popc(e.y) : 0;
+      }
+      write_slots(out + before, mine.x, mine.y);
     }
     return;
   }
   const BlockCloud c = map.of_block(block);
   const int64_t tiles = tiles_of(c.m);
   int64_t placed = 0;
-  for (int64_t first = 0; first < tiles; first += kOrderWords * 32) {
+  for (int64_t first = 0; first < tiles; first += kOrderWords) {
     for (int w = tid; w < kOrderWords; w += kOrderThreads) s_bits[w] = 0;
     __syncthreads();
     for (int64_t i = tid; i < count; i += kOrderThreads) {
       const int64_t t = int64_t(in[i].x) - c.t0 - first;
-      if (t >= 0 && t < kOrderWords * 32) atomicOr(s_bits + (t >> 5), 1u << (t & 31));
+      if (t >= 0 && t < kOrderWords) s_bits[t] = in[i].y;
     }
     __syncthreads();
-    // Exclusive popcount sums; thread t owns words [t * per, (t + 1) * per).
+    // Exclusive counts; thread t owns words [t * per, (t + 1) * per).
     constexpr int per = kOrderWords / kOrderThreads;
     int sum = 0;
 #pragma unroll
@@ -532,16 +554,10 @@ __global__ void __launch_bounds__(kOrderThreads) k_block_order(BlockMap map, Blo
       if (w < (tid >> 5)) before += s_warp[w];
       total += s_warp[w];
     }
-#pragma unroll
     for (int i = 0; i < per; ++i) {
-      s_before[tid * per + i] = before;
-      before += __popc(s_bits[tid * per + i]);
-    }
-    __syncthreads();
-    for (int64_t i = tid; i < count; i += kOrderThreads) {
-      const int64_t t = int64_t(in[i].x) - c.t0 - first;
-      if (t >= 0 && t < kOrderWords * 32)
-        out[placed + s_before[t >> 5] + __popc(s_bits[t >> 5] & ((1u << (t & 31)) - 1))] = in[i];
+      const uint32_t mask = s_bits[tid * per + i];
+      write_slots(out + placed + before, uint32_t(c.t0 + first + tid * per + i), mask);
+      before += __popc(mask);
     }
     placed += total;
     __syncthreads();
@@ -591,7 +607,7 @@ int tbvh_block_table(int64_t num_clouds, const int64_t* point_offsets, const int
 size_t tbvh_block_plan_size(const tbvh_block_geometry* g) {
   tbvh::BlockSetup s;
   if (tbvh::measure_blocks("select_blocks", g, s)) return 0;
-  return tbvh::block_plan_bytes(s.map.num_tiles, s.plan.capacity, s.map.num_blocks, g->backward != 0);
+  return tbvh::plan_total(tbvh::plan_sizes(s, g));
 }
 
 int tbvh_select_blocks(const tbvh_block_geometry* g, int64_t* out_blocks, float* out_distances, void* stream) {
@@ -604,7 +620,9 @@ int tbvh_select_blocks(const tbvh_block_geometry* g, int64_t* out_blocks, float*
     return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL query or output pointer", op);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
-  if (s.plan.block_count) e = cudaMemsetAsync(s.plan.block_count, 0, size_t(s.map.num_blocks) * sizeof(int), st);
+  if (s.plan.entry_count)  // both counts, side by side
+    e = cudaMemsetAsync(s.plan.entry_count, 0,
+                        size_t(reinterpret_cast<char*>(s.plan.unsorted) - reinterpret_cast<char*>(s.plan.entry_count)), st);
   if (e == cudaSuccess && s.map.num_tiles > 0) {
     SelectArgs a{};
     a.map = s.map;
@@ -618,8 +636,8 @@ int tbvh_select_blocks(const tbvh_block_geometry* g, int64_t* out_blocks, float*
     a.status = device_status_ptr();
     e = g->dim == 3 ? launch_select<3>(a, st) : launch_select<2>(a, st);
   }
-  if (e == cudaSuccess && s.plan.block_count) {
-    k_block_begin<<<1, 1024, 0, st>>>(s.plan, s.map.num_blocks);
+  if (e == cudaSuccess && s.plan.entry_count) {
+    k_block_begin<<<2, 1024, 0, st>>>(s.plan, s.map.num_blocks);
     if (s.map.num_tiles > 0) k_block_fill<<<unsigned((s.map.num_tiles + 3) / 4), 128, 0, st>>>(s.map, s.plan);
     k_block_order<<<unsigned(s.map.num_blocks), kOrderThreads, 0, st>>>(s.map, s.plan);
     count_launches(s.map.num_tiles > 0 ? 3 : 2);
