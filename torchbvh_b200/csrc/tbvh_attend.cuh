@@ -27,6 +27,50 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Pairs of float32 in one 64-bit register: two results an instruction, each
+// rounded as the scalar one's.
+using Pair = uint64_t;
+__device__ __forceinline__ Pair pair(float x, float y) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ Pair both(float x) { return pair(x, x); }
+__device__ __forceinline__ float2 unpair(Pair p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// acc[j] = acc[j] * factor + part[j] where `on`, untouched elsewhere.
+__device__ __forceinline__ void keep_where(Pair& a0, Pair& a1, Pair& a2, Pair& a3, Pair factor, Pair p0, Pair p1,
+                                           Pair p2, Pair p3, uint32_t on) {
+  asm("{.reg .pred p;\n setp.ne.u32 p, %9, 0;\n"
+      "@p fma.rn.f32x2 %0, %0, %4, %5;\n @p fma.rn.f32x2 %1, %1, %4, %6;\n"
+      "@p fma.rn.f32x2 %2, %2, %4, %7;\n @p fma.rn.f32x2 %3, %3, %4, %8;}"
+      : "+l"(a0), "+l"(a1), "+l"(a2), "+l"(a3)
+      : "l"(factor), "l"(p0), "l"(p1), "l"(p2), "l"(p3), "r"(on));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
 
 template <int BYTES>
@@ -57,15 +101,24 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
                : "memory");
 }
 
+__device__ __forceinline__ float lds_f32(uint32_t addr) {
+  float x;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
+  return x;
+}
+
 // ---- matrix fragments ---------------------------------------------------------------
 // Frag<T> multiplies 16 x STEP by STEP x 8 into a float accumulator c[4]: lane
 // (g = lane / 4, t = lane % 4) holds rows g and g + 8, columns 2t and 2t + 1.
 //
-// Tiles in shared memory are row-major with LD elements a row (see Tile).
+// Operands come from row-major tiles in shared memory, `rs` bytes a row (see
+// row_bytes). Each load takes the byte address of its first element plus the
+// lane's own offset, which does not change: lane_a / lane_nk / lane_kn.
 //  load_a      A from rows of a tile (row = output row, column = depth)
 //  pair_nk     B for two neighbouring n-tiles from a tile stored [n][depth]
 //  pair_kn     B for two neighbouring n-tiles from a tile stored [depth][n]
 //  from_acc    A from an accumulator tile whose columns are the depth
+//  mma_first   mma into zeros
 template <typename T>
 struct Frag;
 
@@ -79,18 +132,16 @@ struct Frag16 {
   };
   using B = uint32_t[4];  // two n-tiles
 
-  __device__ static __forceinline__ void load_a(A& a, const T* tile, int ld, int row, int k, int lane) {
-    const int m = lane >> 3, r = lane & 7;
-    ldmatrix4(a.r, smem_u32(tile + (row + (m & 1) * 8 + r) * ld + k + (m >> 1) * 8));
+  __device__ static __forceinline__ uint32_t lane_a(uint32_t rs, int lane) {
+    return ((lane >> 3 & 1) * 8 + (lane & 7)) * rs + (lane >> 4) * 16;
   }
-  __device__ static __forceinline__ void pair_nk(B& b, const T* tile, int ld, int n, int k, int lane) {
-    const int m = lane >> 3, r = lane & 7;
-    ldmatrix4(b, smem_u32(tile + (n + (m >> 1) * 8 + r) * ld + k + (m & 1) * 8));
+  __device__ static __forceinline__ uint32_t lane_nk(uint32_t rs, int lane) {
+    return ((lane >> 4) * 8 + (lane & 7)) * rs + (lane >> 3 & 1) * 16;
   }
-  __device__ static __forceinline__ void pair_kn(B& b, const T* tile, int ld, int k, int n, int lane) {
-    const int m = lane >> 3, r = lane & 7;
-    ldmatrix4_t(b, smem_u32(tile + (k + (m & 1) * 8 + r) * ld + n + (m >> 1) * 8));
-  }
+  __device__ static __forceinline__ uint32_t lane_kn(uint32_t rs, int lane) { return lane_a(rs, lane); }
+  __device__ static __forceinline__ void load_a(A& a, uint32_t at, uint32_t) { ldmatrix4(a.r, at); }
+  __device__ static __forceinline__ void pair_nk(B& b, uint32_t at, uint32_t) { ldmatrix4(b, at); }
+  __device__ static __forceinline__ void pair_kn(B& b, uint32_t at, uint32_t) { ldmatrix4_t(b, at); }
 };
 
 template <>
@@ -107,6 +158,13 @@ struct Frag<__nv_bfloat16> : Frag16<__nv_bfloat16> {
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  __device__ static __forceinline__ void mma_first(float (&c)[4], const Frag16<__nv_bfloat16>::A& a, uint32_t b0,
+                                                   uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
   }
   __device__ static __forceinline__ float2 unpack(uint32_t x) {
     return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
@@ -129,6 +187,13 @@ struct Frag<__half> : Frag16<__half> {
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  __device__ static __forceinline__ void mma_first(float (&c)[4], const Frag16<__half>::A& a, uint32_t b0,
+                                                   uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
   }
   __device__ static __forceinline__ float2 unpack(uint32_t x) {
     return __half22float2(*reinterpret_cast<const __half2*>(&x));
@@ -156,28 +221,32 @@ struct Frag<float> {
     // An infinity or NaN is carried by the high part alone.
     if (!(fabsf(x) <= FLT_MAX)) lo = 0;
   }
-  __device__ static __forceinline__ void load_a(A& a, const float* tile, int ld, int row, int k, int lane) {
-    const float* p = tile + (row + (lane >> 2)) * ld + k + (lane & 3);
-    split(p[0], a.hi[0], a.lo[0]);
-    split(p[8 * ld], a.hi[1], a.lo[1]);
-    split(p[4], a.hi[2], a.lo[2]);
-    split(p[8 * ld + 4], a.hi[3], a.lo[3]);
+  __device__ static __forceinline__ uint32_t lane_a(uint32_t rs, int lane) {
+    return (lane >> 2) * rs + (lane & 3) * 4;
   }
-  __device__ static __forceinline__ void pair_nk(B& b, const float* tile, int ld, int n, int k, int lane) {
-    const float* p = tile + (n + (lane >> 2)) * ld + k + (lane & 3);
-    b[0] = p[0];
-    b[1] = p[4];
-    b[2] = p[8 * ld];
-    b[3] = p[8 * ld + 4];
+  __device__ static __forceinline__ uint32_t lane_nk(uint32_t rs, int lane) { return lane_a(rs, lane); }
+  __device__ static __forceinline__ uint32_t lane_kn(uint32_t rs, int lane) {
+    return 2 * (lane & 3) * rs + (lane >> 2) * 4;
+  }
+  __device__ static __forceinline__ void load_a(A& a, uint32_t at, uint32_t rs) {
+    split(lds_f32(at), a.hi[0], a.lo[0]);
+    split(lds_f32(at + 8 * rs), a.hi[1], a.lo[1]);
+    split(lds_f32(at + 16), a.hi[2], a.lo[2]);
+    split(lds_f32(at + 8 * rs + 16), a.hi[3], a.lo[3]);
+  }
+  __device__ static __forceinline__ void pair_nk(B& b, uint32_t at, uint32_t rs) {
+    b[0] = lds_f32(at);
+    b[1] = lds_f32(at + 16);
+    b[2] = lds_f32(at + 8 * rs);
+    b[3] = lds_f32(at + 8 * rs + 16);
   }
   // Depth t of the instruction is row 2t of the tile and depth t + 4 row
   // 2t + 1: the order in which from_acc finds an accumulator's columns.
-  __device__ static __forceinline__ void pair_kn(B& b, const float* tile, int ld, int k, int n, int lane) {
-    const float* p = tile + (k + 2 * (lane & 3)) * ld + n + (lane >> 2);
-    b[0] = p[0];
-    b[1] = p[ld];
-    b[2] = p[8];
-    b[3] = p[ld + 8];
+  __device__ static __forceinline__ void pair_kn(B& b, uint32_t at, uint32_t rs) {
+    b[0] = lds_f32(at);
+    b[1] = lds_f32(at + rs);
+    b[2] = lds_f32(at + 32);
+    b[3] = lds_f32(at + rs + 32);
   }
   __device__ static __forceinline__ void mma1(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -192,6 +261,10 @@ struct Frag<float> {
     mma1(c, a.lo, h0, h1);
     mma1(c, a.hi, l0, l1);
     mma1(c, a.hi, h0, h1);
+  }
+  __device__ static __forceinline__ void mma_first(float (&c)[4], const A& a, float b0, float b1) {
+    c[0] = c[1] = c[2] = c[3] = 0.0f;
+    mma(c, a, b0, b1);
   }
   __device__ static __forceinline__ float to_float(float x) { return x; }
   __device__ static __forceinline__ float from_float(float x) { return x; }
@@ -229,40 +302,46 @@ __device__ __forceinline__ void rest_of_acc(typename Frag<T>::A& rest, const typ
 }
 
 // ---- tiles in shared memory -----------------------------------------------------------
-// Rows of CP elements (the channels rounded up) and 16 bytes of padding, which
-// puts the eight rows that a fragment load touches at once into different banks.
+// [row][head][CP channels], CP the channels rounded up, and 16 bytes of padding
+// a row: an odd number of 16-byte words, which puts the eight rows that a
+// fragment load touches at once into different banks. A row of whole heads is
+// one run of memory in the caller's tensor as well.
 template <typename T, int CP>
-struct Tile {
-  static constexpr int LD = CP + 16 / int(sizeof(T));
-  __host__ __device__ static constexpr int elems(int rows) { return rows * LD; }
-};
+__host__ __device__ constexpr uint32_t row_bytes(int heads) {
+  return uint32_t(heads) * CP * sizeof(T) + 16;
+}
 
-// acc[NT][4] += A(16 rows of `a_tile` from `row`) x B^T, B stored [n][channel], n from n0.
-template <typename T, int CP, int NT, bool HELD>
-__device__ __forceinline__ void multiply_nk(float (&acc)[NT][4], const typename Frag<T>::A* held, const T* a_tile,
-                                            int row, const T* b_tile, int n0, int lane) {
-  constexpr int LD = Tile<T, CP>::LD;
+// acc[NT][4] += (FRESH: =) A(16 rows) x B^T, B stored [n][channel]. `a` and `b`
+// include the lane's offset.
+template <typename T, int CP, int NT, bool HELD, bool FRESH>
+__device__ __forceinline__ void multiply_nk(float (&acc)[NT][4], const typename Frag<T>::A* held, uint32_t a,
+                                            uint32_t a_rs, uint32_t b, uint32_t b_rs) {
 #pragma unroll
   for (int s = 0; s < CP / Frag<T>::STEP; ++s) {
+    const uint32_t depth = s * Frag<T>::STEP * sizeof(T);
     typename Frag<T>::A fresh;
-    if constexpr (!HELD) Frag<T>::load_a(fresh, a_tile, LD, row, s * Frag<T>::STEP, lane);
-    const typename Frag<T>::A& a = HELD ? held[HELD ? s : 0] : fresh;
+    if constexpr (!HELD) Frag<T>::load_a(fresh, a + depth, a_rs);
+    const typename Frag<T>::A& x = HELD ? held[HELD ? s : 0] : fresh;
 #pragma unroll
     for (int j = 0; j < NT / 2; ++j) {
-      typename Frag<T>::B b;
-      Frag<T>::pair_nk(b, b_tile, LD, n0 + j * 16, s * Frag<T>::STEP, lane);
-      Frag<T>::mma(acc[2 * j], a, b[0], b[1]);
-      Frag<T>::mma(acc[2 * j + 1], a, b[2], b[3]);
+      typename Frag<T>::B y;
+      Frag<T>::pair_nk(y, b + j * 16 * b_rs + depth, b_rs);
+      if (FRESH && s == 0) {
+        Frag<T>::mma_first(acc[2 * j], x, y[0], y[1]);
+        Frag<T>::mma_first(acc[2 * j + 1], x, y[2], y[3]);
+      } else {
+        Frag<T>::mma(acc[2 * j], x, y[0], y[1]);
+        Frag<T>::mma(acc[2 * j + 1], x, y[2], y[3]);
+      }
     }
   }
 }
 
 // The fragments of an A operand that stays in registers.
 template <typename T, int CP>
-__device__ __forceinline__ void hold(typename Frag<T>::A* held, const T* a_tile, int row, int lane) {
+__device__ __forceinline__ void hold(typename Frag<T>::A* held, uint32_t a, uint32_t rs) {
 #pragma unroll
-  for (int s = 0; s < CP / Frag<T>::STEP; ++s)
-    Frag<T>::load_a(held[s], a_tile, Tile<T, CP>::LD, row, s * Frag<T>::STEP, lane);
+  for (int s = 0; s < CP / Frag<T>::STEP; ++s) Frag<T>::load_a(held[s], a + s * Frag<T>::STEP * sizeof(T), rs);
 }
 
 // Channel tiles are multiplied in groups of this many so that the partial
@@ -271,75 +350,119 @@ constexpr int kChannelGroup = 4;
 
 // ---- row copies ------------------------------------------------------------------------
 // Widest copy that channels * size and the addresses allow: 16, 8, 4 or 2 bytes.
-inline int copy_width(size_t row_bytes, const void* a, const void* b, const void* c) {
-  const uintptr_t all = uintptr_t(a) | uintptr_t(b) | uintptr_t(c) | uintptr_t(row_bytes);
+inline int copy_width(size_t bytes, const void* a, const void* b, const void* c) {
+  const uintptr_t all = uintptr_t(a) | uintptr_t(b) | uintptr_t(c) | uintptr_t(bytes);
   for (int w = 16; w > 2; w >>= 1)
     if (all % w == 0) return w;
   return 2;
 }
 
-// Copies rows rows[0..count) (packed row numbers, negative: zeros) of a tensor
-// [row][heads][channels] into tiles dst[head][row][LD], heads_here heads from
-// `first`, `step` apart. Asynchronous for widths of 4 bytes and more.
-template <typename T, int CP, int BYTES>
-__device__ __forceinline__ void copy_rows_w(T* dst, int tile_elems, const T* src, const int* rows, int count,
-                                            int heads, int channels, int first, int heads_here, int head_step) {
-  constexpr int E = BYTES / int(sizeof(T));
-  constexpr int LD = Tile<T, CP>::LD;
-  const bool full = channels == CP;
-  const int per = full ? CP / E : channels / E;
-  for (int i = threadIdx.x; i < count * per; i += blockDim.x) {
-    const int r = full ? i / (CP / E) : i / per;
-    const int at = (i - r * per) * E;
-    const int row = rows[r];
-    const T* p = src + (int64_t(row < 0 ? 0 : row) * heads + first) * channels + at;
-    T* d = dst + r * LD + at;
-    for (int h = 0; h < heads_here; ++h, p += int64_t(head_step) * channels, d += tile_elems) {
-      if constexpr (BYTES >= 4) cp_async<BYTES>(smem_u32(d), p, row >= 0);
-      else *d = row >= 0 ? *p : T(0.0f);
+// Copies rows of a tensor [row][heads][channels], `here` heads from `first`,
+// `step` apart, into a tile; row_of(r) is the packed row number of tile row r,
+// negative for zeros. All threads take part; asynchronous for widths of 4 bytes
+// and more.
+template <typename T, int CP>
+struct Rows {
+  const T* src;
+  int heads, channels, first, here, step, width;
+  uint32_t rs;
+
+  template <int BYTES, typename RowOf>
+  __device__ __forceinline__ void part(uint32_t dst, int count, RowOf row_of) const {
+    constexpr int E = BYTES / int(sizeof(T));
+    const int per = channels / E;
+    for (int i = threadIdx.x; i < count * per; i += blockDim.x) {
+      const int r = i / per, at = (i - r * per) * E, row = row_of(r);
+      const T* p = src + (int64_t(row < 0 ? 0 : row) * heads + first) * channels + at;
+      uint32_t d = dst + r * rs + at * uint32_t(sizeof(T));
+      for (int h = 0; h < here; ++h, p += int64_t(step) * channels, d += CP * sizeof(T)) {
+        if constexpr (BYTES >= 4) {
+          cp_async<BYTES>(d, p, row >= 0);
+        } else {
+          const uint16_t x = row >= 0 ? *reinterpret_cast<const uint16_t*>(p) : uint16_t(0);
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(d), "h"(x) : "memory");
+        }
+      }
     }
   }
+  template <typename RowOf>
+  __device__ __forceinline__ void copy(uint32_t dst, int count, RowOf row_of) const {
+    if (width == 16) part<16>(dst, count, row_of);
+    else if (width == 8) part<8>(dst, count, row_of);
+    else if (width == 4) part<4>(dst, count, row_of);
+    else if constexpr (sizeof(T) == 2) part<2>(dst, count, row_of);
+  }
+};
+
+// The copy of every step, two tensors of one shape at a time, where a row's
+// heads are one run of whole 16-byte words on both sides: a thread keeps one
+// word of the row and every `at_once`-th row, and finds the row's place in the
+// tensors, in bytes, in shared memory (row_place). (Bulk copies of a row each
+// were measured at 1.7 times this form's step: one thread issues them one by one.)
+struct RowWords {
+  uint32_t dst, dst_step;
+  int row0, at_once;  // at_once 0: not this shape
+  const char *a, *b;
+
+  __device__ __forceinline__ RowWords(const void* a_, const void* b_, int size, int cp, int channels, int first, int here,
+                                      int step, int width, uint32_t rs) {
+    const int columns = here * cp * size / 16, column = int(threadIdx.x) % columns;
+    at_once = width == 16 && channels == cp && (step == 1 || here == 1) ? int(blockDim.x) / columns : 0;
+    row0 = int(threadIdx.x) / columns;
+    dst = row0 * rs + column * 16;
+    dst_step = at_once * rs;
+    if (row0 >= at_once) row0 = 1 << 20;  // no row
+    const int64_t begin = int64_t(first) * cp * size + column * 16;
+    a = static_cast<const char*>(a_) + begin;
+    b = static_cast<const char*>(b_) + begin;
+  }
+  __device__ __forceinline__ void copy(uint32_t a_tile, uint32_t b_tile, const uint64_t* places, int count) const {
+    uint32_t to = dst;
+    for (int r = row0; r < count; r += at_once, to += dst_step) {
+      const uint64_t place = places[r];
+      const int size = place & 1 ? 0 : 16;
+      const uint64_t at = place & ~uint64_t(1);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(a_tile + to), "l"(a + at), "r"(size) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(b_tile + to), "l"(b + at), "r"(size) : "memory");
+    }
+  }
+};
+
+// Bytes from a tensor's start to row `row` of `row_bytes` (a multiple of 16); odd: a row of zeros.
+__device__ __forceinline__ uint64_t row_place(int row, uint32_t row_bytes) {
+  return row < 0 ? 1 : uint64_t(uint32_t(row)) * row_bytes;
 }
 
+// Zeros in the padding channels of tiles, which copies never write.
 template <typename T, int CP>
-__device__ __forceinline__ void copy_rows(T* dst, int tile_elems, const T* src, const int* rows, int count, int heads,
-                                          int channels, int first, int heads_here, int width, int step = 1) {
-  if (width == 16) copy_rows_w<T, CP, 16>(dst, tile_elems, src, rows, count, heads, channels, first, heads_here, step);
-  else if (width == 8) copy_rows_w<T, CP, 8>(dst, tile_elems, src, rows, count, heads, channels, first, heads_here, step);
-  else if (width == 4) copy_rows_w<T, CP, 4>(dst, tile_elems, src, rows, count, heads, channels, first, heads_here, step);
-  else if constexpr (sizeof(T) == 2)
-    copy_rows_w<T, CP, 2>(dst, tile_elems, src, rows, count, heads, channels, first, heads_here, step);
-}
-
-// Zeros in the padding channels of tiles that copies never write.
-template <typename T, int CP>
-__device__ __forceinline__ void clear_padding(T* tiles, int rows, int channels) {
+__device__ __forceinline__ void clear_padding(char* tile, uint32_t rs, int rows, int heads, int channels) {
   if (channels == CP) return;
-  constexpr int LD = Tile<T, CP>::LD;
   const int pad = CP - channels;
-  for (int i = threadIdx.x; i < rows * pad; i += blockDim.x) tiles[(i / pad) * LD + channels + i % pad] = T(0.0f);
+  for (int i = threadIdx.x; i < rows * heads * pad; i += blockDim.x) {
+    const int at = i % pad, h = i / pad % heads, r = i / (pad * heads);
+    *reinterpret_cast<T*>(tile + r * rs + (h * CP + channels + at) * int(sizeof(T))) = T(0.0f);
+  }
 }
 
 // ---- distance buckets --------------------------------------------------------------------
 // bucket(x) = number of edges not above x. A cell holds the floats of one
-// exponent and three top mantissa bits, counted from the smallest positive edge:
-// 511 cells reach 2^63 times that edge, one takes all that is larger. A cell's
-// entry is the count at its lower end and, where one edge lies inside, that
-// edge: a lookup is one read and one comparison. Only where edges are closer
-// than a cell (12 %) are they stepped over one by one.
-constexpr int kBucketCells = 512;
+// exponent and two top mantissa bits: the table has the count at the cell's
+// lower end and, where an edge lies inside, that edge, so a lookup is one read
+// and one comparison. Only where edges share a cell (closer than 12 to 25 %)
+// are they stepped over one by one.
+constexpr int kBucketCells = 1024;
 
 struct BucketTable {
-  float edge[kMaxBuckets];  // ascending; unused and NaN edges at the end as NaN (never counted)
-  uint2 cell[kBucketCells]; // count | crowded << 8, bits of the edge inside (NaN: none)
-  int first;                // cell number of cell[0]
-  int not_positive;         // edges that are zero or negative
+  uint2 cell[kBucketCells];  // count * 4, bits of the edge inside (NaN: none)
+  float edge[kMaxBuckets];   // ascending; unused and NaN edges at the end as NaN (never counted)
+  int crowded;               // some cell holds several edges
 
   // All threads of the block; a barrier must follow.
   __device__ void make(const float* edges, int count) {
     __shared__ float raw[kMaxBuckets];
     const float nan = __int_as_float(0x7fffffff);
     for (int i = threadIdx.x; i < kMaxBuckets; i += blockDim.x) raw[i] = i < count ? edges[i] : nan;
+    if (threadIdx.x == 0) crowded = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < kMaxBuckets; i += blockDim.x) {
       const float x = raw[i];
@@ -352,61 +475,130 @@ struct BucketTable {
       edge[rank] = x;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-      int n = 0;
-      while (n < count && edge[n] <= 0.0f) ++n;
-      not_positive = n;
-      first = n < count && edge[n] == edge[n] ? int(__float_as_uint(edge[n]) >> 20) - 1 : 0;
-    }
-    __syncthreads();
     for (int i = threadIdx.x; i < kBucketCells; i += blockDim.x) {
-      const int n = max(first + i, 0);
-      // Edges up to the cell's lower end; cell 0 starts at 0.
-      const float low = i == 0 ? 0.0f : __uint_as_float(uint32_t(n) << 20);
-      const float high = i + 1 == kBucketCells ? INFINITY : __uint_as_float(uint32_t(n + 1) << 20);
+      const float low = __uint_as_float(uint32_t(i) << 21);
       int lo = 0, hi = count;
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (edge[mid] <= low) lo = mid + 1; else hi = mid;
       }
-      int inside = 0;
-      while (inside < 2 && lo + inside < count && (edge[lo + inside] < high || i + 1 == kBucketCells) &&
-             edge[lo + inside] == edge[lo + inside])
-        ++inside;
-      cell[i] = make_uint2(uint32_t(lo) | (inside > 1 ? 256u : 0u),
-                           __float_as_uint(inside > 0 ? edge[lo] : nan));
+      // Cells of NaN have low = NaN: no edge counts.
+      const float inside = lo < count && __float_as_uint(edge[lo]) >> 21 == uint32_t(i) ? edge[lo] : nan;
+      if (lo + 1 < count && __float_as_uint(edge[lo + 1]) >> 21 == uint32_t(i) && low == low) crowded = 1;
+      cell[i] = make_uint2(uint32_t(lo) * 4, __float_as_uint(low == low ? inside : nan));
     }
   }
-  // x >= 0 or NaN (a NaN counts no edge).
-  __device__ __forceinline__ int find(float x) const {
-    const int i = min(max(int(__float_as_uint(x) >> 20) - first, 0), kBucketCells - 1);
-    const uint2 c = cell[i];
-    int b = int(c.x) + (x >= __uint_as_float(c.y) ? 1 : 0);
-    if (b >= 256) {  // several edges in the cell
-      b = int(c.x) - 256;
-      while (b < kMaxBuckets && edge[b] <= x) ++b;
-    }
-    return x == x ? b : 0;
+  // Four times the bucket; x >= 0 or NaN (a NaN counts no edge).
+  __device__ __forceinline__ uint32_t find4(float x) const {
+    const uint2 c = cell[__float_as_uint(x) >> 21];
+    uint32_t b = c.x;
+    if (x >= __uint_as_float(c.y)) b += 4;
+    return b;
   }
-  // Any x.
-  __device__ __forceinline__ int find_any(float x) const {
-    if (x > 0.0f) return find(x);
-    int b = 0;
+  // The same where cells may be crowded.
+  __device__ __forceinline__ uint32_t find4_slow(float x) const {
+    if (x != x) return 0;
+    uint32_t b = cell[__float_as_uint(x) >> 21].x / 4;
+    while (b < kMaxBuckets && edge[b] <= x) ++b;
+    return b * 4;
+  }
+  // The bucket of any x.
+  __device__ __forceinline__ uint32_t find_any(float x) const {
+    if (x > 0.0f) return (crowded ? find4_slow(x) : find4(x)) / 4;
+    uint32_t b = 0;
     while (b < kMaxBuckets && edge[b] <= x) ++b;
     return b;
   }
 };
 
-// Squared distance of a pair, each operation rounded.
-__device__ __forceinline__ float pair_distance(float qx, float qy, float qz, float px, float py, float pz, bool three) {
-  const float x = __fsub_rn(qx, px), y = __fsub_rn(qy, py);
-  float d = __fadd_rn(__fmul_rn(x, x), __fmul_rn(y, y));
-  if (three) {
-    const float z = __fsub_rn(qz, pz);
-    d = __fadd_rn(d, __fmul_rn(z, z));
-  }
-  return d;
+// Squared distance of points p (negated) and x, each operation rounded by
+// itself, x first. (Not in pairs of float32: the compiler joins their products
+// and sums, and distances would miss borders they lie on.) In 2-D z is 0, which
+// changes nothing.
+__device__ __forceinline__ float pair_distance(float4 minus_p, float x, float y, float z) {
+  x = __fadd_rn(x, minus_p.x);
+  y = __fadd_rn(y, minus_p.y);
+  z = __fadd_rn(z, minus_p.z);
+  return __fadd_rn(__fadd_rn(__fmul_rn(x, x), __fmul_rn(y, y)), __fmul_rn(z, z));
 }
+
+// Buckets of a step: rows are points p[0..rows), columns the 32 points of `pts`
+// ([3][32]). Leaf (or query) n * 8 + 2t + e of a row is byte t * 8 + n * 2 + e,
+// so that the eight that lane t of a fragment needs lie side by side; a byte is
+// the bucket times four, the offset into a bias row. A thread has four columns
+// and every blockDim / 8-th row.
+template <bool CROWDED>
+__device__ __forceinline__ void sort_step(uint8_t* to, int row_bytes, const BucketTable& table, const float4* p,
+                                          int rows, const float* pts) {
+  const int part = threadIdx.x % 8;  // 2 t + (upper groups)
+  const float* c = pts + (part & 1) * 16 + (part >> 1) * 2;
+  const float2 x0 = *reinterpret_cast<const float2*>(c), x1 = *reinterpret_cast<const float2*>(c + 8);
+  const float2 y0 = *reinterpret_cast<const float2*>(c + 32), y1 = *reinterpret_cast<const float2*>(c + 40);
+  const float2 z0 = *reinterpret_cast<const float2*>(c + 64), z1 = *reinterpret_cast<const float2*>(c + 72);
+  for (int r = threadIdx.x / 8; r < rows; r += blockDim.x / 8) {
+    const float4 q = p[r];
+    auto find = [&](float d) { return CROWDED ? table.find4_slow(d) : table.find4(d); };
+    const uint32_t b0 = find(pair_distance(q, x0.x, y0.x, z0.x)), b1 = find(pair_distance(q, x0.y, y0.y, z0.y));
+    const uint32_t b2 = find(pair_distance(q, x1.x, y1.x, z1.x)), b3 = find(pair_distance(q, x1.y, y1.y, z1.y));
+    *reinterpret_cast<uint32_t*>(to + r * row_bytes + part * 4) =
+        __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
+  }
+}
+
+// One score's bias: `row` is the shared address of the head's biases, a multiple
+// of 256, so that a byte of buckets put in its place is the bias's address.
+__device__ __forceinline__ float bias_of(uint32_t row, uint2 b, int n, int j) {
+  return lds_f32(__byte_perm(n < 2 ? b.x : b.y, row, 0x7650 + (n & 1) * 2 + j));
+}
+
+// s = logits of 16 rows and 32 columns in units of `unit` (see Units).
+template <typename T, int CP, bool HELD>
+__device__ __forceinline__ void logits(float (&s)[4][4], const typename Frag<T>::A* held, uint32_t a, uint32_t a_rs,
+                                       uint32_t b, uint32_t b_rs, bool biased, uint32_t bias, const uint8_t* near,
+                                       int row_step, float scale, bool folded) {
+  if (biased) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const uint2 w = *reinterpret_cast<const uint2*>(near + r * row_step);
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) s[n][2 * r + j] = bias_of(bias, w, n, j);
+    }
+    if (folded) {
+      multiply_nk<T, CP, 4, HELD, false>(s, held, a, a_rs, b, b_rs);
+    } else {
+      float x[4][4];
+      multiply_nk<T, CP, 4, HELD, true>(x, held, a, a_rs, b, b_rs);
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = fmaf(x[n][j], scale, s[n][j]);
+    }
+  } else {
+    multiply_nk<T, CP, 4, HELD, true>(s, held, a, a_rs, b, b_rs);
+    if (!folded) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] *= scale;
+    }
+  }
+}
+
+// Logits are kept as z / unit: the bias starts the products' accumulators
+// divided by the scale, and scale and base change are one factor in the
+// exponential. Scales that this does not suit (negative, tiny, huge) are applied
+// to the products instead.
+struct Units {
+  bool folded;
+  float unit, bias;
+  __device__ __forceinline__ explicit Units(float scale) {
+    folded = scale >= 0x1p-30f && scale <= 0x1p30f;
+    unit = folded ? scale * kLog2e : 1.0f;
+    bias = folded ? 1.0f / scale : kLog2e;
+  }
+};
 
 // ---- arguments shared by the kernels --------------------------------------------------------
 struct AttendArgs {
@@ -473,15 +665,19 @@ __device__ __forceinline__ float gradient_lift(const AttendArgs& a) {
   return exp2f(-floorf(log2f(most)));
 }
 
-// Packed key row of leaf `leaf` of a cloud, or -1 past its end.
-__device__ __forceinline__ int key_row(const AttendArgs& a, const BlockCloud& c, int64_t leaf) {
-  if (leaf >= c.n) return -1;
-  const int64_t i = a.sorted[c.p0 + leaf];
+// Packed row of index `i` of a cloud's order.
+__device__ __forceinline__ int checked_row(const AttendArgs& a, const BlockCloud& c, int64_t i) {
   if (uint64_t(i) >= uint64_t(c.n)) {
     if (a.status) atomicOr(a.status, kDevErrBadIndex);
     return -1;
   }
   return int(c.p0 + i);
+}
+
+// Packed key row of leaf `leaf` of a cloud, or -1 past its end.
+__device__ __forceinline__ int key_row(const AttendArgs& a, const BlockCloud& c, int64_t leaf) {
+  if (leaf >= c.n) return -1;
+  return checked_row(a, c, a.sorted[c.p0 + leaf]);
 }
 
 // First leaf row of a cloud's node rows.

@@ -20,31 +20,34 @@ namespace tbvh {
 constexpr int kKvHeads = 2;  // key/value heads of one thread block, at most
 
 struct KeyBlockSmem {
-  uint32_t k, v, q, d, lse, delta, rows, krows, bias, buckets, pts, kpts, table, total;
+  uint32_t bias, k, v, q, d, lse, delta, places, rows, krows, buckets, pts, kpts, table, total;
 };
+
+constexpr int kKeyBucketRow = kTileQueries + 8;  // bytes of a key's row of buckets
 
 __host__ __device__ inline KeyBlockSmem key_block_smem(int size, int cp, int kvs, int group, bool bias) {
   KeyBlockSmem s{};
-  const uint32_t ld = uint32_t(cp + 16 / size);
+  const uint32_t row = uint32_t(kvs * cp * size + 16);
   uint32_t at = 0;
   auto take = [&](uint32_t bytes) {
     const uint32_t was = at;
     at += (bytes + 15) / 16 * 16;
     return was;
   };
-  s.k = take(kvs * kBlockLeaves * ld * size);
-  s.v = take(kvs * kBlockLeaves * ld * size);
-  s.q = take(2 * kvs * kTileQueries * ld * size);
-  s.d = take(2 * kvs * kTileQueries * ld * size);
+  if (bias) s.bias = take(kvs * group * kMaxBuckets * 4);
+  s.k = take(kBlockLeaves * row);
+  s.v = take(kBlockLeaves * row);
+  s.q = take(2 * kTileQueries * row);
+  s.d = take(2 * kTileQueries * row);
   s.lse = take(2 * kvs * kTileQueries * 4);
   s.delta = take(2 * kvs * kTileQueries * 4);
+  s.places = take(2 * kTileQueries * 8);
   s.rows = take(2 * kTileQueries * 4);
   s.krows = take(kBlockLeaves * 4);
   if (bias) {
-    s.bias = take(kvs * group * kMaxBuckets * 4);
-    s.buckets = take(2 * kBlockLeaves * (kTileQueries + 4));
+    s.buckets = take(2 * kBlockLeaves * kKeyBucketRow);
     s.pts = take(2 * 3 * kTileQueries * 4);
-    s.kpts = take(3 * kBlockLeaves * 4);
+    s.kpts = take(4 * kBlockLeaves * 4);
     s.table = take(sizeof(BucketTable));
   }
   s.total = at;
@@ -54,12 +57,11 @@ __host__ __device__ inline KeyBlockSmem key_block_smem(int size, int cp, int kvs
 template <typename T, int CP>
 __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
   using F = Frag<T>;
-  constexpr int LD = Tile<T, CP>::LD;
+  constexpr uint32_t SIZE = sizeof(T);
   constexpr int NT = kTileQueries / 8;
   constexpr bool HELD = sizeof(T) == 2 && CP <= 64;
   constexpr int HOLD = HELD ? CP / F::STEP : 1;
-  constexpr int BROW = kTileQueries + 4;
-  extern __shared__ __align__(16) char smem[];
+  extern __shared__ __align__(256) char smem[];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t block = blockIdx.x;
@@ -68,21 +70,19 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
   const BlockCloud c = a.map.of_block(block);
   const bool bias = a.table != nullptr;
   const KeyBlockSmem off = key_block_smem(sizeof(T), CP, a.kv_cta, a.group, bias);
-  T* s_k = reinterpret_cast<T*>(smem + off.k);
-  T* s_v = reinterpret_cast<T*>(smem + off.v);
-  T* s_q = reinterpret_cast<T*>(smem + off.q);
-  T* s_d = reinterpret_cast<T*>(smem + off.d);
+  const uint32_t base = smem_u32(smem);
   float* s_lse = reinterpret_cast<float*>(smem + off.lse);
   float* s_delta = reinterpret_cast<float*>(smem + off.delta);
   int* s_rows = reinterpret_cast<int*>(smem + off.rows);
+  uint64_t* s_places = reinterpret_cast<uint64_t*>(smem + off.places);
   int* s_krows = reinterpret_cast<int*>(smem + off.krows);
   float* s_bias = reinterpret_cast<float*>(smem + off.bias);
   uint8_t* s_buckets = reinterpret_cast<uint8_t*>(smem + off.buckets);
   float* s_pts = reinterpret_cast<float*>(smem + off.pts);
-  float* s_kpts = reinterpret_cast<float*>(smem + off.kpts);
+  float4* s_kpts = reinterpret_cast<float4*>(smem + off.kpts);  // negated
   BucketTable& s_table = *reinterpret_cast<BucketTable*>(smem + off.table);
-  const int k_tile = kBlockLeaves * LD, q_tile = kTileQueries * LD;
-  const int stage = a.kv_cta * q_tile;
+  const uint32_t rs = row_bytes<T, CP>(a.kv_cta);
+  const uint32_t stage = kTileQueries * rs;
 
   const int64_t begin = a.plan.query_begin[block];
   const int listed = int(a.plan.query_begin[block + 1] - begin);
@@ -93,16 +93,13 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
   // Steps: every chunk once for each query head that shares a key/value head.
   const int group = a.group;
   const int64_t steps = int64_t(chunks) * group;
-  // As in the query-tile kernel.
-  const bool folded = a.scale >= 0x1p-30f && a.scale <= 0x1p30f;
-  const float unit = folded ? a.scale * kLog2e : 1.0f;
-  const float bias_unit = folded ? 1.0f / a.scale : kLog2e;
+  const Units units(a.scale);
 
   if (tid < kBlockLeaves) {
     s_krows[tid] = key_row(a, c, leaf0 + tid);
     if (bias) {
       const float* p = a.aabbs + (leaf_row0(c) + leaf0 + tid) * 2 * a.dim;
-      for (int x = 0; x < 3; ++x) s_kpts[x * kBlockLeaves + tid] = tid < valid && x < a.dim ? p[x] : 0.0f;
+      s_kpts[tid] = tid < valid ? make_float4(-p[0], -p[1], a.dim == 3 ? -p[2] : 0.0f, 0.0f) : make_float4(0, 0, 0, 0);
     }
   }
   int next_row = -1;
@@ -124,6 +121,7 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
     if (tid < kTileQueries && e < chunks) {
       const int slot = e & 1;
       s_rows[slot * kTileQueries + tid] = next_row;
+      s_places[slot * kTileQueries + tid] = row_place(next_row, a.heads * CP * SIZE);
       if (bias)
         for (int x = 0; x < 3; ++x) s_pts[(slot * 3 + x) * kTileQueries + tid] = next_pt[x];
     }
@@ -133,10 +131,18 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
       const int slot = int(step & 1);
       const int* rows = s_rows + (e & 1) * kTileQueries;
       // Query heads kv * group + member, one a key/value head.
-      copy_rows<T, CP>(s_q + slot * stage, q_tile, static_cast<const T*>(a.q), rows, kTileQueries, a.heads, a.channels,
-                       kv0 * group + member, kvs, a.width, group);
-      copy_rows<T, CP>(s_d + slot * stage, q_tile, static_cast<const T*>(a.grad_out), rows, kTileQueries, a.heads,
-                       a.channels, kv0 * group + member, kvs, a.width, group);
+      const int first = kv0 * group + member;
+      const uint32_t to = base + slot * stage;
+      const RowWords words(a.q, a.grad_out, SIZE, CP, a.channels, first, kvs, group, a.width, rs);
+      if (words.at_once) {
+        words.copy(to + off.q, to + off.d, s_places + (e & 1) * kTileQueries, kTileQueries);
+      } else {
+        auto row_of = [&](int r) { return rows[r]; };
+        const Rows<T, CP> q{static_cast<const T*>(a.q), a.heads, a.channels, first, kvs, group, a.width, rs};
+        const Rows<T, CP> d{static_cast<const T*>(a.grad_out), a.heads, a.channels, first, kvs, group, a.width, rs};
+        q.copy(to + off.q, kTileQueries, row_of);
+        d.copy(to + off.d, kTileQueries, row_of);
+      }
       for (int i = tid; i < kvs * kTileQueries; i += blockDim.x) {
         const int h = i / kTileQueries, q = i % kTileQueries, row = rows[q];
         const int64_t at = int64_t(row < 0 ? 0 : row) * a.heads + (kv0 + h) * group + member;
@@ -149,43 +155,33 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
     }
     cp_commit();
   };
-  // Distance buckets of chunk e, times four: a thread has a key and four neighbouring queries.
-  auto sort_pairs = [&](int e) {
+  auto sort_pairs = [&](int e) {  // distance buckets of chunk e
     if (bias && e < chunks) {
       const int slot = e & 1;
-      for (int u = tid; u < kTileQueries * kBlockLeaves / 4; u += blockDim.x) {
-        const int key = u / (kTileQueries / 4), q4 = u % (kTileQueries / 4) * 4;
-        const float kx = s_kpts[key], ky = s_kpts[kBlockLeaves + key], kz = s_kpts[2 * kBlockLeaves + key];
-        const float* p = s_pts + slot * 3 * kTileQueries + q4;
-        const float4 px = *reinterpret_cast<const float4*>(p);
-        const float4 py = *reinterpret_cast<const float4*>(p + kTileQueries);
-        const float4 pz = *reinterpret_cast<const float4*>(p + 2 * kTileQueries);
-        const bool three = a.dim == 3;
-        const uint32_t b0 = s_table.find(pair_distance(px.x, py.x, pz.x, kx, ky, kz, three));
-        const uint32_t b1 = s_table.find(pair_distance(px.y, py.y, pz.y, kx, ky, kz, three));
-        const uint32_t b2 = s_table.find(pair_distance(px.z, py.z, pz.z, kx, ky, kz, three));
-        const uint32_t b3 = s_table.find(pair_distance(px.w, py.w, pz.w, kx, ky, kz, three));
-        *reinterpret_cast<uint32_t*>(s_buckets + (slot * kBlockLeaves + key) * BROW + q4) =
-            (b0 | b1 << 8 | b2 << 16 | b3 << 24) << 2;
-      }
+      uint8_t* to = s_buckets + slot * kBlockLeaves * kKeyBucketRow;
+      const float* p = s_pts + slot * 3 * kTileQueries;
+      if (s_table.crowded) sort_step<true>(to, kKeyBucketRow, s_table, s_kpts, kBlockLeaves, p);
+      else sort_step<false>(to, kKeyBucketRow, s_table, s_kpts, kBlockLeaves, p);
     }
   };
 
-  clear_padding<T, CP>(s_k, a.kv_cta * kBlockLeaves, a.channels);
-  clear_padding<T, CP>(s_v, a.kv_cta * kBlockLeaves, a.channels);
-  clear_padding<T, CP>(s_q, 2 * a.kv_cta * kTileQueries, a.channels);
-  clear_padding<T, CP>(s_d, 2 * a.kv_cta * kTileQueries, a.channels);
+  clear_padding<T, CP>(smem + off.k, rs, kBlockLeaves, a.kv_cta, a.channels);
+  clear_padding<T, CP>(smem + off.v, rs, kBlockLeaves, a.kv_cta, a.channels);
+  clear_padding<T, CP>(smem + off.q, rs, 2 * kTileQueries, a.kv_cta, a.channels);
+  clear_padding<T, CP>(smem + off.d, rs, 2 * kTileQueries, a.kv_cta, a.channels);
+  if (bias)
+    for (int i = tid; i < kvs * group * a.buckets; i += blockDim.x)
+      s_bias[(i / a.buckets) * kMaxBuckets + i % a.buckets] = a.table[int64_t(kv0) * group * a.buckets + i] * units.bias;
   fetch(0);
   put(0);
-  if (bias) {
-    for (int i = tid; i < kvs * group * a.buckets; i += blockDim.x)
-      s_bias[(i / a.buckets) * kMaxBuckets + i % a.buckets] = a.table[int64_t(kv0) * group * a.buckets + i] * bias_unit;
-  }
   __syncthreads();
-  copy_rows<T, CP>(s_k, k_tile, static_cast<const T*>(a.k), s_krows, kBlockLeaves, a.kv_heads, a.channels, kv0, kvs,
-                   a.width);
-  copy_rows<T, CP>(s_v, k_tile, static_cast<const T*>(a.v), s_krows, kBlockLeaves, a.kv_heads, a.channels, kv0, kvs,
-                   a.width);
+  {
+    auto row_of = [&](int r) { return s_krows[r]; };
+    const Rows<T, CP> keys{static_cast<const T*>(a.k), a.kv_heads, a.channels, kv0, kvs, 1, a.width, rs};
+    const Rows<T, CP> values{static_cast<const T*>(a.v), a.kv_heads, a.channels, kv0, kvs, 1, a.width, rs};
+    keys.copy(base + off.k, kBlockLeaves, row_of);
+    values.copy(base + off.v, kBlockLeaves, row_of);
+  }
   copy(0, 0, 0);
   fetch(1);
   put(1);
@@ -200,14 +196,17 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
   const int kv = warp >> 2, quarter = warp & 3;
   const bool mine = kv < kvs && quarter * 16 < valid;
   const int g = lane >> 2, t = lane & 3;
-  const T* k_rows = s_k + kv * k_tile;
-  const T* v_rows = s_v + kv * k_tile;
-  const float lift = gradient_lift<T>(a);
+  // Byte addresses with the lane's offset; query tiles of stage 0.
+  const uint32_t head_at = base + kv * CP * SIZE;
+  const uint32_t k_at = head_at + off.k + quarter * 16 * rs + F::lane_a(rs, lane), v_at = k_at + (off.v - off.k);
+  const uint32_t nk = F::lane_nk(rs, lane), kn = F::lane_kn(rs, lane);
+  const uint8_t* near0 = s_buckets + (quarter * 16 + g) * kKeyBucketRow + 8 * t;
+  const float lift = gradient_lift<T>(a), unit = units.unit;
   typename F::A held_k[HOLD], held_v[HOLD];
   if constexpr (HELD) {
     if (mine) {
-      hold<T, CP>(held_k, k_rows, quarter * 16, lane);
-      hold<T, CP>(held_v, v_rows, quarter * 16, lane);
+      hold<T, CP>(held_k, k_at, rs);
+      hold<T, CP>(held_v, v_at, rs);
     }
   }
   float dk[CP / 8][4] = {}, dv[CP / 8][4] = {};
@@ -224,58 +223,30 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
     }
     if (mine) {
       const int slot = int(step & 1);
-      const T* q_rows = s_q + slot * stage + kv * q_tile;
-      const T* d_rows = s_d + slot * stage + kv * q_tile;
+      const uint32_t q_at = head_at + off.q + slot * stage, d_at = head_at + off.d + slot * stage;
       const float* lse = s_lse + (slot * a.kv_cta + kv) * kTileQueries + 2 * t;
       const float* delta = s_delta + (slot * a.kv_cta + kv) * kTileQueries + 2 * t;
-      const char* head_bias = reinterpret_cast<const char*>(s_bias + (kv * group + member) * kMaxBuckets);
-      const uint8_t* near = s_buckets + ((e & 1) * kBlockLeaves + quarter * 16 + g) * BROW + 2 * t;
-      float s[NT][4], ds[NT][4] = {};
-      auto read_bias = [&]() {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint32_t lo = *reinterpret_cast<const uint16_t*>(near + n * 8);
-          const uint32_t hi = *reinterpret_cast<const uint16_t*>(near + 8 * BROW + n * 8);
-          s[n][0] = *reinterpret_cast<const float*>(head_bias + (lo & 255));
-          s[n][1] = *reinterpret_cast<const float*>(head_bias + (lo >> 8));
-          s[n][2] = *reinterpret_cast<const float*>(head_bias + (hi & 255));
-          s[n][3] = *reinterpret_cast<const float*>(head_bias + (hi >> 8));
-        }
-      };
-      if (bias && folded) {
-        read_bias();
-        multiply_nk<T, CP, NT, HELD>(s, held_k, k_rows, quarter * 16, q_rows, 0, lane);
-      } else {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[n][j] = 0.0f;
-        multiply_nk<T, CP, NT, HELD>(s, held_k, k_rows, quarter * 16, q_rows, 0, lane);
-        if (!folded) {
-          float x[NT][4];
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              x[n][j] = s[n][j] * (a.scale * kLog2e);
-              s[n][j] = 0.0f;
-            }
-          if (bias) read_bias();
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[n][j] += x[n][j];
-        }
-      }
-      multiply_nk<T, CP, NT, HELD>(ds, held_v, v_rows, quarter * 16, d_rows, 0, lane);
+      const uint32_t head_bias = base + off.bias + (kv * group + member) * kMaxBuckets * 4;
+      float s[NT][4], ds[NT][4];
+      logits<T, CP, HELD>(s, held_k, k_at, rs, q_at + nk, rs, bias, head_bias,
+                          near0 + (e & 1) * kBlockLeaves * kKeyBucketRow, 8 * kKeyBucketRow, a.scale * kLog2e,
+                          units.folded);
+      multiply_nk<T, CP, NT, HELD, true>(ds, held_v, v_at, rs, d_at + nk, rs);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float2 l = *reinterpret_cast<const float2*>(lse + n * 8);
         const float2 d = *reinterpret_cast<const float2*>(delta + n * 8);
+        const Pair minus_l = pair(-l.x, -l.y), minus_d = pair(-d.x, -d.y);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[n][j] = exp2_fast(fmaf(s[n][j], unit, -((j & 1) ? l.y : l.x)));
-          ds[n][j] = s[n][j] * (lift * (ds[n][j] - ((j & 1) ? d.y : d.x)));
+        for (int r = 0; r < 2; ++r) {
+          const float2 x = unpair(fma2(pair(s[n][2 * r], s[n][2 * r + 1]), both(unit), minus_l));
+          s[n][2 * r] = exp2_fast(x.x);
+          s[n][2 * r + 1] = exp2_fast(x.y);
+          Pair y = add2(pair(ds[n][2 * r], ds[n][2 * r + 1]), minus_d);
+          if constexpr (SIZE == 2) y = mul2(y, both(lift));
+          y = mul2(pair(s[n][2 * r], s[n][2 * r + 1]), y);
+          ds[n][2 * r] = unpair(y).x;
+          ds[n][2 * r + 1] = unpair(y).y;
         }
       }
       constexpr int STEPS = kTileQueries / F::STEP;
@@ -288,10 +259,10 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
 #pragma unroll
           for (int j = 0; j < CP / 16; ++j) {
             typename F::B b;
-            F::pair_kn(b, d_rows, LD, st * F::STEP, j * 16, lane);
+            F::pair_kn(b, d_at + kn + st * F::STEP * rs + j * 16 * SIZE, rs);
             F::mma(dv[2 * j], p, b[0], b[1]);
             F::mma(dv[2 * j + 1], p, b[2], b[3]);
-            F::pair_kn(b, q_rows, LD, st * F::STEP, j * 16, lane);
+            F::pair_kn(b, q_at + kn + st * F::STEP * rs + j * 16 * SIZE, rs);
             F::mma(dk[2 * j], x, b[0], b[1]);
             F::mma(dk[2 * j + 1], x, b[2], b[3]);
           }
@@ -309,10 +280,10 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
             from_acc<T>(p, s, st);
             from_acc<T>(x, ds, st);
             typename F::B b;
-            F::pair_kn(b, d_rows, LD, st * F::STEP, j * 16, lane);
+            F::pair_kn(b, d_at + kn + st * F::STEP * rs + j * 16 * SIZE, rs);
             F::mma(part_v[0], p, b[0], b[1]);
             F::mma(part_v[1], p, b[2], b[3]);
-            F::pair_kn(b, q_rows, LD, st * F::STEP, j * 16, lane);
+            F::pair_kn(b, q_at + kn + st * F::STEP * rs + j * 16 * SIZE, rs);
             F::mma(part_k[0], x, b[0], b[1]);
             F::mma(part_k[1], x, b[2], b[3]);
           }

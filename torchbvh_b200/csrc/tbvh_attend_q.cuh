@@ -31,31 +31,34 @@
 namespace tbvh {
 
 constexpr int kStepLeaves = 32;
+constexpr int kBucketRow = kStepLeaves + 8;  // bytes of a query's row of buckets
 
 struct QueryTileSmem {
-  uint32_t k, v, q, d, bias, buckets, pts, rows, qrows, table, hist, total;
+  uint32_t bias, k, v, q, d, places, rows, buckets, pts, qpts, table, hist, total;
 };
 
+// Offsets of a thread block's arrays (bias first: its rows lie on 256 bytes).
 __host__ __device__ inline QueryTileSmem query_tile_smem(int size, int cp, int kvs, int heads, bool back, bool bias,
                                                          int buckets) {
   QueryTileSmem s{};
-  const uint32_t ld = uint32_t(cp + 16 / size);
+  const uint32_t kv_row = uint32_t(kvs * cp * size + 16), q_row = uint32_t(heads * cp * size + 16);
   uint32_t at = 0;
   auto take = [&](uint32_t bytes) {
     const uint32_t was = at;
     at += (bytes + 15) / 16 * 16;
     return was;
   };
-  s.k = take(2 * kvs * kStepLeaves * ld * size);
-  s.v = take(2 * kvs * kStepLeaves * ld * size);
-  s.q = take(heads * kTileQueries * ld * size);
-  s.d = back ? take(heads * kTileQueries * ld * size) : 0;
-  s.rows = take(2 * kStepLeaves * 4);
-  s.qrows = take(kTileQueries * 4);
+  if (bias) s.bias = take(heads * kMaxBuckets * 4);
+  s.k = take(2 * kStepLeaves * kv_row);
+  s.v = take(2 * kStepLeaves * kv_row);
+  s.q = take(kTileQueries * q_row);
+  s.d = back ? take(kTileQueries * q_row) : 0;
+  s.places = take(2 * kStepLeaves * 8);
+  s.rows = take(kTileQueries * 4);
   if (bias) {
-    s.bias = take(heads * kMaxBuckets * 4);
-    s.buckets = take(2 * kTileQueries * (kStepLeaves + 4));
+    s.buckets = take(2 * kTileQueries * kBucketRow);
     s.pts = take(2 * 3 * kStepLeaves * 4);
+    s.qpts = take(kTileQueries * 16);
     s.table = take(sizeof(BucketTable));
     if (back) s.hist = take(uint32_t(buckets) * heads * 64 * 4);
   }
@@ -63,157 +66,162 @@ __host__ __device__ inline QueryTileSmem query_tile_smem(int size, int cp, int k
   return s;
 }
 
+// Row r of a group of accumulator tiles from n0: old * factor + part where `on`.
+template <int N>
+__device__ __forceinline__ void keep_group(Pair (&acc)[N][2], int n0, int r, Pair factor,
+                                           const float (&part)[kChannelGroup][4], uint32_t on) {
+  static_assert(kChannelGroup == 4, "one group is four tiles");
+  keep_where(acc[n0][r], acc[n0 + 1][r], acc[n0 + 2][r], acc[n0 + 3][r], factor, pair(part[0][2 * r], part[0][2 * r + 1]),
+             pair(part[1][2 * r], part[1][2 * r + 1]), pair(part[2][2 * r], part[2][2 * r + 1]),
+             pair(part[3][2 * r], part[3][2 * r + 1]), on);
+}
+
 // Registers: with 32 padded channels three blocks of eight warps share an SM.
 template <typename T, int CP, bool BACK, bool EXACT>
 __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) == 4 ? 2 : 3) : CP <= 64 ? 2 : 1)
     k_query_tile(AttendArgs a) {
   using F = Frag<T>;
-  constexpr int LD = Tile<T, CP>::LD;
   constexpr int NT = kStepLeaves / 8;
   constexpr int STEPS = kStepLeaves / F::STEP;
-  constexpr bool HELD = sizeof(T) == 2 ? CP <= 64 : CP <= 32 && !BACK;
+  constexpr uint32_t SIZE = sizeof(T);
+  constexpr bool HELD = SIZE == 2 ? CP <= 64 : CP <= 32 && !BACK;
   constexpr int HOLD = HELD ? CP / F::STEP : 1;
-  constexpr int BROW = kStepLeaves + 4;  // bytes of one query's bucket row
-  extern __shared__ __align__(16) char smem[];
+  extern __shared__ __align__(256) char smem[];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t tile = blockIdx.x;
   const HeadSpan span(a, blockIdx.y);
   const BlockCloud c = a.map.of_tile(tile);
   const bool bias = a.table != nullptr;
-  const QueryTileSmem off = query_tile_smem(sizeof(T), CP, a.kv_cta, a.heads_cta, BACK, bias, a.buckets);
-  T* s_k = reinterpret_cast<T*>(smem + off.k);
-  T* s_v = reinterpret_cast<T*>(smem + off.v);
-  T* s_q = reinterpret_cast<T*>(smem + off.q);
-  T* s_d = reinterpret_cast<T*>(smem + off.d);
+  const QueryTileSmem off = query_tile_smem(SIZE, CP, a.kv_cta, a.heads_cta, BACK, bias, a.buckets);
+  const uint32_t base = smem_u32(smem);
+  uint64_t* s_places = reinterpret_cast<uint64_t*>(smem + off.places);
   int* s_rows = reinterpret_cast<int*>(smem + off.rows);
-  int* s_qrows = reinterpret_cast<int*>(smem + off.qrows);
-  float* s_bias = reinterpret_cast<float*>(smem + off.bias);
   uint8_t* s_buckets = reinterpret_cast<uint8_t*>(smem + off.buckets);
-  float* s_pts = reinterpret_cast<float*>(smem + off.pts);
-  BucketTable& s_table = *reinterpret_cast<BucketTable*>(smem + off.table);
   float* s_hist = reinterpret_cast<float*>(smem + off.hist);
-  const int kv_tile = kStepLeaves * LD, q_tile = kTileQueries * LD;
-  const int stage = a.kv_cta * kv_tile;
+  const uint32_t kv_rs = row_bytes<T, CP>(a.kv_cta), q_rs = row_bytes<T, CP>(a.heads_cta);
+  const uint32_t stage = kStepLeaves * kv_rs;
+  const RowWords words(a.k, a.v, SIZE, CP, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs);
+  const uint32_t place_unit = words.at_once ? a.kv_heads * CP * SIZE : 16;  // other shapes keep the row number
 
   const int all = a.plan.tile_count[tile];
   const int splits = BACK ? 1 : a.splits;
-  const int from = int(int64_t(all) * blockIdx.z / splits), count = int(int64_t(all) * (blockIdx.z + 1) / splits) - from;
-  const int steps = 2 * count;
+  const int from = int(int64_t(all) * blockIdx.z / splits);
+  const int steps = 2 * (int(int64_t(all) * (blockIdx.z + 1) / splits) - from);
   const uint2* entries = a.plan.entries + tile * a.plan.capacity + from;
-  const int64_t leaves = bias ? leaf_row0(c) : 0;
-  // Logits are kept as z / unit: the bias enters the products' accumulators
-  // divided by the scale, and scale and base change are one factor in the
-  // exponential. Scales that this does not suit (negative, tiny, huge) are
-  // applied to the products instead.
-  const bool folded = a.scale >= 0x1p-30f && a.scale <= 0x1p30f;
-  const float unit = folded ? a.scale * kLog2e : 1.0f;
-  const float bias_unit = folded ? 1.0f / a.scale : kLog2e;
+  const int points = int(c.n);
+  const int64_t* sorted = a.sorted + c.p0;
+  const float* leaf_points = a.aabbs + (bias ? leaf_row0(c) * 2 * a.dim : 0);
+  const Units units(a.scale);
 
-  if (tid < kTileQueries) s_qrows[tid] = a.plan.query_row[tile * kTileQueries + tid];
-  // Rows (and points) of step `i`, one leaf a lane of the first warp.
-  int next_row = -1;
-  float next_pt[3] = {0.0f, 0.0f, 0.0f};
+  auto first_leaf = [&](uint32_t block, int i) { return int(block) * kBlockLeaves + (i & 1) * kStepLeaves; };
+  // Rows and points of a step's leaves, one leaf a lane of the first warp: asked
+  // for two steps ahead, put down for the others one step ahead.
+  int64_t next_index = -1;
   auto fetch = [&](int i) {
-    if (tid < kStepLeaves && i < steps) {
-      const int64_t leaf = int64_t(entries[i >> 1].x) * kBlockLeaves + (i & 1) * kStepLeaves + tid;
-      next_row = key_row(a, c, leaf);
+    if (warp == 0 && i < steps) {
+      const int leaf = first_leaf(entries[i >> 1].x, i) + lane;
+      const bool there = leaf < points;
+      next_index = there ? sorted[leaf] : -1;
       if (bias) {
-        const float* p = a.aabbs + (leaves + leaf) * 2 * a.dim;
-        for (int x = 0; x < 3; ++x) next_pt[x] = leaf < c.n && x < a.dim ? p[x] : 0.0f;
+        const float* p = leaf_points + int64_t(there ? leaf : 0) * 2 * a.dim;
+        const uint32_t to = base + off.pts + ((i & 1) * 3 * kStepLeaves + lane) * 4;
+        cp_async<4>(to, p, there);
+        cp_async<4>(to + 4 * kStepLeaves, p + 1, there);
+        cp_async<4>(to + 8 * kStepLeaves, p + a.dim - 1, there && a.dim == 3);
       }
     }
   };
   auto put = [&](int i) {
-    if (tid < kStepLeaves && i < steps) {
-      const int slot = i & 1;
-      s_rows[slot * kStepLeaves + tid] = next_row;
-      if (bias)
-        for (int x = 0; x < 3; ++x) s_pts[(slot * 3 + x) * kStepLeaves + tid] = next_pt[x];
-    }
+    if (warp == 0 && i < steps)
+      s_places[(i & 1) * kStepLeaves + lane] =
+          row_place(next_index < 0 ? -1 : checked_row(a, c, next_index), place_unit);
   };
   auto copy = [&](int i) {
-    if (i < steps) {
-      const int slot = i & 1;
-      const int* rows = s_rows + slot * kStepLeaves;
-      copy_rows<T, CP>(s_k + slot * stage, kv_tile, static_cast<const T*>(a.k), rows, kStepLeaves, a.kv_heads,
-                       a.channels, span.kv0, span.kvs, a.width);
-      copy_rows<T, CP>(s_v + slot * stage, kv_tile, static_cast<const T*>(a.v), rows, kStepLeaves, a.kv_heads,
-                       a.channels, span.kv0, span.kvs, a.width);
+    const uint32_t at = base + (i & 1) * stage;
+    const uint64_t* places = s_places + (i & 1) * kStepLeaves;
+    if (words.at_once) {
+      words.copy(at + off.k, at + off.v, places, kStepLeaves);
+    } else {
+      auto row_of = [&](int r) { return places[r] & 1 ? -1 : int(places[r] / 16); };
+      const Rows<T, CP> keys{static_cast<const T*>(a.k), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
+      const Rows<T, CP> values{static_cast<const T*>(a.v), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
+      keys.copy(at + off.k, kStepLeaves, row_of);
+      values.copy(at + off.v, kStepLeaves, row_of);
     }
-    cp_commit();
   };
-  // Distance buckets of step i, times four (byte offsets into a bias row): a
-  // thread has one query (the same in every step where the block has 256
-  // threads) and four neighbouring leaves.
-  auto sort_pairs = [&](int i) {
-    if (bias && i < steps) {
-      const int slot = i & 1;
-      for (int u = tid; u < kTileQueries * kStepLeaves / 4; u += blockDim.x) {
-        const int q = u / (kStepLeaves / 4), k4 = u % (kStepLeaves / 4) * 4;
-        const float* qp = a.plan.query_point + tile * 3 * kTileQueries + q;
-        const float qx = __ldg(qp), qy = __ldg(qp + kTileQueries), qz = __ldg(qp + 2 * kTileQueries);
-        const float* p = s_pts + slot * 3 * kStepLeaves + k4;
-        const float4 px = *reinterpret_cast<const float4*>(p);
-        const float4 py = *reinterpret_cast<const float4*>(p + kStepLeaves);
-        const float4 pz = *reinterpret_cast<const float4*>(p + 2 * kStepLeaves);
-        const bool three = a.dim == 3;
-        const uint32_t b0 = s_table.find(pair_distance(qx, qy, qz, px.x, py.x, pz.x, three));
-        const uint32_t b1 = s_table.find(pair_distance(qx, qy, qz, px.y, py.y, pz.y, three));
-        const uint32_t b2 = s_table.find(pair_distance(qx, qy, qz, px.z, py.z, pz.z, three));
-        const uint32_t b3 = s_table.find(pair_distance(qx, qy, qz, px.w, py.w, pz.w, three));
-        *reinterpret_cast<uint32_t*>(s_buckets + (slot * kTileQueries + q) * BROW + k4) =
-            (b0 | b1 << 8 | b2 << 16 | b3 << 24) << 2;
-      }
-    }
+  auto sort_pairs = [&](int i) {  // distance buckets of step i
+    const int slot = i & 1;
+    const BucketTable& table = *reinterpret_cast<const BucketTable*>(smem + off.table);
+    uint8_t* to = s_buckets + slot * kTileQueries * kBucketRow;
+    const float4* q = reinterpret_cast<const float4*>(smem + off.qpts);
+    const float* p = reinterpret_cast<const float*>(smem + off.pts) + slot * 3 * kStepLeaves;
+    if (table.crowded) sort_step<true>(to, kBucketRow, table, q, kTileQueries, p);
+    else sort_step<false>(to, kBucketRow, table, q, kTileQueries, p);
   };
 
-  clear_padding<T, CP>(s_k, 2 * a.kv_cta * kStepLeaves, a.channels);
-  clear_padding<T, CP>(s_v, 2 * a.kv_cta * kStepLeaves, a.channels);
-  clear_padding<T, CP>(s_q, a.heads_cta * kTileQueries, a.channels);
-  if constexpr (BACK) clear_padding<T, CP>(s_d, a.heads_cta * kTileQueries, a.channels);
+  clear_padding<T, CP>(smem + off.k, kv_rs, 2 * kStepLeaves, a.kv_cta, a.channels);
+  clear_padding<T, CP>(smem + off.v, kv_rs, 2 * kStepLeaves, a.kv_cta, a.channels);
+  clear_padding<T, CP>(smem + off.q, q_rs, kTileQueries, a.heads_cta, a.channels);
+  if constexpr (BACK) clear_padding<T, CP>(smem + off.d, q_rs, kTileQueries, a.heads_cta, a.channels);
   fetch(0);
   put(0);
+  if (tid < kTileQueries) {
+    s_rows[tid] = a.plan.query_row[tile * kTileQueries + tid];
+    if (bias) {
+      const float* p = a.plan.query_point + tile * 3 * kTileQueries + tid;
+      reinterpret_cast<float4*>(smem + off.qpts)[tid] =
+          make_float4(-p[0], -p[kTileQueries], -p[2 * kTileQueries], 0.0f);
+    }
+  }
   if (bias) {
+    float* s_bias = reinterpret_cast<float*>(smem + off.bias);
     for (int i = tid; i < span.heads * a.buckets; i += blockDim.x)
-      s_bias[(i / a.buckets) * kMaxBuckets + i % a.buckets] = a.table[int64_t(span.h0) * a.buckets + i] * bias_unit;
+      s_bias[(i / a.buckets) * kMaxBuckets + i % a.buckets] = a.table[int64_t(span.h0) * a.buckets + i] * units.bias;
     if constexpr (BACK)
       for (int i = tid; i < a.buckets * int(blockDim.x); i += blockDim.x) s_hist[i] = 0.0f;
   }
   __syncthreads();
-  copy_rows<T, CP>(s_q, q_tile, static_cast<const T*>(a.q), s_qrows, kTileQueries, a.heads, a.channels, span.h0,
-                   span.heads, a.width);
-  if constexpr (BACK)
-    copy_rows<T, CP>(s_d, q_tile, static_cast<const T*>(a.grad_out), s_qrows, kTileQueries, a.heads, a.channels,
-                     span.h0, span.heads, a.width);
-  copy(0);
+  {
+    auto row_of = [&](int r) { return s_rows[r]; };
+    const Rows<T, CP> q{static_cast<const T*>(a.q), a.heads, a.channels, span.h0, span.heads, 1, a.width, q_rs};
+    q.copy(base + off.q, kTileQueries, row_of);
+    if constexpr (BACK) {
+      const Rows<T, CP> d{static_cast<const T*>(a.grad_out), a.heads, a.channels, span.h0, span.heads, 1, a.width, q_rs};
+      d.copy(base + off.d, kTileQueries, row_of);
+    }
+  }
+  if (steps > 0) copy(0);
+  cp_commit();
   fetch(1);
   put(1);
-  if (bias) {
-    s_table.make(a.edges, a.buckets - 1);
-    __syncthreads();
-  }
-  sort_pairs(0);
+  if (bias) reinterpret_cast<BucketTable*>(smem + off.table)->make(a.edges, a.buckets - 1);
   cp_wait<0>();
   __syncthreads();
+  if (bias && steps > 0) sort_pairs(0);
 
   const int head = warp >> 1, half = warp & 1;
   const bool mine = head < span.heads;
   const int kv = mine ? (span.h0 + head) / a.group - span.kv0 : 0;
   const int g = lane >> 2, t = lane & 3;
-  const T* q_rows = s_q + head * q_tile;
-  const T* d_rows = s_d + head * q_tile;
-  const char* head_bias = reinterpret_cast<const char*>(s_bias + head * kMaxBuckets);
-  char* hist = reinterpret_cast<char*>(s_hist + tid);
+  // Byte addresses with the lane's offset; key and value tiles of stage 0.
+  const uint32_t q_at = base + off.q + half * 16 * q_rs + head * CP * SIZE + F::lane_a(q_rs, lane);
+  const uint32_t d_at = q_at + (off.d - off.q);
+  const uint32_t k_at0 = base + off.k + kv * CP * SIZE, v_at0 = base + off.v + kv * CP * SIZE;
+  const uint32_t nk = F::lane_nk(kv_rs, lane), kn = F::lane_kn(kv_rs, lane);
+  const uint32_t head_bias = base + off.bias + head * kMaxBuckets * 4;
+  const uint8_t* near0 = s_buckets + (half * 16 + g) * kBucketRow + 8 * t;
+  const uint32_t hist = smem_u32(s_hist + tid);
+  const float unit = units.unit;
 
   typename F::A held_q[HOLD], held_d[BACK ? HOLD : 1];
   if constexpr (HELD) {
-    if (mine) hold<T, CP>(held_q, q_rows, half * 16, lane);
+    if (mine) hold<T, CP>(held_q, q_at, q_rs);
     if constexpr (BACK)
-      if (mine) hold<T, CP>(held_d, d_rows, half * 16, lane);
+      if (mine) hold<T, CP>(held_d, d_at, q_rs);
   }
-  float acc[CP / 8][4] = {};
-  float fine[EXACT ? CP / 8 : 1][4] = {};
+  Pair acc[CP / 8][2] = {};  // rows g and g + 8
+  Pair fine[EXACT ? CP / 8 : 1][2] = {};
   float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};  // forward: running maximum, sum
   float lse[2] = {INFINITY, INFINITY}, delta[2] = {0.0f, 0.0f};  // backward
   float lift = 1.0f;  // float16: power of two that brings the gradients to order 1
@@ -221,110 +229,91 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
     lift = gradient_lift<T>(a);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int row = s_qrows[half * 16 + g + 8 * r];
+      const int row = s_rows[half * 16 + g + 8 * r];
       if (mine && row >= 0) {
         lse[r] = a.lse_in[int64_t(row) * a.heads + span.h0 + head];
-        delta[r] = a.delta[int64_t(row) * a.heads + span.h0 + head] * lift;
+        delta[r] = a.delta[int64_t(row) * a.heads + span.h0 + head];
       }
     }
   }
 
+  uint2 entry = steps > 0 ? entries[0] : make_uint2(0, 0), next = entry;
   for (int i = 0; i < steps; ++i) {
     cp_wait<0>();
     __syncthreads();
-    copy(i + 1);
-    fetch(i + 2);
-    sort_pairs(i + 1);
-    const uint2 entry = entries[i >> 1];
+    if (i + 1 < steps) {
+      if (i & 1) next = entries[(i + 1) >> 1];
+      copy(i + 1);
+      fetch(i + 2);
+      if (bias) sort_pairs(i + 1);
+    }
+    cp_commit();
     const unsigned mask = entry.y >> (half * 16);
-    const int64_t left = c.n - int64_t(entry.x) * kBlockLeaves - (i & 1) * kStepLeaves;
-    if (mine && (mask & 0xffffu) && left > 0) {
-      const int slot = i & 1;
-      const T* k_tile = s_k + slot * stage + kv * kv_tile;
-      const T* v_tile = s_v + slot * stage + kv * kv_tile;
-      const bool on[2] = {(mask >> g & 1u) != 0, (mask >> (g + 8) & 1u) != 0};
-      const uint8_t* near = s_buckets + (slot * kTileQueries + half * 16 + g) * BROW + 2 * t;
-      float s[NT][4];
-      auto read_bias = [&]() {
+    const int left = points - first_leaf(entry.x, i);
+    entry = next;
+    if (!mine || (mask & 0xffffu) == 0 || left <= 0) {
+      put(i + 2);
+      continue;
+    }
+    const int slot = i & 1;
+    const uint32_t k_at = k_at0 + slot * stage, v_at = v_at0 + slot * stage;
+    const uint32_t on[2] = {mask >> g & 1u, mask >> (g + 8) & 1u};
+    const uint8_t* near = near0 + slot * kTileQueries * kBucketRow;
+    float s[NT][4];
+    logits<T, CP, HELD>(s, held_q, q_at, q_rs, k_at + nk, kv_rs, bias, head_bias, near, 8 * kBucketRow,
+                        a.scale * kLog2e, units.folded);
+    if (left < kStepLeaves) {  // the cloud's last leaves
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n * 8 + 2 * t + (j & 1) >= left) s[n][j] = -INFINITY;
+    }
+    if constexpr (!BACK) {
+      Pair shrink[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float most = top[r];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) most = max3(most, s[n][2 * r], s[n][2 * r + 1]);
+        most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
+        const float from_top = most == -INFINITY ? 0.0f : -most * unit;  // nothing yet: all p are 0
+        const float fade = exp2_fast(fmaf(top[r], unit, from_top));
+        Pair add = both(0.0f);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const uint32_t lo = *reinterpret_cast<const uint16_t*>(near + n * 8);
-          const uint32_t hi = *reinterpret_cast<const uint16_t*>(near + 8 * BROW + n * 8);
-          s[n][0] = *reinterpret_cast<const float*>(head_bias + (lo & 255));
-          s[n][1] = *reinterpret_cast<const float*>(head_bias + (lo >> 8));
-          s[n][2] = *reinterpret_cast<const float*>(head_bias + (hi & 255));
-          s[n][3] = *reinterpret_cast<const float*>(head_bias + (hi >> 8));
+          const float2 x = unpair(fma2(pair(s[n][2 * r], s[n][2 * r + 1]), both(unit), both(from_top)));
+          s[n][2 * r] = exp2_fast(x.x);
+          s[n][2 * r + 1] = exp2_fast(x.y);
+          add = add2(add, pair(s[n][2 * r], s[n][2 * r + 1]));
         }
-      };
-      if (bias && folded) {
-        read_bias();
-        multiply_nk<T, CP, NT, HELD>(s, held_q, q_rows, half * 16, k_tile, 0, lane);
-      } else {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[n][j] = 0.0f;
-        multiply_nk<T, CP, NT, HELD>(s, held_q, q_rows, half * 16, k_tile, 0, lane);
-        if (!folded) {
-          float x[NT][4];
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              x[n][j] = s[n][j] * (a.scale * kLog2e);
-              s[n][j] = 0.0f;
-            }
-          if (bias) read_bias();
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[n][j] += x[n][j];
+        if (on[r]) {
+          top[r] = most;
+          sum[r] = fmaf(sum[r], fade, unpair(add).x + unpair(add).y);
         }
+        shrink[r] = both(fade);
       }
-      if (left < kStepLeaves) {  // the cloud's last leaves
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+      for (int n0 = 0; n0 < CP / 8; n0 += kChannelGroup) {
+        float part[kChannelGroup][4], low[EXACT ? kChannelGroup : 1][4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (n * 8 + 2 * t + (j & 1) >= left) s[n][j] = -INFINITY;
-      }
-      if constexpr (!BACK) {
-        float shrink[2];
+        for (int st = 0; st < STEPS; ++st) {
+          typename F::A p, rest;
+          from_acc<T>(p, s, st);
+          if constexpr (EXACT) rest_of_acc<T>(rest, p, s, st);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float most = top[r];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) most = fmaxf(most, fmaxf(s[n][2 * r], s[n][2 * r + 1]));
-          most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
-          most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
-          const float base = most == -INFINITY ? 0.0f : most * unit;  // nothing yet: all p are 0
-          shrink[r] = exp2_fast(fmaf(top[r], unit, -base));
-          float add = 0.0f;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              s[n][2 * r + j] = exp2_fast(fmaf(s[n][2 * r + j], unit, -base));
-              add += s[n][2 * r + j];
-            }
-          }
-          if (on[r]) {
-            top[r] = most;
-            sum[r] = fmaf(sum[r], shrink[r], add);
-          }
-        }
-#pragma unroll
-        for (int n0 = 0; n0 < CP / 8; n0 += kChannelGroup) {
-          float part[kChannelGroup][4] = {}, low[EXACT ? kChannelGroup : 1][4] = {};
-#pragma unroll
-          for (int st = 0; st < STEPS; ++st) {
-            typename F::A p, rest;
-            from_acc<T>(p, s, st);
-            if constexpr (EXACT) rest_of_acc<T>(rest, p, s, st);
-#pragma unroll
-            for (int j = 0; j < kChannelGroup / 2; ++j) {
-              typename F::B b;
-              F::pair_kn(b, v_tile, LD, st * F::STEP, (n0 + 2 * j) * 8, lane);
+          for (int j = 0; j < kChannelGroup / 2; ++j) {
+            typename F::B b;
+            F::pair_kn(b, v_at + kn + st * F::STEP * kv_rs + (n0 + 2 * j) * 8 * SIZE, kv_rs);
+            if (st == 0) {
+              F::mma_first(part[2 * j], p, b[0], b[1]);
+              F::mma_first(part[2 * j + 1], p, b[2], b[3]);
+              if constexpr (EXACT) {
+                F::mma_first(low[2 * j], rest, b[0], b[1]);
+                F::mma_first(low[2 * j + 1], rest, b[2], b[3]);
+              }
+            } else {
               F::mma(part[2 * j], p, b[0], b[1]);
               F::mma(part[2 * j + 1], p, b[2], b[3]);
               if constexpr (EXACT) {
@@ -333,58 +322,66 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
               }
             }
           }
-#pragma unroll
-          for (int j = 0; j < kChannelGroup; ++j)
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (on[x >> 1]) {
-                acc[n0 + j][x] = fmaf(acc[n0 + j][x], shrink[x >> 1], part[j][x]);
-                if constexpr (EXACT) fine[n0 + j][x] = fmaf(fine[n0 + j][x], shrink[x >> 1], low[j][x]);
-              }
         }
-      } else {
-        float ds[NT][4] = {};
-        multiply_nk<T, CP, NT, HELD>(ds, held_d, d_rows, half * 16, v_tile, 0, lane);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int r = 0; r < 2; ++r) {
+          keep_group(acc, n0, r, shrink[r], part, on[r]);
+          if constexpr (EXACT) keep_group(fine, n0, r, shrink[r], low, on[r]);
+        }
+      }
+    } else {
+      float ds[NT][4];
+      multiply_nk<T, CP, NT, HELD, true>(ds, held_d, d_at, q_rs, v_at + nk, kv_rs);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            ds[n][j] = exp2_fast(fmaf(s[n][j], unit, -lse[j >> 1])) * fmaf(ds[n][j], lift, -delta[j >> 1]);
-        if (bias) {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            if (on[r]) {
+        for (int r = 0; r < 2; ++r) {
+          const float2 x = unpair(fma2(pair(s[n][2 * r], s[n][2 * r + 1]), both(unit), both(-lse[r])));
+          Pair p = pair(exp2_fast(x.x), exp2_fast(x.y));
+          if constexpr (sizeof(T) == 2) p = mul2(p, both(lift));
+          p = mul2(p, add2(pair(ds[n][2 * r], ds[n][2 * r + 1]), both(-delta[r])));
+          ds[n][2 * r] = unpair(p).x;
+          ds[n][2 * r + 1] = unpair(p).y;
+        }
+      if (bias) {
 #pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                const uint32_t b = *reinterpret_cast<const uint16_t*>(near + r * 8 * BROW + n * 8);
-                // Each thread has a column of its own.
-                *reinterpret_cast<float*>(hist + (b & 255) * blockDim.x) += ds[n][2 * r];
-                *reinterpret_cast<float*>(hist + (b >> 8) * blockDim.x) += ds[n][2 * r + 1];
+        for (int r = 0; r < 2; ++r) {
+          if (on[r]) {
+            const uint2 b = *reinterpret_cast<const uint2*>(near + r * 8 * kBucketRow);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {  // each thread has a column of its own
+                const uint32_t at =
+                    hist + __byte_perm(n < 2 ? b.x : b.y, 0, 0x4440 + (n & 1) * 2 + j) * blockDim.x;
+                const float x = lds_f32(at) + ds[n][2 * r + j];
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(x) : "memory");
               }
-            }
           }
         }
+      }
 #pragma unroll
-        for (int n0 = 0; n0 < CP / 8; n0 += kChannelGroup) {
-          float part[kChannelGroup][4] = {};
+      for (int n0 = 0; n0 < CP / 8; n0 += kChannelGroup) {
+        float part[kChannelGroup][4];
 #pragma unroll
-          for (int st = 0; st < STEPS; ++st) {
-            typename F::A p;
-            from_acc<T>(p, ds, st);
+        for (int st = 0; st < STEPS; ++st) {
+          typename F::A p;
+          from_acc<T>(p, ds, st);
 #pragma unroll
-            for (int j = 0; j < kChannelGroup / 2; ++j) {
-              typename F::B b;
-              F::pair_kn(b, k_tile, LD, st * F::STEP, (n0 + 2 * j) * 8, lane);
+          for (int j = 0; j < kChannelGroup / 2; ++j) {
+            typename F::B b;
+            F::pair_kn(b, k_at + kn + st * F::STEP * kv_rs + (n0 + 2 * j) * 8 * SIZE, kv_rs);
+            if (st == 0) {
+              F::mma_first(part[2 * j], p, b[0], b[1]);
+              F::mma_first(part[2 * j + 1], p, b[2], b[3]);
+            } else {
               F::mma(part[2 * j], p, b[0], b[1]);
               F::mma(part[2 * j + 1], p, b[2], b[3]);
             }
           }
-#pragma unroll
-          for (int j = 0; j < kChannelGroup; ++j)
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (on[x >> 1]) acc[n0 + j][x] += part[j][x];
         }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) keep_group(acc, n0, r, both(1.0f), part, on[r]);
       }
     }
     put(i + 2);
@@ -397,7 +394,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
         sum[r] += __shfl_xor_sync(kFullMask, sum[r], 1);
         sum[r] += __shfl_xor_sync(kFullMask, sum[r], 2);
         const int q = half * 16 + g + 8 * r;
-        const int row = s_qrows[q];
+        const int row = s_rows[q];
         if (splits > 1) {
           const int64_t slot = ((int64_t(blockIdx.z) * a.map.num_tiles + tile) * a.heads + span.h0 + head) *
                                    kTileQueries + q;
@@ -408,11 +405,13 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
           }
 #pragma unroll
           for (int n = 0; n < CP / 8; ++n) {
-            part[2 + n * 8 + 2 * t] = acc[n][2 * r];
-            part[2 + n * 8 + 2 * t + 1] = acc[n][2 * r + 1];
+            const float2 o = unpair(acc[n][r]);
+            part[2 + n * 8 + 2 * t] = o.x;
+            part[2 + n * 8 + 2 * t + 1] = o.y;
             if constexpr (EXACT) {
-              part[2 + CP + n * 8 + 2 * t] = fine[n][2 * r];
-              part[2 + CP + n * 8 + 2 * t + 1] = fine[n][2 * r + 1];
+              const float2 f = unpair(fine[n][r]);
+              part[2 + CP + n * 8 + 2 * t] = f.x;
+              part[2 + CP + n * 8 + 2 * t + 1] = f.y;
             }
           }
           continue;
@@ -422,13 +421,13 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
         T* out = static_cast<T*>(a.out) + (int64_t(row) * a.heads + span.h0 + head) * a.channels;
 #pragma unroll
         for (int n = 0; n < CP / 8; ++n)
-          store_pair(out, n * 8 + 2 * t, a.channels, acc[n][2 * r] * inv, acc[n][2 * r + 1] * inv, a.wide_out);
+          store_pair(out, n * 8 + 2 * t, a.channels, unpair(acc[n][r]).x * inv, unpair(acc[n][r]).y * inv, a.wide_out);
         if constexpr (EXACT) {
           float* exact = a.out_exact + (int64_t(row) * a.heads + span.h0 + head) * a.channels;
 #pragma unroll
           for (int n = 0; n < CP / 8; ++n)
-            store_pair(exact, n * 8 + 2 * t, a.channels, (acc[n][2 * r] + fine[n][2 * r]) * inv,
-                       (acc[n][2 * r + 1] + fine[n][2 * r + 1]) * inv, false);
+            store_pair(exact, n * 8 + 2 * t, a.channels, (unpair(acc[n][r]).x + unpair(fine[n][r]).x) * inv,
+                       (unpair(acc[n][r]).y + unpair(fine[n][r]).y) * inv, false);
         }
         // An empty row keeps +inf: its probabilities come out as 0 in the backward pass.
         if (a.lse != nullptr && t == 0)
@@ -438,12 +437,12 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
       const float back = a.scale / lift;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int row = s_qrows[half * 16 + g + 8 * r];
+        const int row = s_rows[half * 16 + g + 8 * r];
         if (row < 0) continue;
         T* out = static_cast<T*>(a.grad_q) + (int64_t(row) * a.heads + span.h0 + head) * a.channels;
 #pragma unroll
         for (int n = 0; n < CP / 8; ++n)
-          store_pair(out, n * 8 + 2 * t, a.channels, acc[n][2 * r] * back, acc[n][2 * r + 1] * back, a.wide_out);
+          store_pair(out, n * 8 + 2 * t, a.channels, unpair(acc[n][r]).x * back, unpair(acc[n][r]).y * back, a.wide_out);
       }
     }
   }
