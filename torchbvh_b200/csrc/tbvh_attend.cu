@@ -1,5 +1,6 @@
 // C entries of block attention: argument checks, launch plans, and the small
 // kernels around the two backward passes.
+#include <algorithm>
 #include <climits>
 
 #include "tbvh_attend_q.cuh"
@@ -145,6 +146,14 @@ AttendArgs common_args(const tbvh_block_geometry* g, const tbvh_attend_features*
   return a;
 }
 
+// Row copies place rows by 32-bit counts of 16-byte words; tensors past 64 GB
+// take the narrower copies, which count in 64 bits.
+bool words_fit(const BlockSetup& s, const tbvh_attend_features* f) {
+  const int64_t size = element_size(f->dtype);
+  const int64_t most = std::max(s.total_points * f->kv_heads, s.total_queries * f->heads);
+  return most * f->channels * size / 16 < (int64_t(1) << 32);
+}
+
 bool pairs_aligned(int channels, const void* p) { return channels % 2 == 0 && uintptr_t(p) % 4 == 0; }
 
 }  // namespace
@@ -182,6 +191,7 @@ int tbvh_attend_blocks(const tbvh_block_geometry* g, const tbvh_attend_features*
     return blocks_fail(TBVH_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the required %zu", op,
                        workspace_bytes, need);
   a.width = copy_width(size_t(f->channels) * element_size(f->dtype), f->queries, f->keys, f->values);
+  if (!words_fit(s, f)) a.width = std::min(a.width, 8);
   a.wide_out = pairs_aligned(f->channels, out);
   a.out = out;
   a.lse = lse;
@@ -244,6 +254,7 @@ int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_
   a.width = copy_width(row_bytes, f->queries, f->keys, f->values);
   const int grad_width = copy_width(row_bytes, grad_out, nullptr, nullptr);
   if (grad_width < a.width) a.width = grad_width;
+  if (!words_fit(s, f)) a.width = std::min(a.width, 8);
   a.wide_out = (!grad_queries || pairs_aligned(f->channels, grad_queries)) &&
                (!grad_keys || (pairs_aligned(f->channels, grad_keys) && pairs_aligned(f->channels, grad_values)));
 

@@ -302,6 +302,9 @@ __device__ __forceinline__ void rest_of_acc(typename Frag<T>::A& rest, const typ
 }
 
 // ---- tiles in shared memory -----------------------------------------------------------
+// Rows past a block's or a list's end repeat its last row: their weights are
+// zero, and whoever meets that row's non-finite values has met them already.
+//
 // [row][head][CP channels], CP the channels rounded up, and 16 bytes of padding
 // a row: an odd number of 16-byte words, which puts the eight rows that a
 // fragment load touches at once into different banks. A row of whole heads is
@@ -394,44 +397,41 @@ struct Rows {
   }
 };
 
-// The copy of every step, two tensors of one shape at a time, where a row's
+// The copy of every step, 32 rows of two tensors of one shape, where a row's
 // heads are one run of whole 16-byte words on both sides: a thread keeps one
-// word of the row and every `at_once`-th row, and finds the row's place in the
-// tensors, in bytes, in shared memory (row_place). (Bulk copies of a row each
-// were measured at 1.7 times this form's step: one thread issues them one by one.)
+// word of the row and pairs of neighbouring rows, whose places in the tensors
+// (in 16-byte words) it finds in shared memory. (Bulk copies of a row each were
+// measured at 1.7 times this form's step: one thread issues them one by one.)
 struct RowWords {
-  uint32_t dst, dst_step;
-  int row0, at_once;  // at_once 0: not this shape
+  uint32_t dst;
+  int pair0, pairs_at_once;  // 0: not this shape
   const char *a, *b;
 
   __device__ __forceinline__ RowWords(const void* a_, const void* b_, int size, int cp, int channels, int first, int here,
                                       int step, int width, uint32_t rs) {
     const int columns = here * cp * size / 16, column = int(threadIdx.x) % columns;
-    at_once = width == 16 && channels == cp && (step == 1 || here == 1) ? int(blockDim.x) / columns : 0;
-    row0 = int(threadIdx.x) / columns;
-    dst = row0 * rs + column * 16;
-    dst_step = at_once * rs;
-    if (row0 >= at_once) row0 = 1 << 20;  // no row
+    pairs_at_once = width == 16 && channels == cp && (step == 1 || here == 1) ? int(blockDim.x) / columns : 0;
+    pair0 = int(threadIdx.x) / columns;
+    dst = pair0 * 2 * rs + column * 16;
+    if (pair0 >= pairs_at_once) pair0 = 1 << 20;  // no row
     const int64_t begin = int64_t(first) * cp * size + column * 16;
     a = static_cast<const char*>(a_) + begin;
     b = static_cast<const char*>(b_) + begin;
   }
-  __device__ __forceinline__ void copy(uint32_t a_tile, uint32_t b_tile, const uint64_t* places, int count) const {
+  __device__ __forceinline__ void copy(uint32_t a_tile, uint32_t b_tile, const uint32_t* places, uint32_t rs) const {
     uint32_t to = dst;
-    for (int r = row0; r < count; r += at_once, to += dst_step) {
-      const uint64_t place = places[r];
-      const int size = place & 1 ? 0 : 16;
-      const uint64_t at = place & ~uint64_t(1);
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(a_tile + to), "l"(a + at), "r"(size) : "memory");
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(b_tile + to), "l"(b + at), "r"(size) : "memory");
+    for (int p = pair0; p < 16; p += pairs_at_once, to += pairs_at_once * 2 * rs) {
+      const uint2 place = reinterpret_cast<const uint2*>(places)[p];
+      put(a_tile + to, a, place.x);
+      put(b_tile + to, b, place.x);
+      put(a_tile + to + rs, a, place.y);
+      put(b_tile + to + rs, b, place.y);
     }
   }
+  static __device__ __forceinline__ void put(uint32_t dst, const char* from, uint32_t place) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from + uint64_t(place) * 16) : "memory");
+  }
 };
-
-// Bytes from a tensor's start to row `row` of `row_bytes` (a multiple of 16); odd: a row of zeros.
-__device__ __forceinline__ uint64_t row_place(int row, uint32_t row_bytes) {
-  return row < 0 ? 1 : uint64_t(uint32_t(row)) * row_bytes;
-}
 
 // Zeros in the padding channels of tiles, which copies never write.
 template <typename T, int CP>
@@ -529,7 +529,9 @@ __device__ __forceinline__ float pair_distance(float4 minus_p, float x, float y,
 // and every blockDim / 8-th row.
 template <bool CROWDED>
 __device__ __forceinline__ void sort_step(uint8_t* to, int row_bytes, const BucketTable& table, const float4* p,
-                                          int rows, const float* pts) {
+                                          int rows, const float* pts, uint32_t wanted) {
+  // Four rows a warp and pass; those that no one wants are left out (rows 32 apart share a bit).
+  if ((wanted >> (threadIdx.x / 32 * 4 % 32) & 15u) == 0 && blockDim.x >= 256) return;
   const int part = threadIdx.x % 8;  // 2 t + (upper groups)
   const float* c = pts + (part & 1) * 16 + (part >> 1) * 2;
   const float2 x0 = *reinterpret_cast<const float2*>(c), x1 = *reinterpret_cast<const float2*>(c + 8);
@@ -665,19 +667,20 @@ __device__ __forceinline__ float gradient_lift(const AttendArgs& a) {
   return exp2f(-floorf(log2f(most)));
 }
 
-// Packed row of index `i` of a cloud's order.
-__device__ __forceinline__ int checked_row(const AttendArgs& a, const BlockCloud& c, int64_t i) {
-  if (uint64_t(i) >= uint64_t(c.n)) {
+// Packed row of index `i` of a cloud's order (of its first point, and an error
+// bit, where it is none).
+__device__ __forceinline__ uint32_t checked_row(const AttendArgs& a, const BlockCloud& c, uint32_t i) {
+  if (i >= uint32_t(c.n)) {
     if (a.status) atomicOr(a.status, kDevErrBadIndex);
-    return -1;
+    i = 0;
   }
-  return int(c.p0 + i);
+  return uint32_t(c.p0) + i;
 }
 
 // Packed key row of leaf `leaf` of a cloud, or -1 past its end.
 __device__ __forceinline__ int key_row(const AttendArgs& a, const BlockCloud& c, int64_t leaf) {
   if (leaf >= c.n) return -1;
-  return checked_row(a, c, a.sorted[c.p0 + leaf]);
+  return int(checked_row(a, c, uint32_t(a.sorted[c.p0 + leaf])));
 }
 
 // First leaf row of a cloud's node rows.

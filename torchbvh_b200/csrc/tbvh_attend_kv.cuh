@@ -41,7 +41,7 @@ __host__ __device__ inline KeyBlockSmem key_block_smem(int size, int cp, int kvs
   s.d = take(2 * kTileQueries * row);
   s.lse = take(2 * kvs * kTileQueries * 4);
   s.delta = take(2 * kvs * kTileQueries * 4);
-  s.places = take(2 * kTileQueries * 8);
+  s.places = take(2 * kTileQueries * 4);
   s.rows = take(2 * kTileQueries * 4);
   s.krows = take(kBlockLeaves * 4);
   if (bias) {
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
   float* s_lse = reinterpret_cast<float*>(smem + off.lse);
   float* s_delta = reinterpret_cast<float*>(smem + off.delta);
   int* s_rows = reinterpret_cast<int*>(smem + off.rows);
-  uint64_t* s_places = reinterpret_cast<uint64_t*>(smem + off.places);
+  uint32_t* s_places = reinterpret_cast<uint32_t*>(smem + off.places);
   int* s_krows = reinterpret_cast<int*>(smem + off.krows);
   float* s_bias = reinterpret_cast<float*>(smem + off.bias);
   uint8_t* s_buckets = reinterpret_cast<uint8_t*>(smem + off.buckets);
@@ -102,26 +102,23 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
       s_kpts[tid] = tid < valid ? make_float4(-p[0], -p[1], a.dim == 3 ? -p[2] : 0.0f, 0.0f) : make_float4(0, 0, 0, 0);
     }
   }
-  int next_row = -1;
+  int next_row = 0;
   float next_pt[3] = {0.0f, 0.0f, 0.0f};
   auto fetch = [&](int e) {
     if (tid < kTileQueries && e < chunks) {
-      const int at = e * kTileQueries + tid;
-      next_row = -1;
-      if (at < listed) {
-        const uint32_t slot = list[at];
-        next_row = a.plan.query_row[slot];
-        if (bias)
-          for (int x = 0; x < 3; ++x)
-            next_pt[x] = a.plan.query_point[(int64_t(slot / kTileQueries) * 3 + x) * kTileQueries + slot % kTileQueries];
-      }
+      const uint32_t slot = list[min(e * kTileQueries + tid, listed - 1)];
+      next_row = a.plan.query_row[slot];
+      if (bias)
+        for (int x = 0; x < 3; ++x)
+          next_pt[x] = a.plan.query_point[(int64_t(slot / kTileQueries) * 3 + x) * kTileQueries + slot % kTileQueries];
     }
   };
+  const uint32_t row_words = a.heads * CP * SIZE / 16;
   auto put = [&](int e) {
     if (tid < kTileQueries && e < chunks) {
       const int slot = e & 1;
       s_rows[slot * kTileQueries + tid] = next_row;
-      s_places[slot * kTileQueries + tid] = row_place(next_row, a.heads * CP * SIZE);
+      s_places[slot * kTileQueries + tid] = uint32_t(next_row) * row_words;
       if (bias)
         for (int x = 0; x < 3; ++x) s_pts[(slot * 3 + x) * kTileQueries + tid] = next_pt[x];
     }
@@ -134,8 +131,8 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
       const int first = kv0 * group + member;
       const uint32_t to = base + slot * stage;
       const RowWords words(a.q, a.grad_out, SIZE, CP, a.channels, first, kvs, group, a.width, rs);
-      if (words.at_once) {
-        words.copy(to + off.q, to + off.d, s_places + (e & 1) * kTileQueries, kTileQueries);
+      if (words.pairs_at_once) {
+        words.copy(to + off.q, to + off.d, s_places + (e & 1) * kTileQueries, rs);
       } else {
         auto row_of = [&](int r) { return rows[r]; };
         const Rows<T, CP> q{static_cast<const T*>(a.q), a.heads, a.channels, first, kvs, group, a.width, rs};
@@ -144,13 +141,13 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
         d.copy(to + off.d, kTileQueries, row_of);
       }
       for (int i = tid; i < kvs * kTileQueries; i += blockDim.x) {
-        const int h = i / kTileQueries, q = i % kTileQueries, row = rows[q];
-        const int64_t at = int64_t(row < 0 ? 0 : row) * a.heads + (kv0 + h) * group + member;
+        const int h = i / kTileQueries, q = i % kTileQueries;
+        const int64_t at = int64_t(rows[q]) * a.heads + (kv0 + h) * group + member;
         float* lse = s_lse + (slot * a.kv_cta + h) * kTileQueries + q;
-        // Past the list's end the rows are zeros and the sum is infinite: p = 0.
-        if (row >= 0) cp_async<4>(smem_u32(lse), a.lse_in + at, true);
+        // Past the list's end the sum is infinite: p = 0.
+        if (e * kTileQueries + q < listed) cp_async<4>(smem_u32(lse), a.lse_in + at, true);
         else *lse = INFINITY;
-        cp_async<4>(smem_u32(s_delta + (slot * a.kv_cta + h) * kTileQueries + q), a.delta + at, row >= 0);
+        cp_async<4>(smem_u32(s_delta + (slot * a.kv_cta + h) * kTileQueries + q), a.delta + at, true);
       }
     }
     cp_commit();
@@ -160,8 +157,8 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
       const int slot = e & 1;
       uint8_t* to = s_buckets + slot * kBlockLeaves * kKeyBucketRow;
       const float* p = s_pts + slot * 3 * kTileQueries;
-      if (s_table.crowded) sort_step<true>(to, kKeyBucketRow, s_table, s_kpts, kBlockLeaves, p);
-      else sort_step<false>(to, kKeyBucketRow, s_table, s_kpts, kBlockLeaves, p);
+      if (s_table.crowded) sort_step<true>(to, kKeyBucketRow, s_table, s_kpts, kBlockLeaves, p, ~0u);
+      else sort_step<false>(to, kKeyBucketRow, s_table, s_kpts, kBlockLeaves, p, ~0u);
     }
   };
 

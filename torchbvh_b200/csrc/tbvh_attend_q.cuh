@@ -53,7 +53,7 @@ __host__ __device__ inline QueryTileSmem query_tile_smem(int size, int cp, int k
   s.v = take(2 * kStepLeaves * kv_row);
   s.q = take(kTileQueries * q_row);
   s.d = back ? take(kTileQueries * q_row) : 0;
-  s.places = take(2 * kStepLeaves * 8);
+  s.places = take(2 * kStepLeaves * 4);
   s.rows = take(kTileQueries * 4);
   if (bias) {
     s.buckets = take(2 * kTileQueries * kBucketRow);
@@ -66,14 +66,20 @@ __host__ __device__ inline QueryTileSmem query_tile_smem(int size, int cp, int k
   return s;
 }
 
-// Row r of a group of accumulator tiles from n0: old * factor + part where `on`.
+// Row r of a group of accumulator tiles from n0: old * factor + part where `on`
+// (`every`: known to be on in the whole warp).
 template <int N>
 __device__ __forceinline__ void keep_group(Pair (&acc)[N][2], int n0, int r, Pair factor,
-                                           const float (&part)[kChannelGroup][4], uint32_t on) {
+                                           const float (&part)[kChannelGroup][4], uint32_t on, bool every) {
   static_assert(kChannelGroup == 4, "one group is four tiles");
-  keep_where(acc[n0][r], acc[n0 + 1][r], acc[n0 + 2][r], acc[n0 + 3][r], factor, pair(part[0][2 * r], part[0][2 * r + 1]),
-             pair(part[1][2 * r], part[1][2 * r + 1]), pair(part[2][2 * r], part[2][2 * r + 1]),
-             pair(part[3][2 * r], part[3][2 * r + 1]), on);
+  const Pair p[4] = {pair(part[0][2 * r], part[0][2 * r + 1]), pair(part[1][2 * r], part[1][2 * r + 1]),
+                     pair(part[2][2 * r], part[2][2 * r + 1]), pair(part[3][2 * r], part[3][2 * r + 1])};
+  if (every) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[n0 + j][r] = fma2(acc[n0 + j][r], factor, p[j]);
+  } else {
+    keep_where(acc[n0][r], acc[n0 + 1][r], acc[n0 + 2][r], acc[n0 + 3][r], factor, p[0], p[1], p[2], p[3], on);
+  }
 }
 
 // Registers: with 32 padded channels three blocks of eight warps share an SM.
@@ -95,14 +101,14 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   const bool bias = a.table != nullptr;
   const QueryTileSmem off = query_tile_smem(SIZE, CP, a.kv_cta, a.heads_cta, BACK, bias, a.buckets);
   const uint32_t base = smem_u32(smem);
-  uint64_t* s_places = reinterpret_cast<uint64_t*>(smem + off.places);
+  uint32_t* s_places = reinterpret_cast<uint32_t*>(smem + off.places);
   int* s_rows = reinterpret_cast<int*>(smem + off.rows);
   uint8_t* s_buckets = reinterpret_cast<uint8_t*>(smem + off.buckets);
   float* s_hist = reinterpret_cast<float*>(smem + off.hist);
   const uint32_t kv_rs = row_bytes<T, CP>(a.kv_cta), q_rs = row_bytes<T, CP>(a.heads_cta);
   const uint32_t stage = kStepLeaves * kv_rs;
   const RowWords words(a.k, a.v, SIZE, CP, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs);
-  const uint32_t place_unit = words.at_once ? a.kv_heads * CP * SIZE : 16;  // other shapes keep the row number
+  const uint32_t row_words = words.pairs_at_once ? a.kv_heads * CP * SIZE / 16 : 1;  // other shapes keep the row number
 
   const int all = a.plan.tile_count[tile];
   const int splits = BACK ? 1 : a.splits;
@@ -117,47 +123,45 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   auto first_leaf = [&](uint32_t block, int i) { return int(block) * kBlockLeaves + (i & 1) * kStepLeaves; };
   // Rows and points of a step's leaves, one leaf a lane of the first warp: asked
   // for two steps ahead, put down for the others one step ahead.
-  int64_t next_index = -1;
+  uint32_t next_index = 0;
   auto fetch = [&](int i) {
     if (warp == 0 && i < steps) {
-      const int leaf = first_leaf(entries[i >> 1].x, i) + lane;
-      const bool there = leaf < points;
-      next_index = there ? sorted[leaf] : -1;
+      const int leaf = min(first_leaf(entries[i >> 1].x, i) + lane, points - 1);
+      next_index = uint32_t(sorted[leaf]);
       if (bias) {
-        const float* p = leaf_points + int64_t(there ? leaf : 0) * 2 * a.dim;
+        const float* p = leaf_points + int64_t(leaf) * 2 * a.dim;
         const uint32_t to = base + off.pts + ((i & 1) * 3 * kStepLeaves + lane) * 4;
-        cp_async<4>(to, p, there);
-        cp_async<4>(to + 4 * kStepLeaves, p + 1, there);
-        cp_async<4>(to + 8 * kStepLeaves, p + a.dim - 1, there && a.dim == 3);
+        cp_async<4>(to, p, true);
+        cp_async<4>(to + 4 * kStepLeaves, p + 1, true);
+        cp_async<4>(to + 8 * kStepLeaves, p + a.dim - 1, a.dim == 3);
       }
     }
   };
   auto put = [&](int i) {
     if (warp == 0 && i < steps)
-      s_places[(i & 1) * kStepLeaves + lane] =
-          row_place(next_index < 0 ? -1 : checked_row(a, c, next_index), place_unit);
+      s_places[(i & 1) * kStepLeaves + lane] = checked_row(a, c, next_index) * row_words;
   };
   auto copy = [&](int i) {
     const uint32_t at = base + (i & 1) * stage;
-    const uint64_t* places = s_places + (i & 1) * kStepLeaves;
-    if (words.at_once) {
-      words.copy(at + off.k, at + off.v, places, kStepLeaves);
+    const uint32_t* places = s_places + (i & 1) * kStepLeaves;
+    if (words.pairs_at_once) {
+      words.copy(at + off.k, at + off.v, places, kv_rs);
     } else {
-      auto row_of = [&](int r) { return places[r] & 1 ? -1 : int(places[r] / 16); };
+      auto row_of = [&](int r) { return int(places[r]); };
       const Rows<T, CP> keys{static_cast<const T*>(a.k), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
       const Rows<T, CP> values{static_cast<const T*>(a.v), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
       keys.copy(at + off.k, kStepLeaves, row_of);
       values.copy(at + off.v, kStepLeaves, row_of);
     }
   };
-  auto sort_pairs = [&](int i) {  // distance buckets of step i
+  auto sort_pairs = [&](int i, uint32_t mask) {  // distance buckets of step i, for the queries of `mask`
     const int slot = i & 1;
     const BucketTable& table = *reinterpret_cast<const BucketTable*>(smem + off.table);
     uint8_t* to = s_buckets + slot * kTileQueries * kBucketRow;
     const float4* q = reinterpret_cast<const float4*>(smem + off.qpts);
     const float* p = reinterpret_cast<const float*>(smem + off.pts) + slot * 3 * kStepLeaves;
-    if (table.crowded) sort_step<true>(to, kBucketRow, table, q, kTileQueries, p);
-    else sort_step<false>(to, kBucketRow, table, q, kTileQueries, p);
+    if (table.crowded) sort_step<true>(to, kBucketRow, table, q, kTileQueries, p, mask);
+    else sort_step<false>(to, kBucketRow, table, q, kTileQueries, p, mask);
   };
 
   clear_padding<T, CP>(smem + off.k, kv_rs, 2 * kStepLeaves, a.kv_cta, a.channels);
@@ -178,6 +182,9 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
     float* s_bias = reinterpret_cast<float*>(smem + off.bias);
     for (int i = tid; i < span.heads * a.buckets; i += blockDim.x)
       s_bias[(i / a.buckets) * kMaxBuckets + i % a.buckets] = a.table[int64_t(span.h0) * a.buckets + i] * units.bias;
+    // Rows that a step leaves unsorted are still looked up (and dropped): they must hold offsets.
+    for (int i = tid; i < 2 * kTileQueries * kBucketRow / 4; i += blockDim.x)
+      reinterpret_cast<uint32_t*>(s_buckets)[i] = 0;
     if constexpr (BACK)
       for (int i = tid; i < a.buckets * int(blockDim.x); i += blockDim.x) s_hist[i] = 0.0f;
   }
@@ -198,7 +205,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   if (bias) reinterpret_cast<BucketTable*>(smem + off.table)->make(a.edges, a.buckets - 1);
   cp_wait<0>();
   __syncthreads();
-  if (bias && steps > 0) sort_pairs(0);
+  if (bias && steps > 0) sort_pairs(0, entries[0].y);
 
   const int head = warp >> 1, half = warp & 1;
   const bool mine = head < span.heads;
@@ -245,7 +252,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
       if (i & 1) next = entries[(i + 1) >> 1];
       copy(i + 1);
       fetch(i + 2);
-      if (bias) sort_pairs(i + 1);
+      if (bias) sort_pairs(i + 1, next.y);
     }
     cp_commit();
     const unsigned mask = entry.y >> (half * 16);
@@ -258,11 +265,13 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
     const int slot = i & 1;
     const uint32_t k_at = k_at0 + slot * stage, v_at = v_at0 + slot * stage;
     const uint32_t on[2] = {mask >> g & 1u, mask >> (g + 8) & 1u};
+    const bool every = (mask & 0xffffu) == 0xffffu;  // all 16 rows, the same for the warp
     const uint8_t* near = near0 + slot * kTileQueries * kBucketRow;
     float s[NT][4];
     logits<T, CP, HELD>(s, held_q, q_at, q_rs, k_at + nk, kv_rs, bias, head_bias, near, 8 * kBucketRow,
                         a.scale * kLog2e, units.folded);
     if (left < kStepLeaves) {  // the cloud's last leaves
+      asm volatile("" ::: "memory");  // a branch, not 32 selections in every step
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -325,8 +334,8 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          keep_group(acc, n0, r, shrink[r], part, on[r]);
-          if constexpr (EXACT) keep_group(fine, n0, r, shrink[r], low, on[r]);
+          keep_group(acc, n0, r, shrink[r], part, on[r], every);
+          if constexpr (EXACT) keep_group(fine, n0, r, shrink[r], low, on[r], every);
         }
       }
     } else {
@@ -381,7 +390,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
           }
         }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) keep_group(acc, n0, r, both(1.0f), part, on[r]);
+        for (int r = 0; r < 2; ++r) keep_group(acc, n0, r, both(1.0f), part, on[r], every);
       }
     }
     put(i + 2);
