@@ -397,41 +397,49 @@ struct Rows {
   }
 };
 
-// The copy of every step, 32 rows of two tensors of one shape, where a row's
-// heads are one run of whole 16-byte words on both sides: a thread keeps one
-// word of the row and pairs of neighbouring rows, whose places in the tensors
-// (in 16-byte words) it finds in shared memory. (Bulk copies of a row each were
-// measured at 1.7 times this form's step: one thread issues them one by one.)
-struct RowWords {
-  uint32_t dst;
-  int pair0, pairs_at_once;  // 0: not this shape
-  const char *a, *b;
-
-  __device__ __forceinline__ RowWords(const void* a_, const void* b_, int size, int cp, int channels, int first, int here,
-                                      int step, int width, uint32_t rs) {
-    const int columns = here * cp * size / 16, column = int(threadIdx.x) % columns;
-    pairs_at_once = width == 16 && channels == cp && (step == 1 || here == 1) ? int(blockDim.x) / columns : 0;
-    pair0 = int(threadIdx.x) / columns;
-    dst = pair0 * 2 * rs + column * 16;
-    if (pair0 >= pairs_at_once) pair0 = 1 << 20;  // no row
-    const int64_t begin = int64_t(first) * cp * size + column * 16;
-    a = static_cast<const char*>(a_) + begin;
-    b = static_cast<const char*>(b_) + begin;
-  }
-  __device__ __forceinline__ void copy(uint32_t a_tile, uint32_t b_tile, const uint32_t* places, uint32_t rs) const {
-    uint32_t to = dst;
-    for (int p = pair0; p < 16; p += pairs_at_once, to += pairs_at_once * 2 * rs) {
-      const uint2 place = reinterpret_cast<const uint2*>(places)[p];
-      put(a_tile + to, a, place.x);
-      put(b_tile + to, b, place.x);
-      put(a_tile + to + rs, a, place.y);
-      put(b_tile + to + rs, b, place.y);
+// 32 rows of two tensors of one shape, copied by ONE warp, where a row's heads
+// are one run of `columns` whole 16-byte words on both sides: lane r holds row
+// r's place in the tensors, in words, and the lanes share the words of the rows.
+// The warps of a block take turns, a step each: the same copies spread over all
+// warps cost each of them its loop and addresses in every step, three times the
+// instructions. (Bulk copies of a row each, issued by one thread one by one,
+// took 1.7 times as long a step.)
+__device__ __forceinline__ void copy_words(uint32_t a_tile, uint32_t b_tile, const char* a, const char* b,
+                                           uint32_t place, int columns, uint32_t rs, int lane) {
+  auto put = [](uint32_t dst, const char* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  };
+  if (columns <= 32 && (columns & (columns - 1)) == 0) {
+    const int rows = 32 / columns, shift = 31 - __clz(columns);  // rows an instruction
+    const int column = lane & (columns - 1);
+    int r = lane >> shift;
+    uint32_t to = r * rs + column * 16;
+    const uint32_t step = rows * rs;
+    a += column * 16;
+    b += column * 16;
+#pragma unroll 4
+    for (int i = 0; i < columns; ++i, r += rows, to += step) {
+      const uint64_t at = uint64_t(__shfl_sync(kFullMask, place, r)) * 16;
+      put(a_tile + to, a + at);
+      put(b_tile + to, b + at);
+    }
+  } else {
+    int r = lane / columns, column = lane % columns;
+    const int dr = 32 / columns, dc = 32 % columns;
+    for (int i = 0; i < columns; ++i) {
+      const uint64_t at = (uint64_t(__shfl_sync(kFullMask, place, r)) + column) * 16;
+      const uint32_t to = r * rs + column * 16;
+      put(a_tile + to, a + at);
+      put(b_tile + to, b + at);
+      r += dr;
+      column += dc;
+      if (column >= columns) {
+        column -= columns;
+        ++r;
+      }
     }
   }
-  static __device__ __forceinline__ void put(uint32_t dst, const char* from, uint32_t place) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from + uint64_t(place) * 16) : "memory");
-  }
-};
+}
 
 // Zeros in the padding channels of tiles, which copies never write.
 template <typename T, int CP>

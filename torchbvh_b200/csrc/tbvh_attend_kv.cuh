@@ -102,55 +102,54 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
       s_kpts[tid] = tid < valid ? make_float4(-p[0], -p[1], a.dim == 3 ? -p[2] : 0.0f, 0.0f) : make_float4(0, 0, 0, 0);
     }
   }
+  // The warps take turns, a chunk each: a chunk's warp asks for its list elements
+  // three chunks ahead, for their rows and points two chunks ahead (one query a
+  // lane), and copies the rows one step ahead.
+  const bool whole = a.width == 16 && a.channels == CP && (group == 1 || kvs == 1);
+  const int columns = kvs * CP * int(SIZE) / 16, row_words = a.heads * CP * int(SIZE) / 16;
+  const int warps = int(blockDim.x) / 32;
+  uint32_t next_slot = 0;
   int next_row = 0;
   float next_pt[3] = {0.0f, 0.0f, 0.0f};
-  auto fetch = [&](int e) {
-    if (tid < kTileQueries && e < chunks) {
-      const uint32_t slot = list[min(e * kTileQueries + tid, listed - 1)];
-      next_row = a.plan.query_row[slot];
-      if (bias)
-        for (int x = 0; x < 3; ++x)
-          next_pt[x] = a.plan.query_point[(int64_t(slot / kTileQueries) * 3 + x) * kTileQueries + slot % kTileQueries];
+  auto ask_list = [&](int e) { next_slot = list[min(e * kTileQueries + lane, listed - 1)]; };
+  auto ask_rows = [&]() {
+    next_row = a.plan.query_row[next_slot];
+    if (bias) {
+      const float* p =
+          a.plan.query_point + int64_t(next_slot / kTileQueries) * 3 * kTileQueries + next_slot % kTileQueries;
+      for (int x = 0; x < 3; ++x) next_pt[x] = p[x * kTileQueries];
     }
   };
-  const uint32_t row_words = a.heads * CP * SIZE / 16;
   auto put = [&](int e) {
-    if (tid < kTileQueries && e < chunks) {
-      const int slot = e & 1;
-      s_rows[slot * kTileQueries + tid] = next_row;
-      s_places[slot * kTileQueries + tid] = uint32_t(next_row) * row_words;
-      if (bias)
-        for (int x = 0; x < 3; ++x) s_pts[(slot * 3 + x) * kTileQueries + tid] = next_pt[x];
-    }
+    s_rows[(e & 1) * kTileQueries + lane] = next_row;
+    if (bias)
+      for (int x = 0; x < 3; ++x) s_pts[((e & 1) * 3 + x) * kTileQueries + lane] = next_pt[x];
   };
-  auto copy = [&](int64_t step, int e, int member) {  // step = e * group + member
-    if (step < steps) {
-      const int slot = int(step & 1);
-      const int* rows = s_rows + (e & 1) * kTileQueries;
-      // Query heads kv * group + member, one a key/value head.
-      const int first = kv0 * group + member;
-      const uint32_t to = base + slot * stage;
-      const RowWords words(a.q, a.grad_out, SIZE, CP, a.channels, first, kvs, group, a.width, rs);
-      if (words.pairs_at_once) {
-        words.copy(to + off.q, to + off.d, s_places + (e & 1) * kTileQueries, rs);
-      } else {
-        auto row_of = [&](int r) { return rows[r]; };
-        const Rows<T, CP> q{static_cast<const T*>(a.q), a.heads, a.channels, first, kvs, group, a.width, rs};
-        const Rows<T, CP> d{static_cast<const T*>(a.grad_out), a.heads, a.channels, first, kvs, group, a.width, rs};
-        q.copy(to + off.q, kTileQueries, row_of);
-        d.copy(to + off.d, kTileQueries, row_of);
-      }
-      for (int i = tid; i < kvs * kTileQueries; i += blockDim.x) {
-        const int h = i / kTileQueries, q = i % kTileQueries;
-        const int64_t at = int64_t(rows[q]) * a.heads + (kv0 + h) * group + member;
-        float* lse = s_lse + (slot * a.kv_cta + h) * kTileQueries + q;
-        // Past the list's end the sum is infinite: p = 0.
-        if (e * kTileQueries + q < listed) cp_async<4>(smem_u32(lse), a.lse_in + at, true);
-        else *lse = INFINITY;
-        cp_async<4>(smem_u32(s_delta + (slot * a.kv_cta + h) * kTileQueries + q), a.delta + at, true);
-      }
+  auto copy = [&](int64_t step, int e, int member) {  // step = e * group + member, by one warp (or all)
+    const int slot = int(step & 1);
+    const int* rows = s_rows + (e & 1) * kTileQueries;
+    const int first = kv0 * group + member;  // query heads kv * group + member, one a key/value head
+    const uint32_t to = base + slot * stage;
+    if (whole) {
+      const int64_t begin = int64_t(first) * CP * SIZE;
+      copy_words(to + off.q, to + off.d, static_cast<const char*>(a.q) + begin,
+                 static_cast<const char*>(a.grad_out) + begin, uint32_t(rows[lane]) * row_words, columns, rs, lane);
+    } else {
+      auto row_of = [&](int r) { return rows[r]; };
+      const Rows<T, CP> q{static_cast<const T*>(a.q), a.heads, a.channels, first, kvs, group, a.width, rs};
+      const Rows<T, CP> d{static_cast<const T*>(a.grad_out), a.heads, a.channels, first, kvs, group, a.width, rs};
+      q.copy(to + off.q, kTileQueries, row_of);
+      d.copy(to + off.d, kTileQueries, row_of);
+      if (warp != 0) return;
     }
-    cp_commit();
+    for (int h = 0; h < kvs; ++h) {
+      const int64_t at = int64_t(rows[lane]) * a.heads + (kv0 + h) * group + member;
+      float* lse = s_lse + (slot * a.kv_cta + h) * kTileQueries + lane;
+      // Past the list's end the sum is infinite: p = 0.
+      if (e * kTileQueries + lane < listed) cp_async<4>(smem_u32(lse), a.lse_in + at, true);
+      else *lse = INFINITY;
+      cp_async<4>(smem_u32(s_delta + (slot * a.kv_cta + h) * kTileQueries + lane), a.delta + at, true);
+    }
   };
   auto sort_pairs = [&](int e) {  // distance buckets of chunk e
     if (bias && e < chunks) {
@@ -169,8 +168,12 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
   if (bias)
     for (int i = tid; i < kvs * group * a.buckets; i += blockDim.x)
       s_bias[(i / a.buckets) * kMaxBuckets + i % a.buckets] = a.table[int64_t(kv0) * group * a.buckets + i] * units.bias;
-  fetch(0);
-  put(0);
+  if (warp < 2 && warp < chunks) {
+    ask_list(warp);
+    ask_rows();
+    put(warp);
+  }
+  if (chunks > 2 && warp == 2 % warps) ask_list(2);
   __syncthreads();
   {
     auto row_of = [&](int r) { return s_krows[r]; };
@@ -179,9 +182,8 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
     keys.copy(base + off.k, kBlockLeaves, row_of);
     values.copy(base + off.v, kBlockLeaves, row_of);
   }
-  copy(0, 0, 0);
-  fetch(1);
-  put(1);
+  if (chunks > 0 && (!whole || warp == 0)) copy(0, 0, 0);
+  cp_commit();
   if (bias) {
     s_table.make(a.edges, a.buckets - 1);
     __syncthreads();
@@ -213,11 +215,13 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
     cp_wait<0>();
     __syncthreads();
     const bool last = member + 1 == group;  // of this entry
-    copy(step + 1, last ? e + 1 : e, last ? 0 : member + 1);
-    if (member == 0) {
-      sort_pairs(e + 1);
-      fetch(e + 2);
-    }
+    if (step + 1 < steps && (!whole || warp == (last ? (e + 1) % warps : e % warps)))
+      copy(step + 1, last ? e + 1 : e, last ? 0 : member + 1);
+    cp_commit();
+    if (member == 0) sort_pairs(e + 1);
+    const bool asked = last && e + 2 < chunks && warp == (e + 2) % warps;
+    if (asked) ask_rows();
+    if (last && e + 3 < chunks && warp == (e + 3) % warps) ask_list(e + 3);
     if (mine) {
       const int slot = int(step & 1);
       const uint32_t q_at = head_at + off.q + slot * stage, d_at = head_at + off.d + slot * stage;
@@ -294,8 +298,8 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
         }
       }
     }
+    if (asked) put(e + 2);  // its slot held chunk e's rows, which nothing copies any more
     if (last) {
-      put(e + 2);  // its slot holds this entry's rows, which the next step's copies were the last to read
       ++e;
       member = 0;
     } else {

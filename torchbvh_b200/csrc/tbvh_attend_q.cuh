@@ -107,8 +107,11 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   float* s_hist = reinterpret_cast<float*>(smem + off.hist);
   const uint32_t kv_rs = row_bytes<T, CP>(a.kv_cta), q_rs = row_bytes<T, CP>(a.heads_cta);
   const uint32_t stage = kStepLeaves * kv_rs;
-  const RowWords words(a.k, a.v, SIZE, CP, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs);
-  const uint32_t row_words = words.pairs_at_once ? a.kv_heads * CP * SIZE / 16 : 1;  // other shapes keep the row number
+  const bool whole = a.width == 16 && a.channels == CP;
+  const int columns = span.kvs * CP * int(SIZE) / 16, row_words = a.kv_heads * CP * int(SIZE) / 16;
+  const char* k_rows = static_cast<const char*>(a.k) + int64_t(span.kv0) * CP * SIZE;
+  const char* v_rows = static_cast<const char*>(a.v) + int64_t(span.kv0) * CP * SIZE;
+  const int warps = int(blockDim.x) / 32;
 
   const int all = a.plan.tile_count[tile];
   const int splits = BACK ? 1 : a.splits;
@@ -121,38 +124,34 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   const Units units(a.scale);
 
   auto first_leaf = [&](uint32_t block, int i) { return int(block) * kBlockLeaves + (i & 1) * kStepLeaves; };
-  // Rows and points of a step's leaves, one leaf a lane of the first warp: asked
-  // for two steps ahead, put down for the others one step ahead.
+  // The warps take turns: one warp asks for the indices (and points) of a step's
+  // leaves, one leaf a lane, two steps ahead, and copies its rows one step ahead.
   uint32_t next_index = 0;
   auto fetch = [&](int i) {
-    if (warp == 0 && i < steps) {
-      const int leaf = min(first_leaf(entries[i >> 1].x, i) + lane, points - 1);
-      next_index = uint32_t(sorted[leaf]);
-      if (bias) {
-        const float* p = leaf_points + int64_t(leaf) * 2 * a.dim;
-        const uint32_t to = base + off.pts + ((i & 1) * 3 * kStepLeaves + lane) * 4;
-        cp_async<4>(to, p, true);
-        cp_async<4>(to + 4 * kStepLeaves, p + 1, true);
-        cp_async<4>(to + 8 * kStepLeaves, p + a.dim - 1, a.dim == 3);
-      }
+    const int leaf = min(first_leaf(entries[i >> 1].x, i) + lane, points - 1);
+    next_index = uint32_t(sorted[leaf]);
+    if (bias) {
+      const float* p = leaf_points + int64_t(leaf) * 2 * a.dim;
+      const uint32_t to = base + off.pts + ((i & 1) * 3 * kStepLeaves + lane) * 4;
+      cp_async<4>(to, p, true);
+      cp_async<4>(to + 4 * kStepLeaves, p + 1, true);
+      cp_async<4>(to + 8 * kStepLeaves, p + a.dim - 1, a.dim == 3);
     }
   };
-  auto put = [&](int i) {
-    if (warp == 0 && i < steps)
-      s_places[(i & 1) * kStepLeaves + lane] = checked_row(a, c, next_index) * row_words;
+  auto copy = [&](int i) {  // by the warp that fetched step i
+    const uint32_t at = base + (i & 1) * stage;
+    copy_words(at + off.k, at + off.v, k_rows, v_rows, checked_row(a, c, next_index) * row_words, columns, kv_rs, lane);
   };
-  auto copy = [&](int i) {
+  // Other shapes: the rows go through shared memory to all threads.
+  auto publish = [&](int i) { s_places[(i & 1) * kStepLeaves + lane] = checked_row(a, c, next_index); };
+  auto copy_all = [&](int i) {
     const uint32_t at = base + (i & 1) * stage;
     const uint32_t* places = s_places + (i & 1) * kStepLeaves;
-    if (words.pairs_at_once) {
-      words.copy(at + off.k, at + off.v, places, kv_rs);
-    } else {
-      auto row_of = [&](int r) { return int(places[r]); };
-      const Rows<T, CP> keys{static_cast<const T*>(a.k), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
-      const Rows<T, CP> values{static_cast<const T*>(a.v), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
-      keys.copy(at + off.k, kStepLeaves, row_of);
-      values.copy(at + off.v, kStepLeaves, row_of);
-    }
+    auto row_of = [&](int r) { return int(places[r]); };
+    const Rows<T, CP> keys{static_cast<const T*>(a.k), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
+    const Rows<T, CP> values{static_cast<const T*>(a.v), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
+    keys.copy(at + off.k, kStepLeaves, row_of);
+    values.copy(at + off.v, kStepLeaves, row_of);
   };
   auto sort_pairs = [&](int i, uint32_t mask) {  // distance buckets of step i, for the queries of `mask`
     const int slot = i & 1;
@@ -168,8 +167,15 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   clear_padding<T, CP>(smem + off.v, kv_rs, 2 * kStepLeaves, a.kv_cta, a.channels);
   clear_padding<T, CP>(smem + off.q, q_rs, kTileQueries, a.heads_cta, a.channels);
   if constexpr (BACK) clear_padding<T, CP>(smem + off.d, q_rs, kTileQueries, a.heads_cta, a.channels);
-  fetch(0);
-  put(0);
+  if (steps > 0 && warp == 0) {
+    fetch(0);
+    if (whole) copy(0);
+    else publish(0);
+  }
+  if (steps > 0 && warp == 1) {
+    fetch(1);
+    if (!whole) publish(1);
+  }
   if (tid < kTileQueries) {
     s_rows[tid] = a.plan.query_row[tile * kTileQueries + tid];
     if (bias) {
@@ -198,10 +204,8 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
       d.copy(base + off.d, kTileQueries, row_of);
     }
   }
-  if (steps > 0) copy(0);
+  if (steps > 0 && !whole) copy_all(0);
   cp_commit();
-  fetch(1);
-  put(1);
   if (bias) reinterpret_cast<BucketTable*>(smem + off.table)->make(a.edges, a.buckets - 1);
   cp_wait<0>();
   __syncthreads();
@@ -245,23 +249,26 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   }
 
   uint2 entry = steps > 0 ? entries[0] : make_uint2(0, 0), next = entry;
+  int copier = 1 % warps, fetcher = 2 % warps;  // of steps i + 1 and i + 2
   for (int i = 0; i < steps; ++i) {
     cp_wait<0>();
     __syncthreads();
     if (i + 1 < steps) {
       if (i & 1) next = entries[(i + 1) >> 1];
-      copy(i + 1);
-      fetch(i + 2);
+      if (!whole) copy_all(i + 1);
+      else if (warp == copier) copy(i + 1);
+      if (warp == fetcher && i + 2 < steps) fetch(i + 2);
+      copier = fetcher;
+      if (++fetcher == warps) fetcher = 0;
       if (bias) sort_pairs(i + 1, next.y);
     }
     cp_commit();
     const unsigned mask = entry.y >> (half * 16);
     const int left = points - first_leaf(entry.x, i);
     entry = next;
-    if (!mine || (mask & 0xffffu) == 0 || left <= 0) {
-      put(i + 2);
-      continue;
-    }
+    const bool fetched = warp == copier && i + 2 < steps;  // (the copier of the next step by now)
+    if (!whole && fetched) publish(i + 2);
+    if (!mine || (mask & 0xffffu) == 0 || left <= 0) continue;
     const int slot = i & 1;
     const uint32_t k_at = k_at0 + slot * stage, v_at = v_at0 + slot * stage;
     const uint32_t on[2] = {mask >> g & 1u, mask >> (g + 8) & 1u};
@@ -393,7 +400,6 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
         for (int r = 0; r < 2; ++r) keep_group(acc, n0, r, both(1.0f), part, on[r], every);
       }
     }
-    put(i + 2);
   }
 
   if (mine) {
