@@ -2,6 +2,7 @@
 // kernels around the two backward passes.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "tbvh_attend_q.cuh"
 #include "tbvh_kernels.h"
@@ -11,25 +12,43 @@ namespace {
 
 // delta[row][head] = <grad_out, out>, and for float16 the largest |grad_out|
 // (float bits order like unsigned numbers; a maximum has no order of its own).
-// One warp a (row, head).
-template <typename T, typename O>
+// `lanes` lanes a (row, head), four channels each at a time where FOUR (rows of
+// whole 16-byte words), else one. Bound by reading both tensors once.
+template <typename T, typename O, bool FOUR>
 __global__ void __launch_bounds__(256) k_delta(const T* grad, const O* out, float* delta, unsigned* most, int64_t rows,
-                                               int channels) {
+                                               int channels, int lanes) {
   __shared__ unsigned s_most[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = int64_t(blockIdx.x) * 8 + warp;
+  const int64_t row = (int64_t(blockIdx.x) * 256 + threadIdx.x) / lanes;
+  const int part = lane & (lanes - 1);
   unsigned big = 0;
+  float sum = 0.0f;
   if (row < rows) {
-    float sum = 0.0f;
-    for (int i = lane; i < channels; i += 32) {
-      const float x = Frag<T>::to_float(grad[row * channels + i]);
-      sum = fmaf(x, Frag<O>::to_float(out[row * channels + i]), sum);
-      big = max(big, __float_as_uint(fabsf(x)));
-    }
+    const T* g = grad + row * channels;
+    const O* o = out + row * channels;
+    constexpr int W = FOUR ? 4 : 1;
+    for (int i = part * W; i < channels; i += lanes * W) {
+      T x[W];
+      O y[W];
+      if constexpr (FOUR) {
+        using WordT = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
+        using WordO = typename std::conditional<sizeof(O) == 2, uint2, uint4>::type;
+        *reinterpret_cast<WordT*>(x) = *reinterpret_cast<const WordT*>(g + i);
+        *reinterpret_cast<WordO*>(y) = *reinterpret_cast<const WordO*>(o + i);
+      } else {
+        x[0] = g[i];
+        y[0] = o[i];
+      }
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFullMask, sum, d);
-    if (lane == 0) delta[row] = sum;
+      for (int w = 0; w < W; ++w) {
+        const float v = Frag<T>::to_float(x[w]);
+        sum = fmaf(v, Frag<O>::to_float(y[w]), sum);
+        big = max(big, __float_as_uint(fabsf(v)));
+      }
+    }
   }
+  for (int d = lanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(kFullMask, sum, d);
+  if (row < rows && part == 0) delta[row] = sum;
   if (most == nullptr) return;
   big = __reduce_max_sync(kFullMask, big);
   if (lane == 0) s_most[warp] = big;
@@ -43,10 +62,21 @@ __global__ void __launch_bounds__(256) k_delta(const T* grad, const O* out, floa
 template <typename T>
 cudaError_t run_delta(const void* grad, const void* out, const float* exact, float* delta, unsigned* most,
                       int64_t pairs, int channels, cudaStream_t stream) {
-  const unsigned grid = unsigned((pairs + 7) / 8);
   const T* g = static_cast<const T*>(grad);
-  if (exact) k_delta<T, float><<<grid, 256, 0, stream>>>(g, exact, delta, most, pairs, channels);
-  else k_delta<T, T><<<grid, 256, 0, stream>>>(g, static_cast<const T*>(out), delta, most, pairs, channels);
+  const void* o = exact ? static_cast<const void*>(exact) : out;
+  const bool four = channels % 4 == 0 && uintptr_t(g) % (4 * sizeof(T)) == 0 &&
+                    uintptr_t(o) % (4 * (exact ? sizeof(float) : sizeof(T))) == 0;
+  int lanes = 1;
+  while (lanes < 32 && lanes * (four ? 4 : 1) < channels) lanes *= 2;
+  const unsigned grid = unsigned((pairs * lanes + 255) / 256);
+  if (exact) {
+    if (four) k_delta<T, float, true><<<grid, 256, 0, stream>>>(g, exact, delta, most, pairs, channels, lanes);
+    else k_delta<T, float, false><<<grid, 256, 0, stream>>>(g, exact, delta, most, pairs, channels, lanes);
+  } else {
+    const T* same = static_cast<const T*>(out);
+    if (four) k_delta<T, T, true><<<grid, 256, 0, stream>>>(g, same, delta, most, pairs, channels, lanes);
+    else k_delta<T, T, false><<<grid, 256, 0, stream>>>(g, same, delta, most, pairs, channels, lanes);
+  }
   count_launches(1);
   return cudaGetLastError();
 }

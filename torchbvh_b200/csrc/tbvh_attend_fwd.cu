@@ -15,31 +15,41 @@ cudaError_t launch_attend_forward(const AttendArgs& a, int dtype, cudaStream_t s
 namespace {
 
 // Joins the splits of one row: with m = max m_s, l = sum l_s 2^(m_s - m) and
-// o = sum o_s 2^(m_s - m) / l. One warp a row.
+// o = sum o_s 2^(m_s - m) / l. One warp a row; a lane has one split's m and l,
+// then every 32nd channel of all splits, four splits in flight.
 template <typename T>
 __global__ void __launch_bounds__(256) k_merge(AttendArgs a, int cp) {
   const int64_t tile = blockIdx.x;
   const int head = blockIdx.y, lane = threadIdx.x & 31;
+  const int64_t stride = a.map.num_tiles * a.heads * kTileQueries * a.part_row;  // floats between splits
   for (int q = threadIdx.x >> 5; q < kTileQueries; q += 8) {
     const int row = a.plan.query_row[tile * kTileQueries + q];
     if (row < 0) continue;
-    const int64_t slot = (tile * a.heads + head) * kTileQueries + q;
-    const int64_t stride = a.map.num_tiles * a.heads * kTileQueries;
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part[(s * stride + slot) * a.part_row]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, o[4] = {}, fine[4] = {};
-    const bool exact = a.out_exact != nullptr;
-    for (int s = 0; s < a.splits; ++s) {
-      const float* p = a.part + (s * stride + slot) * a.part_row;
-      const float w = exp2_fast(p[0] - base);
-      sum = fmaf(p[1], w, sum);
+    const float* part = a.part + ((tile * a.heads + head) * kTileQueries + q) * a.part_row;
+    const bool mine = lane < a.splits;
+    float top = mine ? part[lane * stride] : -INFINITY;
+    float sum = mine ? part[lane * stride + 1] : 0.0f;
+    float most = top;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+    for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(kFullMask, most, d));
+    const float base = most == -INFINITY ? 0.0f : most;
+    const float w = exp2_fast(top - base);
+    sum *= w;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFullMask, sum, d);
+    float o[4] = {}, fine[4] = {};
+    const bool exact = a.out_exact != nullptr;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+      const float ws = __shfl_sync(kFullMask, w, s);
+      const float* p = part + s * stride + 2;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
         if (lane + 32 * i < cp) {
-          o[i] = fmaf(p[2 + lane + 32 * i], w, o[i]);
-          if (exact) fine[i] = fmaf(p[2 + cp + lane + 32 * i], w, fine[i]);
+          o[i] = fmaf(p[lane + 32 * i], ws, o[i]);
+          if (exact) fine[i] = fmaf(p[cp + lane + 32 * i], ws, fine[i]);
         }
+      }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     T* out = static_cast<T*>(a.out) + (int64_t(row) * a.heads + head) * a.channels;
@@ -50,7 +60,8 @@ __global__ void __launch_bounds__(256) k_merge(AttendArgs a, int cp) {
         if (exact) a.out_exact[(int64_t(row) * a.heads + head) * a.channels + lane + 32 * i] = (o[i] + fine[i]) * inv;
       }
     }
-    if (a.lse != nullptr && lane == 0) a.lse[int64_t(row) * a.heads + head] = sum == 0.0f ? INFINITY : top + log2f(sum);
+    if (a.lse != nullptr && lane == 0)
+      a.lse[int64_t(row) * a.heads + head] = sum == 0.0f ? INFINITY : most + log2f(sum);
   }
 }
 

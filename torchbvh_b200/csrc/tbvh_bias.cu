@@ -34,7 +34,8 @@ __global__ void __launch_bounds__(256) k_table_sum(const In* part, Out* out, int
   }
 }
 
-constexpr int kBiasThreads = 256;
+constexpr int kBiasThreads = 256;    // backward
+constexpr int kForwardThreads = 512;
 constexpr int kBiasTable = 8192;  // table values kept in shared memory
 
 struct BiasArgs {
@@ -49,31 +50,37 @@ struct BiasArgs {
 };
 
 // W values of a row at once (W = 4: k a multiple of 4 and 16-byte addresses).
+// Few, large thread blocks: each makes the bucket table once.
 template <int W>
-__global__ void __launch_bounds__(kBiasThreads) k_bias(BiasArgs a, bool table_here) {
+__global__ void __launch_bounds__(kForwardThreads) k_bias(BiasArgs a, bool table_here) {
   __shared__ BucketTable s_buckets;
   extern __shared__ float s_table[];
   const int values = a.heads * a.buckets;
-  s_buckets.make(a.edges, a.buckets - 1);
   if (table_here)
-    for (int i = threadIdx.x; i < values; i += kBiasThreads) s_table[i] = a.table[i];
+    for (int i = threadIdx.x; i < values; i += kForwardThreads) s_table[i] = a.table[i];
+  s_buckets.make(a.edges, a.buckets - 1);
   __syncthreads();
   const float* table = table_here ? s_table : a.table;
   const int64_t per_row = a.k / W;
   const int64_t lists = a.per_head ? a.rows * a.heads : a.rows;
-  const int64_t total = lists * per_row, step = int64_t(gridDim.x) * kBiasThreads;
+  const int64_t total = lists * per_row, step = int64_t(gridDim.x) * kForwardThreads;
   const bool small = total <= UINT_MAX;
-  for (int64_t i = int64_t(blockIdx.x) * kBiasThreads + threadIdx.x; i < total; i += step) {
-    const int64_t list = small ? int64_t(uint32_t(i) / uint32_t(per_row)) : i / per_row;
-    const int64_t at = (i - list * per_row) * W;
-    float d[W];
+  auto read = [&](int64_t i, float (&d)[W]) {
     if constexpr (W == 4) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(a.d2 + list * a.k + at));
+      const float4 v = __ldg(reinterpret_cast<const float4*>(a.d2) + i);
       d[0] = v.x; d[1] = v.y; d[2] = v.z; d[3] = v.w;
     } else {
-      d[0] = __ldg(a.d2 + list * a.k + at);
+      d[0] = __ldg(a.d2 + i);
     }
-    int b[W];
+  };
+  int64_t i = int64_t(blockIdx.x) * kForwardThreads + threadIdx.x;
+  float d[W], next[W];
+  if (i < total) read(i, d);
+  for (; i < total; i += step) {
+    if (i + step < total) read(i + step, next);
+    const int64_t list = small ? int64_t(uint32_t(i) / uint32_t(per_row)) : i / per_row;
+    const int64_t at = (i - list * per_row) * W;
+    uint32_t b[W];
 #pragma unroll
     for (int w = 0; w < W; ++w) b[w] = s_buckets.find_any(d[w]);
     auto store = [&](int64_t row_head, int head) {
@@ -85,27 +92,26 @@ __global__ void __launch_bounds__(kBiasThreads) k_bias(BiasArgs a, bool table_he
     if (a.per_head) store(list, int(small ? uint32_t(list) % uint32_t(a.heads) : list % a.heads));
     else
       for (int h = 0; h < a.heads; ++h) store(list * a.heads + h, h);
+#pragma unroll
+    for (int w = 0; w < W; ++w) d[w] = next[w];
   }
 }
 
-// blockIdx.y: head. Thread blocks of a head stride over its rows.
+// blockIdx.y: head. Thread blocks of a head stride over its rows; the next
+// iteration's values are in flight while this one's are summed.
 template <int W>
 __global__ void __launch_bounds__(kBiasThreads) k_bias_grad(BiasArgs a) {
   __shared__ BucketTable s_buckets;
   extern __shared__ float s_hist[];  // [buckets][threads]
   const int tid = threadIdx.x, lane = tid & 31, head = blockIdx.y;
-  for (int b = 0; b < a.buckets; ++b) s_hist[b * kBiasThreads + tid] = 0.0f;
-  s_buckets.make(a.edges, a.buckets - 1);
-  __syncthreads();
   const int64_t per_row = a.k / W;
   const int64_t total = a.rows * per_row, step = int64_t(gridDim.x) * kBiasThreads;
   const bool small = total <= UINT_MAX;
-  for (int64_t i = int64_t(blockIdx.x) * kBiasThreads + tid; i < total; i += step) {
+  auto read = [&](int64_t i, float (&d)[W], float (&x)[W]) {
     const int64_t row = small ? int64_t(uint32_t(i) / uint32_t(per_row)) : i / per_row;
     const int64_t at = (i - row * per_row) * W;
     const float* p = a.d2 + (a.per_head ? row * a.heads + head : row) * a.k + at;
     const float* q = a.grad + (row * a.heads + head) * a.k + at;
-    float d[W], x[W];
     if constexpr (W == 4) {
       const float4 v = __ldg(reinterpret_cast<const float4*>(p)), u = __ldg(reinterpret_cast<const float4*>(q));
       d[0] = v.x; d[1] = v.y; d[2] = v.z; d[3] = v.w;
@@ -114,8 +120,22 @@ __global__ void __launch_bounds__(kBiasThreads) k_bias_grad(BiasArgs a) {
       d[0] = __ldg(p);
       x[0] = __ldg(q);
     }
+  };
+  int64_t i = int64_t(blockIdx.x) * kBiasThreads + tid;
+  float d[W], x[W], next_d[W], next_x[W];
+  if (i < total) read(i, d, x);
+  for (int b = 0; b < a.buckets; ++b) s_hist[b * kBiasThreads + tid] = 0.0f;
+  s_buckets.make(a.edges, a.buckets - 1);
+  __syncthreads();
+  for (; i < total; i += step) {
+    if (i + step < total) read(i + step, next_d, next_x);
 #pragma unroll
     for (int w = 0; w < W; ++w) s_hist[s_buckets.find_any(d[w]) * kBiasThreads + tid] += x[w];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      d[w] = next_d[w];
+      x[w] = next_x[w];
+    }
   }
   for (int b = 0; b < a.buckets; ++b) {
     float v = s_hist[b * kBiasThreads + tid];
@@ -135,10 +155,10 @@ bool by_four(int64_t k, const void* a, const void* b) {
   return k % 4 == 0 && (uintptr_t(a) | uintptr_t(b)) % 16 == 0;
 }
 
-// Thread blocks of one head of the backward pass: about three an SM in all, at
+// Thread blocks of one head of the backward pass: about four an SM in all, at
 // least eight values a thread.
 int64_t grad_blocks(int64_t rows, int heads, int64_t k) {
-  int64_t want = (3 * 148 + heads - 1) / heads;
+  int64_t want = (4 * 148 + heads - 1) / heads;
   const int64_t most = (rows * k + 8 * kBiasThreads - 1) / (8 * kBiasThreads);
   if (want > most) want = most;
   return want < 1 ? 1 : want;
@@ -167,6 +187,11 @@ int use_device(const char* op, int device) {
 cudaError_t launch_table_sum(const float* part, double* scratch, float* grad_table, int64_t rows, int values,
                              cudaStream_t stream) {
   const unsigned columns = unsigned((values + 31) / 32);
+  if (rows <= 256) {  // 32 rows a warp: one launch is sooner done than two
+    k_table_sum<float, float><<<dim3(columns, 1), 256, 0, stream>>>(part, grad_table, rows, values);
+    count_launches(1);
+    return cudaGetLastError();
+  }
   const int rows_out = rows < 8 * kTableRows ? int((rows + 7) / 8) : kTableRows;
   k_table_sum<float, double><<<dim3(columns, unsigned(rows_out)), 256, 0, stream>>>(part, scratch, rows, values);
   k_table_sum<double, float><<<dim3(columns, 1), 256, 0, stream>>>(scratch, grad_table, rows_out, values);
@@ -192,13 +217,13 @@ int tbvh_distance_bias(int device, const float* squared_distances, int64_t rows,
   BiasArgs a{squared_distances, table, edges, nullptr, out, rows, k, heads, num_buckets, per_head != 0};
   const bool four = by_four(k, squared_distances, out);
   const int64_t items = rows * (per_head ? heads : 1) * (four ? k / 4 : k);
-  int64_t grid = (items + kBiasThreads - 1) / kBiasThreads;
-  if (grid > 8 * 148) grid = 8 * 148;
+  int64_t grid = (items + kForwardThreads - 1) / kForwardThreads;
+  if (grid > 4 * 148) grid = 4 * 148;
   const bool here = heads * num_buckets <= kBiasTable;
   const size_t smem = here ? size_t(heads) * num_buckets * 4 : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (four) k_bias<4><<<unsigned(grid), kBiasThreads, smem, st>>>(a, here);
-  else k_bias<1><<<unsigned(grid), kBiasThreads, smem, st>>>(a, here);
+  if (four) k_bias<4><<<unsigned(grid), kForwardThreads, smem, st>>>(a, here);
+  else k_bias<1><<<unsigned(grid), kForwardThreads, smem, st>>>(a, here);
   count_launches(1);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? TBVH_OK : blocks_cuda_fail(e, op);
