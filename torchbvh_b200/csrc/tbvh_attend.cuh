@@ -360,10 +360,14 @@ inline int copy_width(size_t bytes, const void* a, const void* b, const void* c)
   return 2;
 }
 
+// The threads that share a piece of work, and a thread's number among them.
+struct Crew {
+  int id, count;
+};
+
 // Copies rows of a tensor [row][heads][channels], `here` heads from `first`,
 // `step` apart, into a tile; row_of(r) is the packed row number of tile row r,
-// negative for zeros. All threads take part; asynchronous for widths of 4 bytes
-// and more.
+// negative for zeros. Asynchronous for widths of 4 bytes and more.
 template <typename T, int CP>
 struct Rows {
   const T* src;
@@ -371,10 +375,10 @@ struct Rows {
   uint32_t rs;
 
   template <int BYTES, typename RowOf>
-  __device__ __forceinline__ void part(uint32_t dst, int count, RowOf row_of) const {
+  __device__ __forceinline__ void part(uint32_t dst, int count, RowOf row_of, Crew crew) const {
     constexpr int E = BYTES / int(sizeof(T));
     const int per = channels / E;
-    for (int i = threadIdx.x; i < count * per; i += blockDim.x) {
+    for (int i = crew.id; i < count * per; i += crew.count) {
       const int r = i / per, at = (i - r * per) * E, row = row_of(r);
       const T* p = src + (int64_t(row < 0 ? 0 : row) * heads + first) * channels + at;
       uint32_t d = dst + r * rs + at * uint32_t(sizeof(T));
@@ -389,27 +393,28 @@ struct Rows {
     }
   }
   template <typename RowOf>
-  __device__ __forceinline__ void copy(uint32_t dst, int count, RowOf row_of) const {
-    if (width == 16) part<16>(dst, count, row_of);
-    else if (width == 8) part<8>(dst, count, row_of);
-    else if (width == 4) part<4>(dst, count, row_of);
-    else if constexpr (sizeof(T) == 2) part<2>(dst, count, row_of);
+  __device__ __forceinline__ void copy(uint32_t dst, int count, RowOf row_of, Crew crew) const {
+    if (width == 16) part<16>(dst, count, row_of, crew);
+    else if (width == 8) part<8>(dst, count, row_of, crew);
+    else if (width == 4) part<4>(dst, count, row_of, crew);
+    else if constexpr (sizeof(T) == 2) part<2>(dst, count, row_of, crew);
   }
 };
 
-// 32 rows of two tensors of one shape, copied by ONE warp, where a row's heads
-// are one run of `columns` whole 16-byte words on both sides: lane r holds row
+// ROWS (16 or 32) rows of two tensors of one shape, copied by ONE warp, where a row's heads
+// are one run of `columns` whole 16-byte words on both sides: lane r has row
 // r's place in the tensors, in words, and the lanes share the words of the rows.
 // The warps of a block take turns, a step each: the same copies spread over all
 // warps cost each of them its loop and addresses in every step, three times the
 // instructions. (Bulk copies of a row each, issued by one thread one by one,
 // took 1.7 times as long a step.)
+template <int ROWS>
 __device__ __forceinline__ void copy_words(uint32_t a_tile, uint32_t b_tile, const char* a, const char* b,
                                            uint32_t place, int columns, uint32_t rs, int lane) {
   auto put = [](uint32_t dst, const char* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   };
-  if (columns <= 32 && (columns & (columns - 1)) == 0) {
+  if (columns <= 32 && columns >= 32 / ROWS && (columns & (columns - 1)) == 0) {
     const int rows = 32 / columns, shift = 31 - __clz(columns);  // rows an instruction
     const int column = lane & (columns - 1);
     int r = lane >> shift;
@@ -418,7 +423,7 @@ __device__ __forceinline__ void copy_words(uint32_t a_tile, uint32_t b_tile, con
     a += column * 16;
     b += column * 16;
 #pragma unroll 4
-    for (int i = 0; i < columns; ++i, r += rows, to += step) {
+    for (int i = 0; i < columns; i += 32 / ROWS, r += rows, to += step) {
       const uint64_t at = uint64_t(__shfl_sync(kFullMask, place, r)) * 16;
       put(a_tile + to, a + at);
       put(b_tile + to, b + at);
@@ -426,11 +431,14 @@ __device__ __forceinline__ void copy_words(uint32_t a_tile, uint32_t b_tile, con
   } else {
     int r = lane / columns, column = lane % columns;
     const int dr = 32 / columns, dc = 32 % columns;
-    for (int i = 0; i < columns; ++i) {
+    for (int i = 0; i < ROWS * columns; i += 32) {
+      const bool there = r < ROWS;
       const uint64_t at = (uint64_t(__shfl_sync(kFullMask, place, r)) + column) * 16;
       const uint32_t to = r * rs + column * 16;
-      put(a_tile + to, a + at);
-      put(b_tile + to, b + at);
+      if (there) {
+        put(a_tile + to, a + at);
+        put(b_tile + to, b + at);
+      }
       r += dr;
       column += dc;
       if (column >= columns) {
@@ -443,10 +451,10 @@ __device__ __forceinline__ void copy_words(uint32_t a_tile, uint32_t b_tile, con
 
 // Zeros in the padding channels of tiles, which copies never write.
 template <typename T, int CP>
-__device__ __forceinline__ void clear_padding(char* tile, uint32_t rs, int rows, int heads, int channels) {
+__device__ __forceinline__ void clear_padding(char* tile, uint32_t rs, int rows, int heads, int channels, Crew crew) {
   if (channels == CP) return;
   const int pad = CP - channels;
-  for (int i = threadIdx.x; i < rows * heads * pad; i += blockDim.x) {
+  for (int i = crew.id; i < rows * heads * pad; i += crew.count) {
     const int at = i % pad, h = i / pad % heads, r = i / (pad * heads);
     *reinterpret_cast<T*>(tile + r * rs + (h * CP + channels + at) * int(sizeof(T))) = T(0.0f);
   }
@@ -561,12 +569,13 @@ __device__ __forceinline__ float bias_of(uint32_t row, uint2 b, int n, int j) {
   return lds_f32(__byte_perm(n < 2 ? b.x : b.y, row, 0x7650 + (n & 1) * 2 + j));
 }
 
-// s = logits of 16 rows and 32 columns in units of `unit` (see Units).
-template <typename T, int CP, bool HELD>
+// s = logits of 16 rows and 32 columns in units of `unit` (see Units). PLAIN: the
+// scale is known to be folded.
+template <typename T, int CP, bool HELD, bool BIASED, bool PLAIN>
 __device__ __forceinline__ void logits(float (&s)[4][4], const typename Frag<T>::A* held, uint32_t a, uint32_t a_rs,
-                                       uint32_t b, uint32_t b_rs, bool biased, uint32_t bias, const uint8_t* near,
-                                       int row_step, float scale, bool folded) {
-  if (biased) {
+                                       uint32_t b, uint32_t b_rs, uint32_t bias, const uint8_t* near, int row_step,
+                                       float scale, bool folded) {
+  if constexpr (BIASED) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const uint2 w = *reinterpret_cast<const uint2*>(near + r * row_step);
@@ -575,7 +584,7 @@ __device__ __forceinline__ void logits(float (&s)[4][4], const typename Frag<T>:
 #pragma unroll
         for (int j = 0; j < 2; ++j) s[n][2 * r + j] = bias_of(bias, w, n, j);
     }
-    if (folded) {
+    if (PLAIN || folded) {
       multiply_nk<T, CP, 4, HELD, false>(s, held, a, a_rs, b, b_rs);
     } else {
       float x[4][4];
@@ -587,7 +596,7 @@ __device__ __forceinline__ void logits(float (&s)[4][4], const typename Frag<T>:
     }
   } else {
     multiply_nk<T, CP, 4, HELD, true>(s, held, a, a_rs, b, b_rs);
-    if (!folded) {
+    if (!PLAIN && !folded) {
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
@@ -664,6 +673,12 @@ struct HeadSpan {
     }
   }
 };
+
+// Groups of heads_cta query heads.
+__host__ __device__ inline int head_groups(const AttendArgs& a) {
+  return a.heads_cta >= a.group ? (a.kv_heads + a.kv_cta - 1) / a.kv_cta
+                                : a.kv_heads * ((a.group + a.heads_cta - 1) / a.heads_cta);
+}
 
 // float16: the power of two that brings the largest |grad_out| to [1, 2), so that
 // products of small gradients stay normal numbers; taken out again at the end.

@@ -64,6 +64,7 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
   extern __shared__ __align__(256) char smem[];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Crew crew{tid, int(blockDim.x)};
   const int64_t block = blockIdx.x;
   const int kv0 = blockIdx.y * a.kv_cta;
   const int kvs = min(a.kv_cta, a.kv_heads - kv0);
@@ -132,14 +133,14 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
     const uint32_t to = base + slot * stage;
     if (whole) {
       const int64_t begin = int64_t(first) * CP * SIZE;
-      copy_words(to + off.q, to + off.d, static_cast<const char*>(a.q) + begin,
+      copy_words<32>(to + off.q, to + off.d, static_cast<const char*>(a.q) + begin,
                  static_cast<const char*>(a.grad_out) + begin, uint32_t(rows[lane]) * row_words, columns, rs, lane);
     } else {
       auto row_of = [&](int r) { return rows[r]; };
       const Rows<T, CP> q{static_cast<const T*>(a.q), a.heads, a.channels, first, kvs, group, a.width, rs};
       const Rows<T, CP> d{static_cast<const T*>(a.grad_out), a.heads, a.channels, first, kvs, group, a.width, rs};
-      q.copy(to + off.q, kTileQueries, row_of);
-      d.copy(to + off.d, kTileQueries, row_of);
+      q.copy(to + off.q, kTileQueries, row_of, crew);
+      d.copy(to + off.d, kTileQueries, row_of, crew);
       if (warp != 0) return;
     }
     for (int h = 0; h < kvs; ++h) {
@@ -161,10 +162,10 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
     }
   };
 
-  clear_padding<T, CP>(smem + off.k, rs, kBlockLeaves, a.kv_cta, a.channels);
-  clear_padding<T, CP>(smem + off.v, rs, kBlockLeaves, a.kv_cta, a.channels);
-  clear_padding<T, CP>(smem + off.q, rs, 2 * kTileQueries, a.kv_cta, a.channels);
-  clear_padding<T, CP>(smem + off.d, rs, 2 * kTileQueries, a.kv_cta, a.channels);
+  clear_padding<T, CP>(smem + off.k, rs, kBlockLeaves, a.kv_cta, a.channels, crew);
+  clear_padding<T, CP>(smem + off.v, rs, kBlockLeaves, a.kv_cta, a.channels, crew);
+  clear_padding<T, CP>(smem + off.q, rs, 2 * kTileQueries, a.kv_cta, a.channels, crew);
+  clear_padding<T, CP>(smem + off.d, rs, 2 * kTileQueries, a.kv_cta, a.channels, crew);
   if (bias)
     for (int i = tid; i < kvs * group * a.buckets; i += blockDim.x)
       s_bias[(i / a.buckets) * kMaxBuckets + i % a.buckets] = a.table[int64_t(kv0) * group * a.buckets + i] * units.bias;
@@ -179,8 +180,8 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
     auto row_of = [&](int r) { return s_krows[r]; };
     const Rows<T, CP> keys{static_cast<const T*>(a.k), a.kv_heads, a.channels, kv0, kvs, 1, a.width, rs};
     const Rows<T, CP> values{static_cast<const T*>(a.v), a.kv_heads, a.channels, kv0, kvs, 1, a.width, rs};
-    keys.copy(base + off.k, kBlockLeaves, row_of);
-    values.copy(base + off.v, kBlockLeaves, row_of);
+    keys.copy(base + off.k, kBlockLeaves, row_of, crew);
+    values.copy(base + off.v, kBlockLeaves, row_of, crew);
   }
   if (chunks > 0 && (!whole || warp == 0)) copy(0, 0, 0);
   cp_commit();
@@ -229,9 +230,13 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
       const float* delta = s_delta + (slot * a.kv_cta + kv) * kTileQueries + 2 * t;
       const uint32_t head_bias = base + off.bias + (kv * group + member) * kMaxBuckets * 4;
       float s[NT][4], ds[NT][4];
-      logits<T, CP, HELD>(s, held_k, k_at, rs, q_at + nk, rs, bias, head_bias,
-                          near0 + (e & 1) * kBlockLeaves * kKeyBucketRow, 8 * kKeyBucketRow, a.scale * kLog2e,
-                          units.folded);
+      const uint8_t* near = near0 + (e & 1) * kBlockLeaves * kKeyBucketRow;
+      if (bias)
+        logits<T, CP, HELD, true, false>(s, held_k, k_at, rs, q_at + nk, rs, head_bias, near, 8 * kKeyBucketRow,
+                                         a.scale * kLog2e, units.folded);
+      else
+        logits<T, CP, HELD, false, false>(s, held_k, k_at, rs, q_at + nk, rs, head_bias, near, 8 * kKeyBucketRow,
+                                          a.scale * kLog2e, units.folded);
       multiply_nk<T, CP, NT, HELD, true>(ds, held_v, v_at, rs, d_at + nk, rs);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {

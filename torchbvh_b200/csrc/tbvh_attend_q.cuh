@@ -26,6 +26,8 @@
 // values reach only the rows that attend to them.
 #pragma once
 
+#include <type_traits>
+
 #include "tbvh_attend.cuh"
 
 namespace tbvh {
@@ -66,20 +68,14 @@ __host__ __device__ inline QueryTileSmem query_tile_smem(int size, int cp, int k
   return s;
 }
 
-// Row r of a group of accumulator tiles from n0: old * factor + part where `on`
-// (`every`: known to be on in the whole warp).
+// Row r of a group of accumulator tiles from n0: old * factor + part where `on`.
 template <int N>
 __device__ __forceinline__ void keep_group(Pair (&acc)[N][2], int n0, int r, Pair factor,
-                                           const float (&part)[kChannelGroup][4], uint32_t on, bool every) {
+                                           const float (&part)[kChannelGroup][4], uint32_t on) {
   static_assert(kChannelGroup == 4, "one group is four tiles");
-  const Pair p[4] = {pair(part[0][2 * r], part[0][2 * r + 1]), pair(part[1][2 * r], part[1][2 * r + 1]),
-                     pair(part[2][2 * r], part[2][2 * r + 1]), pair(part[3][2 * r], part[3][2 * r + 1])};
-  if (every) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[n0 + j][r] = fma2(acc[n0 + j][r], factor, p[j]);
-  } else {
-    keep_where(acc[n0][r], acc[n0 + 1][r], acc[n0 + 2][r], acc[n0 + 3][r], factor, p[0], p[1], p[2], p[3], on);
-  }
+  keep_where(acc[n0][r], acc[n0 + 1][r], acc[n0 + 2][r], acc[n0 + 3][r], factor, pair(part[0][2 * r], part[0][2 * r + 1]),
+             pair(part[1][2 * r], part[1][2 * r + 1]), pair(part[2][2 * r], part[2][2 * r + 1]),
+             pair(part[3][2 * r], part[3][2 * r + 1]), on);
 }
 
 // Registers: with 32 padded channels three blocks of eight warps share an SM.
@@ -95,6 +91,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   extern __shared__ __align__(256) char smem[];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Crew crew{tid, int(blockDim.x)};
   const int64_t tile = blockIdx.x;
   const HeadSpan span(a, blockIdx.y);
   const BlockCloud c = a.map.of_tile(tile);
@@ -140,7 +137,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   };
   auto copy = [&](int i) {  // by the warp that fetched step i
     const uint32_t at = base + (i & 1) * stage;
-    copy_words(at + off.k, at + off.v, k_rows, v_rows, checked_row(a, c, next_index) * row_words, columns, kv_rs, lane);
+    copy_words<32>(at + off.k, at + off.v, k_rows, v_rows, checked_row(a, c, next_index) * row_words, columns, kv_rs, lane);
   };
   // Other shapes: the rows go through shared memory to all threads.
   auto publish = [&](int i) { s_places[(i & 1) * kStepLeaves + lane] = checked_row(a, c, next_index); };
@@ -150,8 +147,8 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
     auto row_of = [&](int r) { return int(places[r]); };
     const Rows<T, CP> keys{static_cast<const T*>(a.k), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
     const Rows<T, CP> values{static_cast<const T*>(a.v), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
-    keys.copy(at + off.k, kStepLeaves, row_of);
-    values.copy(at + off.v, kStepLeaves, row_of);
+    keys.copy(at + off.k, kStepLeaves, row_of, crew);
+    values.copy(at + off.v, kStepLeaves, row_of, crew);
   };
   auto sort_pairs = [&](int i, uint32_t mask) {  // distance buckets of step i, for the queries of `mask`
     const int slot = i & 1;
@@ -163,10 +160,10 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
     else sort_step<false>(to, kBucketRow, table, q, kTileQueries, p, mask);
   };
 
-  clear_padding<T, CP>(smem + off.k, kv_rs, 2 * kStepLeaves, a.kv_cta, a.channels);
-  clear_padding<T, CP>(smem + off.v, kv_rs, 2 * kStepLeaves, a.kv_cta, a.channels);
-  clear_padding<T, CP>(smem + off.q, q_rs, kTileQueries, a.heads_cta, a.channels);
-  if constexpr (BACK) clear_padding<T, CP>(smem + off.d, q_rs, kTileQueries, a.heads_cta, a.channels);
+  clear_padding<T, CP>(smem + off.k, kv_rs, 2 * kStepLeaves, a.kv_cta, a.channels, crew);
+  clear_padding<T, CP>(smem + off.v, kv_rs, 2 * kStepLeaves, a.kv_cta, a.channels, crew);
+  clear_padding<T, CP>(smem + off.q, q_rs, kTileQueries, a.heads_cta, a.channels, crew);
+  if constexpr (BACK) clear_padding<T, CP>(smem + off.d, q_rs, kTileQueries, a.heads_cta, a.channels, crew);
   if (steps > 0 && warp == 0) {
     fetch(0);
     if (whole) copy(0);
@@ -198,10 +195,10 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   {
     auto row_of = [&](int r) { return s_rows[r]; };
     const Rows<T, CP> q{static_cast<const T*>(a.q), a.heads, a.channels, span.h0, span.heads, 1, a.width, q_rs};
-    q.copy(base + off.q, kTileQueries, row_of);
+    q.copy(base + off.q, kTileQueries, row_of, crew);
     if constexpr (BACK) {
       const Rows<T, CP> d{static_cast<const T*>(a.grad_out), a.heads, a.channels, span.h0, span.heads, 1, a.width, q_rs};
-      d.copy(base + off.d, kTileQueries, row_of);
+      d.copy(base + off.d, kTileQueries, row_of, crew);
     }
   }
   if (steps > 0 && !whole) copy_all(0);
@@ -272,13 +269,16 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
     const int slot = i & 1;
     const uint32_t k_at = k_at0 + slot * stage, v_at = v_at0 + slot * stage;
     const uint32_t on[2] = {mask >> g & 1u, mask >> (g + 8) & 1u};
-    const bool every = (mask & 0xffffu) == 0xffffu;  // all 16 rows, the same for the warp
     const uint8_t* near = near0 + slot * kTileQueries * kBucketRow;
+    // The step's work: written without branches, so that its chains of dependent
+    // instructions overlap; the rare forms (the cloud's last leaves, scales that are
+    // not folded) have their own copy.
+    auto work = [&](auto biased, auto plain) {
+    constexpr bool BIASED = decltype(biased)::value, PLAIN = decltype(plain)::value;
     float s[NT][4];
-    logits<T, CP, HELD>(s, held_q, q_at, q_rs, k_at + nk, kv_rs, bias, head_bias, near, 8 * kBucketRow,
-                        a.scale * kLog2e, units.folded);
-    if (left < kStepLeaves) {  // the cloud's last leaves
-      asm volatile("" ::: "memory");  // a branch, not 32 selections in every step
+    logits<T, CP, HELD, BIASED, PLAIN>(s, held_q, q_at, q_rs, k_at + nk, kv_rs, head_bias, near, 8 * kBucketRow,
+                                       a.scale * kLog2e, units.folded);
+    if constexpr (!PLAIN) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -296,18 +296,18 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
         most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
         const float from_top = most == -INFINITY ? 0.0f : -most * unit;  // nothing yet: all p are 0
         const float fade = exp2_fast(fmaf(top[r], unit, from_top));
-        Pair add = both(0.0f);
+        Pair add;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const float2 x = unpair(fma2(pair(s[n][2 * r], s[n][2 * r + 1]), both(unit), both(from_top)));
           s[n][2 * r] = exp2_fast(x.x);
           s[n][2 * r + 1] = exp2_fast(x.y);
-          add = add2(add, pair(s[n][2 * r], s[n][2 * r + 1]));
+          const Pair p = pair(s[n][2 * r], s[n][2 * r + 1]);
+          add = n == 0 ? p : add2(add, p);
         }
-        if (on[r]) {
-          top[r] = most;
-          sum[r] = fmaf(sum[r], fade, unpair(add).x + unpair(add).y);
-        }
+        const float grown = fmaf(sum[r], fade, unpair(add).x + unpair(add).y);
+        top[r] = on[r] ? most : top[r];
+        sum[r] = on[r] ? grown : sum[r];
         shrink[r] = both(fade);
       }
 #pragma unroll
@@ -341,8 +341,8 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          keep_group(acc, n0, r, shrink[r], part, on[r], every);
-          if constexpr (EXACT) keep_group(fine, n0, r, shrink[r], low, on[r], every);
+          keep_group(acc, n0, r, shrink[r], part, on[r]);
+          if constexpr (EXACT) keep_group(fine, n0, r, shrink[r], low, on[r]);
         }
       }
     } else {
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
           ds[n][2 * r] = unpair(p).x;
           ds[n][2 * r + 1] = unpair(p).y;
         }
-      if (bias) {
+      if constexpr (BIASED) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           if (on[r]) {
@@ -397,8 +397,16 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
           }
         }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) keep_group(acc, n0, r, both(1.0f), part, on[r], every);
+        for (int r = 0; r < 2; ++r) keep_group(acc, n0, r, both(1.0f), part, on[r]);
       }
+    }
+    };
+    if (left >= kStepLeaves && units.folded) {
+      if (bias) work(std::true_type{}, std::true_type{});
+      else work(std::false_type{}, std::true_type{});
+    } else {
+      if (bias) work(std::true_type{}, std::false_type{});
+      else work(std::false_type{}, std::false_type{});
     }
   }
 
