@@ -106,8 +106,10 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
   // The warps take turns, a chunk each: a chunk's warp asks for its list elements
   // three chunks ahead, for their rows and points two chunks ahead (one query a
   // lane), and copies the rows one step ahead.
-  const bool whole = a.width == 16 && a.channels == CP && (group == 1 || kvs == 1);
-  const int columns = kvs * CP * int(SIZE) / 16, row_words = a.heads * CP * int(SIZE) / 16;
+  const bool whole = a.width == 16 && a.channels == CP;
+  // Heads that lie side by side are copied as one; those of shared keys lie `group` apart.
+  const int runs = group == 1 ? 1 : kvs, columns = kvs / runs * CP * int(SIZE) / 16;
+  const int row_words = a.heads * CP * int(SIZE) / 16;
   const int warps = int(blockDim.x) / 32;
   uint32_t next_slot = 0;
   int next_row = 0;
@@ -132,9 +134,11 @@ __global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
     const int first = kv0 * group + member;  // query heads kv * group + member, one a key/value head
     const uint32_t to = base + slot * stage;
     if (whole) {
-      const int64_t begin = int64_t(first) * CP * SIZE;
-      copy_words<32>(to + off.q, to + off.d, static_cast<const char*>(a.q) + begin,
-                 static_cast<const char*>(a.grad_out) + begin, uint32_t(rows[lane]) * row_words, columns, rs, lane);
+      for (int h = 0; h < runs; ++h) {
+        const int64_t begin = int64_t(first + h * group) * CP * SIZE;
+        copy_words<32>(to + off.q + h * CP * SIZE, to + off.d + h * CP * SIZE, static_cast<const char*>(a.q) + begin,
+                       static_cast<const char*>(a.grad_out) + begin, uint32_t(rows[lane]) * row_words, columns, rs, lane);
+      }
     } else {
       auto row_of = [&](int r) { return rows[r]; };
       const Rows<T, CP> q{static_cast<const T*>(a.q), a.heads, a.channels, first, kvs, group, a.width, rs};

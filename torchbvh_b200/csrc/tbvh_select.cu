@@ -182,6 +182,10 @@ struct SelectArgs {
 };
 
 constexpr int kSelectStack = 44;  // <= 3 more nodes per two levels, 25 levels at most
+// The tree is cut this many levels above the blocks: the up to 16 blocks below a
+// node there are a bunch, scored together.
+constexpr int kBunchLevels = 4;
+constexpr int kBunch = 1 << kBunchLevels;
 
 template <int D>
 struct Box {
@@ -221,15 +225,21 @@ __device__ __forceinline__ uint64_t score_key(float s, uint32_t block) {
 }
 
 // One warp a tile. The warp walks the tree as a packet, two levels a step: the
-// (up to four) grandchildren of a node are scored by every lane, those that
-// some lane admits are pushed, the one nearest to most lanes last. A popped
-// node is scored again against the meanwhile lower k-th keys.
+// (up to four) grandchildren of a node are scored by every lane, those that some
+// lane admits are pushed, the one nearest to most lanes last. A popped node is
+// scored again against the meanwhile lower k-th keys. At a bunch each of 16
+// lanes loads one block's box and scores it against the box of the tile's
+// queries, a lower bound for all of them; the boxes go to shared memory in
+// ascending order of that bound, so that near blocks enter the lists first, few
+// are displaced again, and the scan ends at the first block no query can want.
+// Bound by issue: an insertion shifts a list of 64-bit keys in registers.
 template <int D, int CAP>
 __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
   __shared__ uint32_t s_stack[kSelectStack];
   __shared__ int64_t s_row[32];
   __shared__ uint64_t s_keys[32 * CAP];
   __shared__ int64_t s_query[32];
+  __shared__ float4 s_lo[kBunch], s_hi[kBunch];  // w: lower bound, block
   const int lane = threadIdx.x;
   const int64_t tile = blockIdx.x;
   const BlockCloud c = a.map.of_tile(tile);
@@ -295,9 +305,71 @@ __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
     }
   };
 
+  // The box of the tile's queries.
+  float q_lo[D], q_hi[D];
+#pragma unroll
+  for (int x = 0; x < D; ++x) {
+    q_lo[x] = searching ? q[x] : INFINITY;
+    q_hi[x] = searching ? q[x] : -INFINITY;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      q_lo[x] = fminf(q_lo[x], __shfl_xor_sync(kFullMask, q_lo[x], d));
+      q_hi[x] = fmaxf(q_hi[x], __shfl_xor_sync(kFullMask, q_hi[x], d));
+    }
+  }
+  // The largest k-th score of any lane.
+  auto worst = [&]() { return __uint_as_float(__reduce_max_sync(kFullMask, uint32_t(bound >> 32))); };
+
+  const int bunch_level = last > kBunchLevels ? last - kBunchLevels : 0;
+  const int below = last - bunch_level;  // levels from a bunch's node to its blocks
+  auto scan_bunch = [&](uint32_t node) {
+    const uint32_t base = node << below;
+    const int64_t there = level_count(c.n, leaf_level, last) - base;
+    const int blocks = there < (1 << below) ? int(there) : 1 << below;
+    float least = INFINITY;
+    Box<D> box{};
+    if (lane < blocks) {
+      box = load_box<D>(a.aabbs, s_row[last] + base + lane);
+      float sum = 0.0f;
+#pragma unroll
+      for (int x = 0; x < D; ++x) {
+        const float gap = fmaxf(__fsub_rn(box.lo[x], q_hi[x]), fmaxf(__fsub_rn(q_lo[x], box.hi[x]), 0.0f));
+        const float sq = __fmul_rn(gap, gap);
+        sum = x == 0 ? sq : __fadd_rn(sum, sq);
+      }
+      least = sum == sum ? sum : 0.0f;
+    }
+    // Place in ascending order of the bound (the lower block first among equals).
+    int place = 0;
+#pragma unroll
+    for (int k = 0; k < kBunch; ++k) {
+      const float other = __shfl_sync(kFullMask, least, k);
+      place += other < least || (other == least && k < lane);
+    }
+    __syncwarp();
+    if (lane < blocks) {
+      s_lo[place] = make_float4(box.lo[0], box.lo[1], D == 3 ? box.lo[D - 1] : 0.0f, least);
+      s_hi[place] = make_float4(box.hi[0], box.hi[1], D == 3 ? box.hi[D - 1] : 0.0f, __uint_as_float(base + lane));
+    }
+    __syncwarp();
+    float reach = worst();
+    for (int k = 0; k < blocks; ++k) {
+      const float4 lo = s_lo[k], hi = s_hi[k];
+      if (lo.w > reach) break;
+      Box<D> b;
+      b.lo[0] = lo.x, b.lo[1] = lo.y, b.hi[0] = hi.x, b.hi[1] = hi.y;
+      if constexpr (D == 3) b.lo[2] = lo.z, b.hi[2] = hi.z;
+      const uint64_t x = score_key(box_score<D>(q, b), __float_as_uint(hi.w));
+      if (__any_sync(kFullMask, x < bound)) {
+        insert(x);
+        reach = worst();
+      }
+    }
+  };
+
   int depth = 0;
-  if (last == 0) {
-    insert(score_key(box_score<D>(q, load_box<D>(a.aabbs, s_row[0])), 0));
+  if (bunch_level == 0) {
+    scan_bunch(0);
   } else {
     if (lane == 0) s_stack[0] = 0;
     depth = 1;
@@ -315,7 +387,11 @@ __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
       if (!__any_sync(kFullMask, score_key(s, j << (last - level)) < bound)) continue;
     }
     fresh = false;
-    const int step = last - level >= 2 ? 2 : 1;
+    if (level == bunch_level) {
+      scan_bunch(j);
+      continue;
+    }
+    const int step = bunch_level - level >= 2 ? 2 : 1;
     const int child_level = level + step;
     const uint32_t base = j << step;
     const int64_t there = level_count(c.n, leaf_level, child_level) - base;
@@ -324,12 +400,6 @@ __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       score[k] = k < children ? box_score<D>(q, load_box<D>(a.aabbs, s_row[child_level] + base + k)) : kFar;
-    if (child_level == last) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (k < children) insert(score_key(score[k], base + k));
-      continue;
-    }
     // Every lane votes for its nearest child that it admits.
     int nearest = -1;
     float least = kFar;
