@@ -25,7 +25,14 @@ import math
 import torch
 
 from . import _native
-from ._constants import BLOCK_SIZE, MAX_BIAS_BUCKETS, MAX_BLOCK_CHANNELS, MAX_SELECTED_BLOCKS
+from ._constants import (
+    BLOCK_SIZE,
+    MAX_BIAS_BUCKETS,
+    MAX_BLOCK_CHANNELS,
+    MAX_BLOCK_HEADS,
+    MAX_SELECTED_BLOCKS,
+    MAX_SHARED_HEADS,
+)
 from ._handles import (
     BVHHandle,
     BatchedBVHHandle,
@@ -65,11 +72,13 @@ class BlockSelection(_Handle):
         self._keep = keep  # tensors and host tables behind the geometry's pointers
         self._key_shape = key_shape      # leading shape of keys and values
         self._query_shape = query_shape  # leading shape of queries
-        self._stream = torch.cuda.current_stream(self.device) if self.device.type == "cuda" else None
+        self._device = fields["block_indices"].device
+        self._stream = _native.raw_stream(self._device) if self._device.type == "cuda" else None
 
     @property
     def device(self) -> torch.device:
-        return self._live_fields()["block_indices"].device
+        self._live_fields()
+        return self._device
 
     def destroy(self) -> None:
         self._geometry = None
@@ -78,22 +87,26 @@ class BlockSelection(_Handle):
 
     def _used_here(self) -> None:
         """Tells the allocator that the current stream reads the selection's memory."""
-        stream = torch.cuda.current_stream(self.device)
-        if stream != self._stream and not torch.cuda.is_current_stream_capturing():
+        if _native.raw_stream(self._device) != self._stream and not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream(self._device)
             for item in self._keep:
                 if isinstance(item, torch.Tensor) and item.is_cuda:
                     item.record_stream(stream)
 
 
+# The messages are put together only for a call that is refused.
+
 def _check_query_points(query_points: torch.Tensor, rank: int, dim: int, device: torch.device) -> torch.Tensor:
     prefix = "select_blocks"
-    shape = {2: "(M, D)", 3: "(B, M, D)"}[rank]
-    _reject_unless(query_points.dim() == rank, f"{prefix}: query_points must have shape {shape}")
-    _reject_unless(query_points.size(-1) == dim, f"{prefix}: query_points last dimension must match BVH dim")
+    if query_points.dim() != rank:
+        raise ValueError(f"{prefix}: query_points must have shape {'(M, D)' if rank == 2 else '(B, M, D)'}")
+    if query_points.size(-1) != dim:
+        raise ValueError(f"{prefix}: query_points last dimension must match BVH dim")
     _validate_cuda_float32(prefix, query_points, "query_points")
-    _reject_unless(query_points.device == device, f"{prefix}: query_points must be on the same device as the BVH")
-    _reject_unless(query_points.numel() // dim <= 2**31 - 1,
-                   f"{prefix}: total query count must fit in signed int32")
+    if query_points.device != device:
+        raise ValueError(f"{prefix}: query_points must be on the same device as the BVH")
+    if query_points.numel() // dim > 2**31 - 1:
+        raise ValueError(f"{prefix}: total query count must fit in signed int32")
     return _as_contiguous(query_points.detach())
 
 
@@ -114,8 +127,8 @@ def select_blocks(bvh: BVHHandle | BatchedBVHHandle | RaggedBVHHandle, query_poi
     ``attend_blocks`` needs, for inference. Carries no gradient.
     """
     prefix = "select_blocks"
-    _reject_unless(isinstance(num_blocks, int) and 1 <= num_blocks <= MAX_SELECTED_BLOCKS,
-                   f"{prefix}: num_blocks must be 1 to {MAX_SELECTED_BLOCKS}")
+    if not (isinstance(num_blocks, int) and 1 <= num_blocks <= MAX_SELECTED_BLOCKS):
+        raise ValueError(f"{prefix}: num_blocks must be 1 to {MAX_SELECTED_BLOCKS}")
     geometry = _native.BlockGeometry(num_blocks=num_blocks, backward=1 if backward else 0)
     if isinstance(bvh, RaggedBVHHandle):
         _reject_unless(query_offsets is not None, f"{prefix}: query_offsets is required for a ragged BVH")
@@ -165,16 +178,17 @@ def select_blocks(bvh: BVHHandle | BatchedBVHHandle | RaggedBVHHandle, query_poi
 
 def _check_bias(prefix: str, table: torch.Tensor, edges: torch.Tensor, heads: int | None, device: torch.device,
                 table_name: str, edges_name: str) -> None:
-    _reject_unless(table.dim() == 2 and (heads is None or table.size(0) == heads),
-                   f"{prefix}: {table_name} must have shape (H, num_buckets)")
-    _reject_unless(1 <= table.size(1) <= MAX_BIAS_BUCKETS,
-                   f"{prefix}: {table_name} must have 1 to {MAX_BIAS_BUCKETS} buckets")
-    _reject_unless(edges.dim() == 1 and edges.size(0) == table.size(1) - 1,
-                   f"{prefix}: {edges_name} must have shape (num_buckets - 1,)")
+    if table.dim() != 2 or (heads is not None and table.size(0) != heads):
+        raise ValueError(f"{prefix}: {table_name} must have shape (H, num_buckets)")
+    buckets = table.size(1)
+    if not 1 <= buckets <= MAX_BIAS_BUCKETS:
+        raise ValueError(f"{prefix}: {table_name} must have 1 to {MAX_BIAS_BUCKETS} buckets")
+    if edges.dim() != 1 or edges.size(0) != buckets - 1:
+        raise ValueError(f"{prefix}: {edges_name} must have shape (num_buckets - 1,)")
     _validate_cuda_float32(prefix, table, table_name)
     _validate_cuda_float32(prefix, edges, edges_name)
-    _reject_unless(table.device == device and edges.device == device,
-                   f"{prefix}: {table_name} and {edges_name} must be on the same device as the other inputs")
+    if table.device != device or edges.device != device:
+        raise ValueError(f"{prefix}: {table_name} and {edges_name} must be on the same device as the other inputs")
 
 
 class _AttendBlocks(torch.autograd.Function):
@@ -235,35 +249,43 @@ def attend_blocks(selection: BlockSelection, queries: torch.Tensor, keys: torch.
     if not isinstance(selection, BlockSelection):
         raise TypeError(f"{prefix}: selection must be a BlockSelection returned by select_blocks")
     device = selection.device
-    _reject_unless(queries.dim() == len(selection._query_shape) + 2
-                   and tuple(queries.shape[:-2]) == selection._query_shape,
-                   f"{prefix}: queries must have shape {(*selection._query_shape, 'H', 'C')}".replace("'", ""))
-    heads, channels = int(queries.size(-2)), int(queries.size(-1))
+    query_shape, key_shape = selection._query_shape, selection._key_shape
+    if queries.dim() != len(query_shape) + 2 or tuple(queries.shape[:-2]) != query_shape:
+        raise ValueError(f"{prefix}: queries must have shape {(*query_shape, 'H', 'C')}".replace("'", ""))
+    heads, channels = queries.shape[-2:]
     for name, t in (("keys", keys), ("values", values)):
-        _reject_unless(t.dim() == len(selection._key_shape) + 2 and tuple(t.shape[:-2]) == selection._key_shape
-                       and t.size(-1) == channels,
-                       f"{prefix}: {name} must have shape {(*selection._key_shape, 'Hkv', 'C')}".replace("'", ""))
-    _reject_unless(keys.size(-2) == values.size(-2), f"{prefix}: keys and values must have the same heads")
-    _reject_unless(heads >= 1 and keys.size(-2) >= 1 and heads % keys.size(-2) == 0,
-                   f"{prefix}: query heads must be a multiple of key heads")
-    _reject_unless(1 <= channels <= MAX_BLOCK_CHANNELS, f"{prefix}: channels must be 1 to {MAX_BLOCK_CHANNELS}")
+        if t.dim() != len(key_shape) + 2 or tuple(t.shape[:-2]) != key_shape or t.size(-1) != channels:
+            raise ValueError(f"{prefix}: {name} must have shape {(*key_shape, 'Hkv', 'C')}".replace("'", ""))
+    key_heads = keys.size(-2)
+    if key_heads != values.size(-2):
+        raise ValueError(f"{prefix}: keys and values must have the same heads")
+    if heads < 1 or key_heads < 1 or heads % key_heads != 0:
+        raise ValueError(f"{prefix}: query heads must be a multiple of key heads")
+    if heads // key_heads > MAX_SHARED_HEADS or heads > MAX_BLOCK_HEADS:
+        raise ValueError(f"{prefix}: at most {MAX_BLOCK_HEADS} query heads, and {MAX_SHARED_HEADS} to a key head")
+    if not 1 <= channels <= MAX_BLOCK_CHANNELS:
+        raise ValueError(f"{prefix}: channels must be 1 to {MAX_BLOCK_CHANNELS}")
+    dtype = queries.dtype
     for name, t in (("queries", queries), ("keys", keys), ("values", values)):
-        _reject_unless(t.is_cuda, f"{prefix}: {name} must be a CUDA tensor")
-        _reject_unless(t.device == device, f"{prefix}: {name} must be on the same device as the selection")
-        _reject_unless(t.dtype in _native._FEATURE_TYPES and t.dtype == queries.dtype,
-                       f"{prefix}: queries, keys and values must share one type: float32, float16 or bfloat16")
-    _reject_unless((bias_table is None) == (bias_edges is None),
-                   f"{prefix}: bias_table and bias_edges must be given together")
+        if not t.is_cuda:
+            raise ValueError(f"{prefix}: {name} must be a CUDA tensor")
+        if t.device != device:
+            raise ValueError(f"{prefix}: {name} must be on the same device as the selection")
+        if t.dtype != dtype or dtype not in _native._FEATURE_TYPES:
+            raise ValueError(f"{prefix}: queries, keys and values must share one type: float32, float16 or bfloat16")
+    if (bias_table is None) != (bias_edges is None):
+        raise ValueError(f"{prefix}: bias_table and bias_edges must be given together")
     if bias_table is not None:
         _check_bias(prefix, bias_table, bias_edges, heads, device, "bias_table", "bias_edges")
         bias_table, bias_edges = _as_contiguous(bias_table), _as_contiguous(bias_edges.detach())
     scale = channels**-0.5 if scale is None else float(scale)
-    _reject_unless(math.isfinite(scale), f"{prefix}: scale must be finite")
+    if not math.isfinite(scale):
+        raise ValueError(f"{prefix}: scale must be finite")
     queries, keys, values = _as_contiguous(queries), _as_contiguous(keys), _as_contiguous(values)
     selection._used_here()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (queries, keys, values, bias_table)):
-        _reject_unless(bool(selection._geometry.backward),
-                       f"{prefix}: gradients need a selection made with backward=True")
+        if not selection._geometry.backward:
+            raise ValueError(f"{prefix}: gradients need a selection made with backward=True")
         return _AttendBlocks.apply(queries, keys, values, bias_table, bias_edges, selection, scale)
     return _native.attend_blocks(selection._geometry, queries, keys, values, bias_table, bias_edges, scale, False,
                                  False)[0]
@@ -297,16 +319,18 @@ def distance_bias(squared_distances: torch.Tensor, table: torch.Tensor, edges: t
     in a fixed order.
     """
     prefix = "distance_bias"
-    _reject_unless(squared_distances.dim() in (3, 4),
-                   f"{prefix}: squared_distances must have shape (B, N, H, k) or (B, N, k)")
+    rank = squared_distances.dim()
+    if rank not in (3, 4):
+        raise ValueError(f"{prefix}: squared_distances must have shape (B, N, H, k) or (B, N, k)")
     _validate_cuda_float32(prefix, squared_distances, "squared_distances")
     _check_bias(prefix, table, edges, None, squared_distances.device, "table", "edges")
-    per_head = squared_distances.dim() == 4
-    _reject_unless(not per_head or squared_distances.size(2) == table.size(0),
-                   f"{prefix}: squared_distances head dimension must match table")
-    _reject_unless(table.size(0) >= 1, f"{prefix}: table must have at least one head")
+    heads = table.size(0)
+    if rank == 4 and squared_distances.size(2) != heads:
+        raise ValueError(f"{prefix}: squared_distances head dimension must match table")
+    if not 1 <= heads <= MAX_BLOCK_HEADS:
+        raise ValueError(f"{prefix}: table must have at least one head, and at most {MAX_BLOCK_HEADS}")
     squared_distances = _as_contiguous(squared_distances.detach())
     table, edges = _as_contiguous(table), _as_contiguous(edges.detach())
     if torch.is_grad_enabled() and table.requires_grad:
-        return _DistanceBias.apply(squared_distances, table, edges, per_head)
-    return _native.distance_bias(squared_distances, int(table.size(0)), per_head, table, edges)
+        return _DistanceBias.apply(squared_distances, table, edges, rank == 4)
+    return _native.distance_bias(squared_distances, heads, rank == 4, table, edges)

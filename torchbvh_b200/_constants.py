@@ -8,6 +8,8 @@ SUPPORTED_DIMS = (2, 3)
 BLOCK_SIZE = 64
 MAX_SELECTED_BLOCKS = 32
 MAX_BLOCK_CHANNELS = 128
+MAX_BLOCK_HEADS = 4096
+MAX_SHARED_HEADS = 64  # query heads of one key/value head
 MAX_BIAS_BUCKETS = 64
 
 # Squared distance at or below which a neighbour counts as an exact hit in

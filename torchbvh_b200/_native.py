@@ -574,6 +574,12 @@ def _data(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+def raw_stream(device: torch.device) -> int:
+    """The current stream's handle, without the Python object around it: single-query calls
+    of this section are bound by the host."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def block_table(point_offsets: list[int], query_offsets: list[int]):
     """Host table of a ragged selection: seven int64 a cloud (tbvh_block_table)."""
     clouds = len(point_offsets) - 1
@@ -593,7 +599,7 @@ def select_blocks(geometry: BlockGeometry, total_queries: int, device: torch.dev
     shape = (total_queries, geometry.num_blocks)
     blocks = torch.empty(shape, dtype=torch.int64, device=device)
     distances = torch.empty(shape, dtype=torch.float32, device=device)
-    _check(lib.tbvh_select_blocks(ctypes.byref(geometry), blocks.data_ptr(), distances.data_ptr(), _stream(device)))
+    _check(lib.tbvh_select_blocks(ctypes.byref(geometry), blocks.data_ptr(), distances.data_ptr(), raw_stream(device)))
     # Read by the selection alone; nothing keeps them past this call.
     geometry.query_points = geometry.order = None
     return blocks, distances, plan
@@ -615,9 +621,9 @@ def attend_blocks(geometry: BlockGeometry, queries, keys, values, table, edges, 
     lse = torch.empty(queries.shape[:-1], dtype=torch.float32, device=device) if keep_lse else None
     exact = torch.empty(queries.shape, dtype=torch.float32, device=device) if keep_exact else None
     nbytes = int(lib.tbvh_attend_blocks_workspace_size(ctypes.byref(geometry), ctypes.byref(features)))
-    ws = _workspace(nbytes, device) if nbytes > 256 else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 256 else None
     _check(lib.tbvh_attend_blocks(ctypes.byref(geometry), ctypes.byref(features), out.data_ptr(), _data(lse),
-                                  _data(exact), _data(ws), nbytes, _stream(device)))
+                                  _data(exact), _data(ws), nbytes, raw_stream(device)))
     return out, lse, exact
 
 
@@ -635,7 +641,7 @@ def attend_blocks_backward(geometry: BlockGeometry, queries, keys, values, table
                     device)
     _check(lib.tbvh_attend_blocks_backward(
         ctypes.byref(geometry), ctypes.byref(features), _data(out), _data(exact), lse.data_ptr(), grad_out.data_ptr(),
-        _data(grad_q), _data(grad_k), _data(grad_v), _data(grad_t), ws.data_ptr(), ws.numel(), _stream(device)))
+        _data(grad_q), _data(grad_k), _data(grad_v), _data(grad_t), ws.data_ptr(), ws.numel(), raw_stream(device)))
     return grad_q, grad_k, grad_v, grad_t
 
 
@@ -648,7 +654,7 @@ def distance_bias(squared_distances: torch.Tensor, heads: int, per_head: bool, t
     out = torch.empty((*lead, heads, k), dtype=torch.float32, device=device)
     _check(load_library().tbvh_distance_bias(
         device.index, squared_distances.data_ptr(), rows, heads, k, 1 if per_head else 0, table.data_ptr(),
-        edges.data_ptr(), int(table.size(1)), out.data_ptr(), _stream(device)))
+        edges.data_ptr(), int(table.size(1)), out.data_ptr(), raw_stream(device)))
     return out
 
 
@@ -663,7 +669,7 @@ def distance_bias_backward(squared_distances, heads: int, per_head: bool, edges,
     ws = _workspace(lib.tbvh_distance_bias_backward_workspace_size(rows, heads, k, buckets), device)
     _check(lib.tbvh_distance_bias_backward(
         device.index, squared_distances.data_ptr(), rows, heads, k, 1 if per_head else 0, edges.data_ptr(), buckets,
-        grad_out.data_ptr(), grad.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device)))
+        grad_out.data_ptr(), grad.data_ptr(), ws.data_ptr(), ws.numel(), raw_stream(device)))
     return grad
 
 

@@ -111,14 +111,18 @@ int forward_splits(const BlockSetup& s, const AttendArgs& a) {
   return int(want < 1 ? 1 : want > 32 ? 32 : want);
 }
 
-// Heads of a thread block of the query-tile kernels: at most four (eight warps),
-// fewer where two thread blocks would not share an SM's memory.
+// Heads of a thread block of the query-tile kernels: four (eight warps) share the
+// buckets of a bias, two are enough without one (measured at 65,536 queries, 4
+// heads of 32 / 64 channels, bf16: with bias 319 / 501 us for four and 364 / 521
+// for two; without 242 / 414 and 229 / 357); fewer where two thread blocks would
+// not share an SM's memory.
 void plan_heads(AttendArgs& a, int size, bool back) {
   const int cp = padded_channels(a.channels);
-  int kv = a.group > 4 ? 1 : 4 / a.group;
+  const int most = a.buckets > 0 ? 4 : 2;
+  int kv = a.group > most ? 1 : most / a.group;
   if (kv > a.kv_heads) kv = a.kv_heads;
   a.kv_cta = kv;
-  a.heads_cta = a.group > 4 ? 4 : kv * a.group;
+  a.heads_cta = a.group > most ? most : kv * a.group;
   while (a.heads_cta > 1 &&
          query_tile_smem(size, cp, a.kv_cta, a.heads_cta, back, a.buckets > 0, a.buckets).total > 110 * 1024) {
     if (a.kv_cta > 1) {

@@ -4,8 +4,8 @@
 //   p = 2^(z - lse), dS = p (V dO^T - <dO, O>)  (rows: keys, columns: queries)
 //   dV = sum p dO;  dK = scale sum dS Q
 //
-// A thread block serves one block of 64 keys and up to two key/value heads;
-// four warps a head, 16 keys each. It walks the block's list of queries, 32 a
+// A thread block serves one block of 64 keys and one key/value head; four warps,
+// 16 keys each. It walks the block's list of queries, 32 a
 // step: only those that selected it, so no score is computed in vain, in
 // ascending order, so the sums run in a fixed order without atomics, and over
 // the query heads that share a key/value head. Every key row belongs to exactly
@@ -17,7 +17,11 @@
 
 namespace tbvh {
 
-constexpr int kKvHeads = 2;  // key/value heads of one thread block, at most
+// Key/value heads of one thread block. Two share a step's buckets, but one, and
+// more thread blocks an SM, was faster (16,384 queries, 8 heads of 32, bf16, the
+// whole training pass: 1.10 ms for two, 1.06 for one; 2 heads of 64 shared by 8:
+// 0.99 and 0.86; four: 1.19 and 1.16).
+constexpr int kKvHeads = 1;
 
 struct KeyBlockSmem {
   uint32_t bias, k, v, q, d, lse, delta, places, rows, krows, buckets, pts, kpts, table, total;
@@ -55,7 +59,7 @@ __host__ __device__ inline KeyBlockSmem key_block_smem(int size, int cp, int kvs
 }
 
 template <typename T, int CP>
-__global__ void __launch_bounds__(256) k_key_block(AttendArgs a) {
+__global__ void __launch_bounds__(128 * kKvHeads, CP <= 32 && sizeof(T) == 2 ? 4 : CP <= 64 ? 3 : 2) k_key_block(AttendArgs a) {
   using F = Frag<T>;
   constexpr uint32_t SIZE = sizeof(T);
   constexpr int NT = kTileQueries / 8;
