@@ -16,14 +16,16 @@ namespace {
 
 // Joins the splits of one row: with m = max m_s, l = sum l_s 2^(m_s - m) and
 // o = sum o_s 2^(m_s - m) / l. One warp a row; a lane has one split's m and l,
-// then every 32nd channel of all splits, four splits in flight.
+// then every 32nd channel of all splits, eight splits in flight.
 template <typename T>
 __global__ void __launch_bounds__(256) k_merge(AttendArgs a, int cp) {
   const int64_t tile = blockIdx.x;
   const int head = blockIdx.y, lane = threadIdx.x & 31;
   const int64_t stride = a.map.num_tiles * a.heads * kTileQueries * a.part_row;  // floats between splits
-  for (int q = threadIdx.x >> 5; q < kTileQueries; q += 8) {
-    const int row = a.plan.query_row[tile * kTileQueries + q];
+  const int rows = a.plan.query_row[tile * kTileQueries + lane];  // a tile's missing queries are its last
+  const int there = __popc(__ballot_sync(kFullMask, rows >= 0));
+  for (int q = threadIdx.x >> 5; q < there; q += 8) {
+    const int row = __shfl_sync(kFullMask, rows, q);
     if (row < 0) continue;
     const float* part = a.part + ((tile * a.heads + head) * kTileQueries + q) * a.part_row;
     const bool mine = lane < a.splits;
@@ -39,7 +41,7 @@ __global__ void __launch_bounds__(256) k_merge(AttendArgs a, int cp) {
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFullMask, sum, d);
     float o[4] = {}, fine[4] = {};
     const bool exact = a.out_exact != nullptr;
-#pragma unroll 4
+#pragma unroll 8
     for (int s = 0; s < a.splits; ++s) {
       const float ws = __shfl_sync(kFullMask, w, s);
       const float* p = part + s * stride + 2;

@@ -33,6 +33,10 @@
 namespace tbvh {
 
 constexpr int kStepLeaves = 32;
+#ifndef V_NS
+#define V_NS 2
+#endif
+constexpr int kStages = V_NS;  // steps whose rows are in shared memory or on their way
 constexpr int kBucketRow = kStepLeaves + 8;  // bytes of a query's row of buckets
 
 struct QueryTileSmem {
@@ -51,15 +55,15 @@ __host__ __device__ inline QueryTileSmem query_tile_smem(int size, int cp, int k
     return was;
   };
   if (bias) s.bias = take(heads * kMaxBuckets * 4);
-  s.k = take(2 * kStepLeaves * kv_row);
-  s.v = take(2 * kStepLeaves * kv_row);
+  s.k = take(kStages * kStepLeaves * kv_row);
+  s.v = take(kStages * kStepLeaves * kv_row);
   s.q = take(kTileQueries * q_row);
   s.d = back ? take(kTileQueries * q_row) : 0;
-  s.places = take(2 * kStepLeaves * 4);
+  s.places = take(kStages * kStepLeaves * 4);
   s.rows = take(kTileQueries * 4);
   if (bias) {
     s.buckets = take(2 * kTileQueries * kBucketRow);
-    s.pts = take(2 * 3 * kStepLeaves * 4);
+    s.pts = take(kStages * 3 * kStepLeaves * 4);
     s.qpts = take(kTileQueries * 16);
     s.table = take(sizeof(BucketTable));
     if (back) s.hist = take(uint32_t(buckets) * heads * 64 * 4);
@@ -129,21 +133,21 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
     next_index = uint32_t(sorted[leaf]);
     if (bias) {
       const float* p = leaf_points + int64_t(leaf) * 2 * a.dim;
-      const uint32_t to = base + off.pts + ((i & 1) * 3 * kStepLeaves + lane) * 4;
+      const uint32_t to = base + off.pts + (i % kStages * 3 * kStepLeaves + lane) * 4;
       cp_async<4>(to, p, true);
       cp_async<4>(to + 4 * kStepLeaves, p + 1, true);
       cp_async<4>(to + 8 * kStepLeaves, p + a.dim - 1, a.dim == 3);
     }
   };
   auto copy = [&](int i) {  // by the warp that fetched step i
-    const uint32_t at = base + (i & 1) * stage;
+    const uint32_t at = base + i % kStages * stage;
     copy_words<32>(at + off.k, at + off.v, k_rows, v_rows, checked_row(a, c, next_index) * row_words, columns, kv_rs, lane);
   };
   // Other shapes: the rows go through shared memory to all threads.
-  auto publish = [&](int i) { s_places[(i & 1) * kStepLeaves + lane] = checked_row(a, c, next_index); };
+  auto publish = [&](int i) { s_places[i % kStages * kStepLeaves + lane] = checked_row(a, c, next_index); };
   auto copy_all = [&](int i) {
-    const uint32_t at = base + (i & 1) * stage;
-    const uint32_t* places = s_places + (i & 1) * kStepLeaves;
+    const uint32_t at = base + i % kStages * stage;
+    const uint32_t* places = s_places + i % kStages * kStepLeaves;
     auto row_of = [&](int r) { return int(places[r]); };
     const Rows<T, CP> keys{static_cast<const T*>(a.k), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
     const Rows<T, CP> values{static_cast<const T*>(a.v), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
@@ -155,24 +159,22 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
     const BucketTable& table = *reinterpret_cast<const BucketTable*>(smem + off.table);
     uint8_t* to = s_buckets + slot * kTileQueries * kBucketRow;
     const float4* q = reinterpret_cast<const float4*>(smem + off.qpts);
-    const float* p = reinterpret_cast<const float*>(smem + off.pts) + slot * 3 * kStepLeaves;
+    const float* p = reinterpret_cast<const float*>(smem + off.pts) + i % kStages * 3 * kStepLeaves;
     if (table.crowded) sort_step<true>(to, kBucketRow, table, q, kTileQueries, p, mask);
     else sort_step<false>(to, kBucketRow, table, q, kTileQueries, p, mask);
   };
 
-  clear_padding<T, CP>(smem + off.k, kv_rs, 2 * kStepLeaves, a.kv_cta, a.channels, crew);
-  clear_padding<T, CP>(smem + off.v, kv_rs, 2 * kStepLeaves, a.kv_cta, a.channels, crew);
+  clear_padding<T, CP>(smem + off.k, kv_rs, kStages * kStepLeaves, a.kv_cta, a.channels, crew);
+  clear_padding<T, CP>(smem + off.v, kv_rs, kStages * kStepLeaves, a.kv_cta, a.channels, crew);
   clear_padding<T, CP>(smem + off.q, q_rs, kTileQueries, a.heads_cta, a.channels, crew);
   if constexpr (BACK) clear_padding<T, CP>(smem + off.d, q_rs, kTileQueries, a.heads_cta, a.channels, crew);
-  if (steps > 0 && warp == 0) {
-    fetch(0);
-    if (whole) copy(0);
-    else publish(0);
-  }
-  if (steps > 0 && warp == 1) {
-    fetch(1);
-    if (!whole) publish(1);
-  }
+#pragma unroll
+  for (int i = 0; i < kStages; ++i)
+    if (i < steps && warp == i % warps) {
+      fetch(i);
+      if (!whole) publish(i);
+      else if (i + 1 < kStages) copy(i);
+    }
   if (tid < kTileQueries) {
     s_rows[tid] = a.plan.query_row[tile * kTileQueries + tid];
     if (bias) {
@@ -201,7 +203,8 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
       d.copy(base + off.d, kTileQueries, row_of, crew);
     }
   }
-  if (steps > 0 && !whole) copy_all(0);
+  if (!whole)
+    for (int i = 0; i + 1 < kStages && i < steps; ++i) copy_all(i);
   cp_commit();
   if (bias) reinterpret_cast<BucketTable*>(smem + off.table)->make(a.edges, a.buckets - 1);
   cp_wait<0>();
@@ -246,28 +249,30 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   }
 
   uint2 entry = steps > 0 ? entries[0] : make_uint2(0, 0), next = entry;
-  int copier = 1 % warps, fetcher = 2 % warps;  // of steps i + 1 and i + 2
+  int copier = (kStages - 1) % warps, fetcher = kStages % warps;  // of steps i + kStages - 1 and i + kStages
   for (int i = 0; i < steps; ++i) {
-    cp_wait<0>();
+    cp_wait<kStages - 2>();
     __syncthreads();
-    if (i + 1 < steps) {
-      if (i & 1) next = entries[(i + 1) >> 1];
-      if (!whole) copy_all(i + 1);
-      else if (warp == copier) copy(i + 1);
-      if (warp == fetcher && i + 2 < steps) fetch(i + 2);
+    if (i + kStages - 1 < steps) {
+      if (!whole) copy_all(i + kStages - 1);
+      else if (warp == copier) copy(i + kStages - 1);
+      if (warp == fetcher && i + kStages < steps) fetch(i + kStages);
       copier = fetcher;
       if (++fetcher == warps) fetcher = 0;
+    }
+    if (i + 1 < steps) {
+      if (i & 1) next = entries[(i + 1) >> 1];
       if (bias) sort_pairs(i + 1, next.y);
     }
     cp_commit();
     const unsigned mask = entry.y >> (half * 16);
     const int left = points - first_leaf(entry.x, i);
     entry = next;
-    const bool fetched = warp == copier && i + 2 < steps;  // (the copier of the next step by now)
-    if (!whole && fetched) publish(i + 2);
+    const bool fetched = warp == copier && i + kStages < steps;  // (the copier of the next step by now)
+    if (!whole && fetched) publish(i + kStages);
     if (!mine || (mask & 0xffffu) == 0 || left <= 0) continue;
     const int slot = i & 1;
-    const uint32_t k_at = k_at0 + slot * stage, v_at = v_at0 + slot * stage;
+    const uint32_t k_at = k_at0 + i % kStages * stage, v_at = v_at0 + i % kStages * stage;
     const uint32_t on[2] = {mask >> g & 1u, mask >> (g + 8) & 1u};
     const uint8_t* near = near0 + slot * kTileQueries * kBucketRow;
     // The step's work: written without branches, so that its chains of dependent

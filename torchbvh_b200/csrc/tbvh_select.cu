@@ -76,7 +76,7 @@ int measure_blocks(const char* op, const tbvh_block_geometry* g, BlockSetup& s) 
     return blocks_fail(TBVH_ERR_BAD_ARG, "%s: num_blocks must be 1 to %d", op, kMaxSelect);
   if (g->num_clouds < 1 || g->num_clouds > INT_MAX)
     return blocks_fail(TBVH_ERR_BAD_ARG, "%s: number of clouds must be in [1, 2^31)", op);
-  int64_t most_blocks = 0;
+  int64_t most_blocks = 0, most_queries = 0;
   BlockMap& map = s.map;
   map.num_clouds = int(g->num_clouds);
   if (g->points_per_cloud > 0) {
@@ -91,6 +91,7 @@ int measure_blocks(const char* op, const tbvh_block_geometry* g, BlockSetup& s) 
     map.num_tiles = g->num_clouds * tiles_of(map.m);
     map.num_blocks = g->num_clouds * blocks_of(map.n);
     most_blocks = blocks_of(map.n);
+    most_queries = map.m;
     s.total_points = g->num_clouds * map.n;
     s.total_queries = g->num_clouds * map.m;
   } else {
@@ -110,13 +111,14 @@ int measure_blocks(const char* op, const tbvh_block_geometry* g, BlockSetup& s) 
       if (want.p0 > INT_MAX) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: total point count must fit in signed int32", op);
       if (want.q0 > INT_MAX) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: total query count must fit in signed int32", op);
       if (blocks_of(c.n) > most_blocks) most_blocks = blocks_of(c.n);
+      if (c.m > most_queries) most_queries = c.m;
     }
     map.num_tiles = want.t0;
     map.num_blocks = want.b0;
     s.total_points = want.p0;
     s.total_queries = want.q0;
   }
-  s.plan.capacity = int64_t(kTileQueries) * g->num_blocks;
+  s.plan.capacity = (most_queries < kTileQueries ? most_queries : kTileQueries) * g->num_blocks;
   if (s.plan.capacity > most_blocks) s.plan.capacity = most_blocks;
   return TBVH_OK;
 }
