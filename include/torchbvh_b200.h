@@ -349,12 +349,12 @@ typedef struct tbvh_attend_features {
 } tbvh_attend_features;
 
 /* out [total_queries][heads][channels] of the features' type; for the backward
- * pass lse [total_queries][heads] float32, the base-2 logarithm of each row's
- * sum of exponentials, and out_exact, out before its rounding to 16 bits (both
- * may be NULL: not kept). A row without a key (no block, or all logits
- * -infinity) is 0. */
+ * pass stats [total_queries][heads][2] float32 (8-byte aligned), what it keeps of
+ * each row's softmax, and out_exact, out before its rounding to 16 bits (both may
+ * be NULL: not kept). A row without a key (no block, or all logits -infinity) is
+ * 0. A bias that is finite stays finite: below -FLT_MAX * scale it counts as that. */
 size_t tbvh_attend_blocks_workspace_size(const tbvh_block_geometry* g, const tbvh_attend_features* f);
-int tbvh_attend_blocks(const tbvh_block_geometry* g, const tbvh_attend_features* f, void* out, float* lse,
+int tbvh_attend_blocks(const tbvh_block_geometry* g, const tbvh_attend_features* f, void* out, float* stats,
                        float* out_exact, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gradients from grad_out (shape and type of out). out_exact: used in place of
@@ -365,7 +365,7 @@ int tbvh_attend_blocks(const tbvh_block_geometry* g, const tbvh_attend_features*
  * order: equal inputs give equal bits. */
 size_t tbvh_attend_blocks_backward_workspace_size(const tbvh_block_geometry* g, const tbvh_attend_features* f);
 int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_features* f, const void* out,
-                                const float* out_exact, const float* lse, const void* grad_out, void* grad_queries,
+                                const float* out_exact, const float* stats, const void* grad_out, void* grad_queries,
                                 void* grad_keys, void* grad_values, float* grad_table, void* workspace,
                                 size_t workspace_bytes, void* stream);
 

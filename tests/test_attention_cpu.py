@@ -111,6 +111,19 @@ def test_attend_rejects_bad_shapes():
         attend(q, k, v)
 
 
+@pytest.mark.parametrize("h, kv", [(65, 1), (130, 2), (4097, 4097)])
+def test_attend_rejects_too_many_heads(h, kv):
+    with pytest.raises(ValueError, match="at most 4096 query heads, and 64 to a key head"):
+        torchbvh.attend_blocks(_selection(), *_qkv(h=h, kv=kv, c=1, m=5, n=100))
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e300, float("nan"), float("-inf")])
+def test_attend_rejects_scales_past_float32(scale, monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    with pytest.raises(ValueError, match="scale must be finite in float32"):
+        torchbvh.attend_blocks(_selection(), *_qkv(), scale=scale)
+
+
 @pytest.mark.parametrize("table, edges, text", [
     (torch.zeros(2, 4), None, "must be given together"),
     (None, torch.zeros(3), "must be given together"),

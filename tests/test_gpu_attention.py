@@ -289,6 +289,59 @@ def test_half_gradients_keep_their_precision_at_any_size(scale):
     _check(scene, selection, f, got)
 
 
+def test_half_gradients_of_large_values_stay_in_range():
+    # <grad, value> is up to 2^17 for a gradient of 1: float16's range has room for it only
+    # if the power of two that lifts the gradients looks at the values too.
+    scene = Scene("single", [300], [64], 3, seed=13)
+    selection = scene.select(4)
+    f = _features(scene, F16, 2, 2, 128, 5, seed=13)
+    f["v"][0] = (f["v"][0].float() * 4096).clamp(-65000, 65000).to(F16)
+    f["grad"][0] = (f["grad"][0].float() * 2.0**-12).to(F16)
+    _check(scene, selection, f, _run(scene, selection, f))
+
+
+def test_half_gradients_without_queries():
+    scene = Scene("single", [100], [0], 3, seed=13)
+    selection = scene.select(4)
+    for _ in range(2):  # the workspace is not cleared: fill the memory that it may get
+        torch.full((1 << 20,), 3e4, device="cuda")
+        k = torch.randn((100, 2, 8), device="cuda").half().requires_grad_()
+        torchbvh.attend_blocks(selection, torch.zeros((0, 2, 8), device="cuda").half(), k, k).sum().backward()
+        assert not k.grad.any()  # (NaN is not zero)
+
+
+@pytest.mark.parametrize("scale", [None, 1.0, 40.0, 0.0])
+@pytest.mark.parametrize("size", [-1e9, 3e7, -1e30, torch.finfo(F32).min, torch.finfo(F32).max])
+@pytest.mark.parametrize("queries", [2, 200])
+def test_a_bias_that_all_points_share_changes_nothing(queries, size, scale):
+    # Without products the logits are the bias alone: their differences are 0 exactly, whatever
+    # its size, so every bit of the result is that of no bias.
+    scene = Scene("single", [500], [queries], 3, seed=14)
+    selection = scene.select(5)
+    f = _features(scene, BF16, 2, 2, 32, 3, seed=14)
+    f["q"][0].zero_()
+    f["table"].zero_()
+    want = _run(scene, selection, f, scale=scale)
+    f["table"].fill_(size)
+    for got, plain in zip(_run(scene, selection, f, scale=scale), want):
+        assert torch.equal(got, plain)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["fp32", "fp16", "bf16"])
+def test_a_row_of_the_lowest_bias_is_the_mean(dtype):
+    # What is added to the type's lowest value is rounded away: such logits are equal.
+    scene = Scene("batched", [130] * 2, [40] * 2, 2, seed=15)
+    selection = scene.select(2)
+    f = _features(scene, dtype, 2, 2, 16, 4, seed=15)
+    f["table"].fill_(torch.finfo(F32).min)
+    got = _run(scene, selection, f)
+    assert all(bool(x.isfinite().all()) for x in got)
+    f["q"] = [torch.zeros_like(x) for x in f["q"]]
+    f["table"].zero_()
+    want = _run(scene, selection, f)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(got[3], want[3])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("queries", [1, 2, 31])
 @pytest.mark.parametrize("n", [1, 7, 32])

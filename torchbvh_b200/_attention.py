@@ -20,7 +20,6 @@ same points.
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -193,29 +192,29 @@ def _check_bias(prefix: str, table: torch.Tensor, edges: torch.Tensor, heads: in
 
 class _AttendBlocks(torch.autograd.Function):
     """Attention with the backward pass of the native library. Keeps its inputs,
-    its output and one number a row (the logarithm of the softmax sum). Where a
-    bias table trains with 16-bit features the kept output is float32: the
-    table's gradient sums float32 terms whose errors would otherwise all lean
-    with the rounding of their row's output."""
+    its output and two numbers a row (its softmax's maximum and sum). Where a bias
+    table trains with 16-bit features the kept output is float32: the table's
+    gradient sums float32 terms whose errors would otherwise all lean with the
+    rounding of their row's output."""
 
     @staticmethod
     def forward(ctx, queries, keys, values, table, edges, selection, scale):
         geometry = selection._geometry
         exactly = ctx.needs_input_grad[3] and queries.dtype != torch.float32
-        out, lse, exact = _native.attend_blocks(geometry, queries, keys, values, table, edges, scale, True, exactly)
-        ctx.save_for_backward(queries, keys, values, table, edges, None if exactly else out, exact, lse)
+        out, stats, exact = _native.attend_blocks(geometry, queries, keys, values, table, edges, scale, True, exactly)
+        ctx.save_for_backward(queries, keys, values, table, edges, None if exactly else out, exact, stats)
         ctx.selection, ctx.geometry, ctx.keep, ctx.scale = selection, geometry, selection._keep, scale
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        queries, keys, values, table, edges, out, exact, lse = ctx.saved_tensors
+        queries, keys, values, table, edges, out, exact, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
         if ctx.selection._alive:
             ctx.selection._used_here()
         grads = _native.attend_blocks_backward(ctx.geometry, queries, keys, values, table, edges, ctx.scale, out,
-                                               exact, lse, _as_contiguous(grad_out), need[0], need[1] or need[2],
+                                               exact, stats, _as_contiguous(grad_out), need[0], need[1] or need[2],
                                                need[3] and table is not None)
         return (*(g if wanted else None for g, wanted in zip(grads, need)), None, None, None)
 
@@ -279,8 +278,8 @@ def attend_blocks(selection: BlockSelection, queries: torch.Tensor, keys: torch.
         _check_bias(prefix, bias_table, bias_edges, heads, device, "bias_table", "bias_edges")
         bias_table, bias_edges = _as_contiguous(bias_table), _as_contiguous(bias_edges.detach())
     scale = channels**-0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"{prefix}: scale must be finite")
+    if not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"{prefix}: scale must be finite in float32")
     queries, keys, values = _as_contiguous(queries), _as_contiguous(keys), _as_contiguous(values)
     selection._used_here()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (queries, keys, values, bias_table)):

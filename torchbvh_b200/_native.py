@@ -611,24 +611,24 @@ def _attend_features(queries, keys, values, table, edges, scale: float) -> Atten
                           values.data_ptr(), _data(table), _data(edges))
 
 
-def attend_blocks(geometry: BlockGeometry, queries, keys, values, table, edges, scale: float, keep_lse: bool,
+def attend_blocks(geometry: BlockGeometry, queries, keys, values, table, edges, scale: float, keep_stats: bool,
                   keep_exact: bool):
-    """(out, lse, out before its rounding to 16 bits); the latter two None unless kept."""
+    """(out, softmax statistics, out before its rounding to 16 bits); the latter two None unless kept."""
     lib = load_library()
     device = queries.device
     features = _attend_features(queries, keys, values, table, edges, scale)
     out = torch.empty_like(queries)
-    lse = torch.empty(queries.shape[:-1], dtype=torch.float32, device=device) if keep_lse else None
+    stats = torch.empty((*queries.shape[:-1], 2), dtype=torch.float32, device=device) if keep_stats else None
     exact = torch.empty(queries.shape, dtype=torch.float32, device=device) if keep_exact else None
     nbytes = int(lib.tbvh_attend_blocks_workspace_size(ctypes.byref(geometry), ctypes.byref(features)))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 256 else None
-    _check(lib.tbvh_attend_blocks(ctypes.byref(geometry), ctypes.byref(features), out.data_ptr(), _data(lse),
+    _check(lib.tbvh_attend_blocks(ctypes.byref(geometry), ctypes.byref(features), out.data_ptr(), _data(stats),
                                   _data(exact), _data(ws), nbytes, raw_stream(device)))
-    return out, lse, exact
+    return out, stats, exact
 
 
 def attend_blocks_backward(geometry: BlockGeometry, queries, keys, values, table, edges, scale: float, out,
-                           exact, lse, grad_out, need_queries: bool, need_keys: bool, need_table: bool):
+                           exact, stats, grad_out, need_queries: bool, need_keys: bool, need_table: bool):
     """(grad_queries, grad_keys, grad_values, grad_table), None where not needed."""
     lib = load_library()
     device = queries.device
@@ -640,7 +640,7 @@ def attend_blocks_backward(geometry: BlockGeometry, queries, keys, values, table
     ws = _workspace(lib.tbvh_attend_blocks_backward_workspace_size(ctypes.byref(geometry), ctypes.byref(features)),
                     device)
     _check(lib.tbvh_attend_blocks_backward(
-        ctypes.byref(geometry), ctypes.byref(features), _data(out), _data(exact), lse.data_ptr(), grad_out.data_ptr(),
+        ctypes.byref(geometry), ctypes.byref(features), _data(out), _data(exact), stats.data_ptr(), grad_out.data_ptr(),
         _data(grad_q), _data(grad_k), _data(grad_v), _data(grad_t), ws.data_ptr(), ws.numel(), raw_stream(device)))
     return grad_q, grad_k, grad_v, grad_t
 

@@ -10,15 +10,61 @@
 namespace tbvh {
 namespace {
 
-// delta[row][head] = <grad_out, out>, and for float16 the largest |grad_out|
-// (float bits order like unsigned numbers; a maximum has no order of its own).
+// The largest finite |x| as float bits, which order like unsigned numbers.
+__device__ __forceinline__ unsigned largest_bits(unsigned most, float x) {
+  x = fabsf(x);
+  return x <= FLT_MAX ? max(most, __float_as_uint(x)) : most;
+}
+
+// The block's largest into *most (a maximum has no order of its own).
+__device__ void join_largest(unsigned big, unsigned* most) {
+  __shared__ unsigned s_most[8];
+  big = __reduce_max_sync(kFullMask, big);
+  if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = big;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) big = max(big, s_most[w]);
+    atomicMax(most, big);
+  }
+}
+
+// Largest finite |x| of `count` values; WIDE: read eight at a time.
+template <bool WIDE>
+__global__ void __launch_bounds__(256) k_largest(const __half* x, int64_t count, unsigned* most) {
+  unsigned big = 0;
+  const int64_t first = int64_t(blockIdx.x) * 256 + threadIdx.x, step = int64_t(gridDim.x) * 256;
+  if constexpr (WIDE) {
+    for (int64_t i = first; i < count / 8; i += step) {
+      const uint4 w = reinterpret_cast<const uint4*>(x)[i];
+#pragma unroll
+      for (const unsigned two : {w.x, w.y, w.z, w.w}) {
+        const float2 y = Frag<__half>::unpack(two);
+        big = largest_bits(largest_bits(big, y.x), y.y);
+      }
+    }
+  } else {
+    for (int64_t i = first; i < count; i += step) big = largest_bits(big, __half2float(x[i]));
+  }
+  join_largest(big, most);
+}
+
+cudaError_t run_largest(const __half* x, int64_t count, unsigned* most, cudaStream_t stream) {
+  const bool wide = count % 8 == 0 && uintptr_t(x) % 16 == 0;
+  const int64_t blocks = (count / (wide ? 8 : 1) + 255) / 256;
+  const unsigned grid = unsigned(blocks < 1 ? 1 : blocks > 1184 ? 1184 : blocks);
+  if (wide) k_largest<true><<<grid, 256, 0, stream>>>(x, count, most);
+  else k_largest<false><<<grid, 256, 0, stream>>>(x, count, most);
+  count_launches(1);
+  return cudaGetLastError();
+}
+
+// delta[row][head] = <grad_out, out>, and for float16 the largest finite |grad_out|.
 // `lanes` lanes a (row, head), four channels each at a time where FOUR (rows of
 // whole 16-byte words), else one. Bound by reading both tensors once.
 template <typename T, typename O, bool FOUR>
 __global__ void __launch_bounds__(256) k_delta(const T* grad, const O* out, float* delta, unsigned* most, int64_t rows,
                                                int channels, int lanes) {
-  __shared__ unsigned s_most[8];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t(blockIdx.x) * 256 + threadIdx.x) / lanes;
   const int part = lane & (lanes - 1);
   unsigned big = 0;
@@ -43,20 +89,13 @@ __global__ void __launch_bounds__(256) k_delta(const T* grad, const O* out, floa
       for (int w = 0; w < W; ++w) {
         const float v = Frag<T>::to_float(x[w]);
         sum = fmaf(v, Frag<O>::to_float(y[w]), sum);
-        big = max(big, __float_as_uint(fabsf(v)));
+        big = largest_bits(big, v);
       }
     }
   }
   for (int d = lanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(kFullMask, sum, d);
   if (row < rows && part == 0) delta[row] = sum;
-  if (most == nullptr) return;
-  big = __reduce_max_sync(kFullMask, big);
-  if (lane == 0) s_most[warp] = big;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 8; ++w) big = max(big, s_most[w]);
-    atomicMax(most, big);
-  }
+  if (most != nullptr) join_largest(big, most);
 }
 
 template <typename T>
@@ -102,9 +141,7 @@ BackwardSizes backward_sizes(const BlockSetup& s, const tbvh_attend_features* f)
 // Splits of the forward pass: enough thread blocks for two an SM when the tiles
 // alone are fewer, never more than a tile can have entries.
 int forward_splits(const BlockSetup& s, const AttendArgs& a) {
-  const int64_t groups = a.heads_cta >= a.group ? (a.kv_heads + a.kv_cta - 1) / a.kv_cta
-                                                : int64_t(a.kv_heads) * ((a.group + a.heads_cta - 1) / a.heads_cta);
-  const int64_t blocks = s.map.num_tiles * groups;
+  const int64_t blocks = s.map.num_tiles * head_groups(a);
   if (blocks <= 0 || blocks >= 148) return 1;
   int64_t want = (296 + blocks - 1) / blocks;
   if (want > s.plan.capacity) want = s.plan.capacity;
@@ -205,7 +242,7 @@ size_t tbvh_attend_blocks_workspace_size(const tbvh_block_geometry* g, const tbv
   return size_t(splits) * s.map.num_tiles * f->heads * kTileQueries * (2 * padded_channels(f->channels) + 2) * 4;
 }
 
-int tbvh_attend_blocks(const tbvh_block_geometry* g, const tbvh_attend_features* f, void* out, float* lse,
+int tbvh_attend_blocks(const tbvh_block_geometry* g, const tbvh_attend_features* f, void* out, float* stats,
                        float* out_exact, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace tbvh;
   const char* op = "attend_blocks";
@@ -228,7 +265,7 @@ int tbvh_attend_blocks(const tbvh_block_geometry* g, const tbvh_attend_features*
   if (!words_fit(s, f)) a.width = std::min(a.width, 8);
   a.wide_out = pairs_aligned(f->channels, out);
   a.out = out;
-  a.lse = lse;
+  a.stats = reinterpret_cast<float2*>(stats);
   a.out_exact = out_exact;
   a.part_row = padded_channels(f->channels) * (out_exact ? 2 : 1) + 2;
   a.part = static_cast<float*>(workspace);
@@ -246,7 +283,7 @@ size_t tbvh_attend_blocks_backward_workspace_size(const tbvh_block_geometry* g, 
 }
 
 int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_features* f, const void* out,
-                                const float* out_exact, const float* lse, const void* grad_out, void* grad_queries,
+                                const float* out_exact, const float* stats, const void* grad_out, void* grad_queries,
                                 void* grad_keys, void* grad_values, float* grad_table, void* workspace,
                                 size_t workspace_bytes, void* stream) {
   using namespace tbvh;
@@ -262,7 +299,7 @@ int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_
     return blocks_fail(TBVH_ERR_BAD_ARG, "%s: the selection was made without the backward lists", op);
   if (grad_table && f->num_buckets == 0)
     return blocks_fail(TBVH_ERR_BAD_ARG, "%s: grad_table needs a bias", op);
-  if (s.total_queries > 0 && (!f->queries || (!out && !out_exact) || !lse || !grad_out))
+  if (s.total_queries > 0 && (!f->queries || (!out && !out_exact) || !stats || !grad_out))
     return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL query, output or gradient pointer", op);
   const BackwardSizes b = backward_sizes(s, f);
   if (workspace == nullptr || workspace_bytes < b.total())
@@ -277,12 +314,12 @@ int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_
   float* part = reinterpret_cast<float*>(at);
   at += b.part;
   double* rows = reinterpret_cast<double*>(at);
-  a.lse_in = lse;
+  a.stats_in = reinterpret_cast<const float2*>(stats);
   a.grad_out = grad_out;
   a.grad_q = grad_queries;
   a.grad_k = grad_keys;
   a.grad_v = grad_values;
-  a.grad_max = f->dtype == TBVH_F16 ? most : nullptr;
+  a.largest = f->dtype == TBVH_F16 && s.total_queries > 0 ? most : nullptr;
   a.table_part = grad_table ? part : nullptr;
   const size_t row_bytes = size_t(f->channels) * element_size(f->dtype);
   a.width = copy_width(row_bytes, f->queries, f->keys, f->values);
@@ -296,7 +333,9 @@ int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_
   cudaError_t e = cudaSuccess;
   const int values = f->heads * f->num_buckets;
   if (s.total_queries > 0) {
-    if (a.grad_max) e = cudaMemsetAsync(most, 0, 4, st);
+    if (a.largest) e = cudaMemsetAsync(most, 0, 8, st);
+    if (a.largest && e == cudaSuccess)
+      e = run_largest(static_cast<const __half*>(f->values), s.total_points * f->kv_heads * f->channels, most + 1, st);
     const int64_t pairs = s.total_queries * f->heads;
     if ((pairs + 7) / 8 > INT_MAX) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: too many query rows", op);
     if (e == cudaSuccess) {

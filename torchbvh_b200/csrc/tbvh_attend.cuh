@@ -147,7 +147,7 @@ struct Frag16 {
 template <>
 struct Frag<__nv_bfloat16> : Frag16<__nv_bfloat16> {
   // Probabilities and their gradients enter the second products in 16 bits: a
-  // relative half step of 2^-9 each, the same as the values they multiply.
+  // relative half step of 2^-8 each, the same as the values they multiply.
   __device__ static __forceinline__ uint32_t pack(float x, float y) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
@@ -175,7 +175,7 @@ struct Frag<__nv_bfloat16> : Frag16<__nv_bfloat16> {
 
 template <>
 struct Frag<__half> : Frag16<__half> {
-  // As above with 2^-12; the backward pass scales by a power of two so that
+  // As above with 2^-11; the backward pass scales by a power of two so that
   // small gradients stay normal numbers.
   __device__ static __forceinline__ uint32_t pack(float x, float y) {
     uint32_t r;
@@ -365,13 +365,13 @@ struct Crew {
   int id, count;
 };
 
-// Copies rows of a tensor [row][heads][channels], `here` heads from `first`,
-// `step` apart, into a tile; row_of(r) is the packed row number of tile row r,
+// Copies rows of a tensor [row][heads][channels], `here` heads from `first`, into
+// a tile; row_of(r) is the packed row number of tile row r,
 // negative for zeros. Asynchronous for widths of 4 bytes and more.
 template <typename T, int CP>
 struct Rows {
   const T* src;
-  int heads, channels, first, here, step, width;
+  int heads, channels, first, here, width;
   uint32_t rs;
 
   template <int BYTES, typename RowOf>
@@ -382,7 +382,7 @@ struct Rows {
       const int r = i / per, at = (i - r * per) * E, row = row_of(r);
       const T* p = src + (int64_t(row < 0 ? 0 : row) * heads + first) * channels + at;
       uint32_t d = dst + r * rs + at * uint32_t(sizeof(T));
-      for (int h = 0; h < here; ++h, p += int64_t(step) * channels, d += CP * sizeof(T)) {
+      for (int h = 0; h < here; ++h, p += channels, d += CP * sizeof(T)) {
         if constexpr (BYTES >= 4) {
           cp_async<BYTES>(d, p, row >= 0);
         } else {
@@ -401,20 +401,19 @@ struct Rows {
   }
 };
 
-// ROWS (16 or 32) rows of two tensors of one shape, copied by ONE warp, where a row's heads
-// are one run of `columns` whole 16-byte words on both sides: lane r has row
-// r's place in the tensors, in words, and the lanes share the words of the rows.
+// 32 rows of two tensors of one shape, copied by ONE warp, where a row's heads are
+// one run of `columns` whole 16-byte words on both sides: lane r has row r's place
+// in the tensors, in words, and the lanes share the words of the rows.
 // The warps of a block take turns, a step each: the same copies spread over all
 // warps cost each of them its loop and addresses in every step, three times the
 // instructions. (Bulk copies of a row each, issued by one thread one by one,
 // took 1.7 times as long a step.)
-template <int ROWS>
 __device__ __forceinline__ void copy_words(uint32_t a_tile, uint32_t b_tile, const char* a, const char* b,
                                            uint32_t place, int columns, uint32_t rs, int lane) {
   auto put = [](uint32_t dst, const char* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   };
-  if (columns <= 32 && columns >= 32 / ROWS && (columns & (columns - 1)) == 0) {
+  if (columns <= 32 && (columns & (columns - 1)) == 0) {
     const int rows = 32 / columns, shift = 31 - __clz(columns);  // rows an instruction
     const int column = lane & (columns - 1);
     int r = lane >> shift;
@@ -423,7 +422,7 @@ __device__ __forceinline__ void copy_words(uint32_t a_tile, uint32_t b_tile, con
     a += column * 16;
     b += column * 16;
 #pragma unroll 4
-    for (int i = 0; i < columns; i += 32 / ROWS, r += rows, to += step) {
+    for (int i = 0; i < columns; ++i, r += rows, to += step) {
       const uint64_t at = uint64_t(__shfl_sync(kFullMask, place, r)) * 16;
       put(a_tile + to, a + at);
       put(b_tile + to, b + at);
@@ -431,14 +430,11 @@ __device__ __forceinline__ void copy_words(uint32_t a_tile, uint32_t b_tile, con
   } else {
     int r = lane / columns, column = lane % columns;
     const int dr = 32 / columns, dc = 32 % columns;
-    for (int i = 0; i < ROWS * columns; i += 32) {
-      const bool there = r < ROWS;
+    for (int i = 0; i < 32 * columns; i += 32) {
       const uint64_t at = (uint64_t(__shfl_sync(kFullMask, place, r)) + column) * 16;
       const uint32_t to = r * rs + column * 16;
-      if (there) {
-        put(a_tile + to, a + at);
-        put(b_tile + to, b + at);
-      }
+      put(a_tile + to, a + at);
+      put(b_tile + to, b + at);
       r += dr;
       column += dc;
       if (column >= columns) {
@@ -612,6 +608,11 @@ __device__ __forceinline__ void logits(float (&s)[4][4], const typename Frag<T>:
 struct Units {
   bool folded;
   float unit, bias;
+  // A finite bias stays finite: the type's lowest value everywhere leaves a row its mean.
+  __device__ __forceinline__ float of_bias(float x) const {
+    const float y = x * bias;
+    return fabsf(x) <= FLT_MAX ? fminf(fmaxf(y, -FLT_MAX), FLT_MAX) : y;
+  }
   __device__ __forceinline__ explicit Units(float scale) {
     folded = scale >= 0x1p-30f && scale <= 0x1p30f;
     unit = folded ? scale * kLog2e : 1.0f;
@@ -640,16 +641,16 @@ struct AttendArgs {
   unsigned* status;
   // forward
   void* out;
-  float* lse;      // nullable
+  float2* stats;   // nullable; row_stats of every row and head
   float* out_exact;  // nullable
   int splits;
   float* part;     // splits > 1: [split][tile][head][query] of part_row floats
   int part_row;
   // backward
   const void* grad_out;
-  const float* lse_in;
+  const float2* stats_in;
   float* delta;    // [total_queries][heads] <grad_out, out>
-  const unsigned* grad_max;  // float bits of the largest |grad_out| (float16 only)
+  const unsigned* largest;  // float bits of the largest finite |grad_out| and |value| (float16 only)
   void *grad_q, *grad_k, *grad_v;
   float* table_part;  // [tiles][heads][buckets], nullable
 };
@@ -680,14 +681,21 @@ __host__ __device__ inline int head_groups(const AttendArgs& a) {
                                 : a.kv_heads * ((a.group + a.heads_cta - 1) / a.heads_cta);
 }
 
-// float16: the power of two that brings the largest |grad_out| to [1, 2), so that
-// products of small gradients stay normal numbers; taken out again at the end.
+// float16: the power of two that brings the product of the largest |grad_out| and
+// |value| to [1, 2), so that dS, at most 2 * 2 * 128 of it, stays in float16's range
+// and its small numbers stay normal; taken out again at the end.
 template <typename T>
 __device__ __forceinline__ float gradient_lift(const AttendArgs& a) {
-  if (a.grad_max == nullptr) return 1.0f;
-  const float most = __uint_as_float(*a.grad_max);
-  if (!(most > 0.0f && most <= FLT_MAX)) return 1.0f;
-  return exp2f(-floorf(log2f(most)));
+  if (a.largest == nullptr) return 1.0f;
+  const float most = __uint_as_float(a.largest[0]) * __uint_as_float(a.largest[1]);
+  return most > 0.0f ? exp2f(-floorf(log2f(most))) : 1.0f;
+}
+
+// What the backward pass keeps of a row's softmax: the largest logit, in units of
+// Units, and the base-2 logarithm of the sum (apart, since their sum would round it
+// away under large logits). An empty row keeps an infinite sum: its p come out as 0.
+__device__ __forceinline__ float2 row_stats(float top, float sum) {
+  return sum == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(top, log2f(sum));
 }
 
 // Packed row of index `i` of a cloud's order (of its first point, and an error

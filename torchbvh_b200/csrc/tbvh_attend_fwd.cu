@@ -20,6 +20,7 @@ namespace {
 template <typename T>
 __global__ void __launch_bounds__(256) k_merge(AttendArgs a, int cp) {
   const int64_t tile = blockIdx.x;
+  const float unit = Units(a.scale).unit;
   const int head = blockIdx.y, lane = threadIdx.x & 31;
   const int64_t stride = a.map.num_tiles * a.heads * kTileQueries * a.part_row;  // floats between splits
   const int rows = a.plan.query_row[tile * kTileQueries + lane];  // a tile's missing queries are its last
@@ -35,7 +36,7 @@ __global__ void __launch_bounds__(256) k_merge(AttendArgs a, int cp) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(kFullMask, most, d));
     const float base = most == -INFINITY ? 0.0f : most;
-    const float w = exp2_fast(top - base);
+    const float w = exp2_fast((top - base) * unit);
     sum *= w;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFullMask, sum, d);
@@ -62,8 +63,7 @@ __global__ void __launch_bounds__(256) k_merge(AttendArgs a, int cp) {
         if (exact) a.out_exact[(int64_t(row) * a.heads + head) * a.channels + lane + 32 * i] = (o[i] + fine[i]) * inv;
       }
     }
-    if (a.lse != nullptr && lane == 0)
-      a.lse[int64_t(row) * a.heads + head] = sum == 0.0f ? INFINITY : most + log2f(sum);
+    if (a.stats != nullptr && lane == 0) a.stats[int64_t(row) * a.heads + head] = row_stats(most, sum);
   }
 }
 

@@ -1,51 +1,48 @@
 // Block attention by key block: the part of the backward pass that sums over
 // queries.
 //
-//   p = 2^(z - lse), dS = p (V dO^T - <dO, O>)  (rows: keys, columns: queries)
+//   p = 2^(z - m - log2 l), dS = p (V dO^T - <dO, O>)  (rows: keys, columns: queries)
 //   dV = sum p dO;  dK = scale sum dS Q
 //
 // A thread block serves one block of 64 keys and one key/value head; four warps,
-// 16 keys each. It walks the block's list of queries, 32 a
-// step: only those that selected it, so no score is computed in vain, in
-// ascending order, so the sums run in a fixed order without atomics, and over
-// the query heads that share a key/value head. Every key row belongs to exactly
-// one block, so every gradient row is written once, also for blocks that nobody
-// selected.
+// 16 keys each. It walks the block's list of queries, 32 a step: only those that
+// selected it, so no score is computed in vain, in ascending order, so the sums
+// run in a fixed order without atomics, and over the query heads that share the
+// key/value head. Every key row belongs to exactly one block, so every gradient
+// row is written once, also for blocks that nobody selected.
+//
+// Two or four key/value heads a thread block would share a step's buckets, but
+// one, and more thread blocks an SM, was faster (16,384 queries, 8 heads of 32,
+// bf16, the whole training pass: 1.06 ms for one, 1.10 for two, 1.19 for four; 2
+// heads of 64 shared by 8: 0.86, 0.99 and 1.16).
 #pragma once
 
 #include "tbvh_attend.cuh"
 
 namespace tbvh {
 
-// Key/value heads of one thread block. Two share a step's buckets, but one, and
-// more thread blocks an SM, was faster (16,384 queries, 8 heads of 32, bf16, the
-// whole training pass: 1.10 ms for two, 1.06 for one; 2 heads of 64 shared by 8:
-// 0.99 and 0.86; four: 1.19 and 1.16).
-constexpr int kKvHeads = 1;
-
 struct KeyBlockSmem {
-  uint32_t bias, k, v, q, d, lse, delta, places, rows, krows, buckets, pts, kpts, table, total;
+  uint32_t bias, k, v, q, d, stats, delta, rows, krows, buckets, pts, kpts, table, total;
 };
 
 constexpr int kKeyBucketRow = kTileQueries + 8;  // bytes of a key's row of buckets
 
-__host__ __device__ inline KeyBlockSmem key_block_smem(int size, int cp, int kvs, int group, bool bias) {
+__host__ __device__ inline KeyBlockSmem key_block_smem(int size, int cp, int group, bool bias) {
   KeyBlockSmem s{};
-  const uint32_t row = uint32_t(kvs * cp * size + 16);
+  const uint32_t row = uint32_t(cp * size + 16);
   uint32_t at = 0;
   auto take = [&](uint32_t bytes) {
     const uint32_t was = at;
     at += (bytes + 15) / 16 * 16;
     return was;
   };
-  if (bias) s.bias = take(kvs * group * kMaxBuckets * 4);
+  if (bias) s.bias = take(group * kMaxBuckets * 4);
   s.k = take(kBlockLeaves * row);
   s.v = take(kBlockLeaves * row);
   s.q = take(2 * kTileQueries * row);
   s.d = take(2 * kTileQueries * row);
-  s.lse = take(2 * kvs * kTileQueries * 4);
-  s.delta = take(2 * kvs * kTileQueries * 4);
-  s.places = take(2 * kTileQueries * 4);
+  s.stats = take(2 * kTileQueries * 8);
+  s.delta = take(2 * kTileQueries * 4);
   s.rows = take(2 * kTileQueries * 4);
   s.krows = take(kBlockLeaves * 4);
   if (bias) {
@@ -59,7 +56,8 @@ __host__ __device__ inline KeyBlockSmem key_block_smem(int size, int cp, int kvs
 }
 
 template <typename T, int CP>
-__global__ void __launch_bounds__(128 * kKvHeads, CP <= 32 && sizeof(T) == 2 ? 4 : CP <= 64 ? 3 : 2) k_key_block(AttendArgs a) {
+__global__ void __launch_bounds__(128, CP <= 32 && sizeof(T) == 2 ? 4 : CP <= 64 ? 3 : 2)
+    k_key_block(AttendArgs a) {
   using F = Frag<T>;
   constexpr uint32_t SIZE = sizeof(T);
   constexpr int NT = kTileQueries / 8;
@@ -70,23 +68,21 @@ __global__ void __launch_bounds__(128 * kKvHeads, CP <= 32 && sizeof(T) == 2 ? 4
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Crew crew{tid, int(blockDim.x)};
   const int64_t block = blockIdx.x;
-  const int kv0 = blockIdx.y * a.kv_cta;
-  const int kvs = min(a.kv_cta, a.kv_heads - kv0);
+  const int kv = blockIdx.y;
   const BlockCloud c = a.map.of_block(block);
   const bool bias = a.table != nullptr;
-  const KeyBlockSmem off = key_block_smem(sizeof(T), CP, a.kv_cta, a.group, bias);
+  const KeyBlockSmem off = key_block_smem(sizeof(T), CP, a.group, bias);
   const uint32_t base = smem_u32(smem);
-  float* s_lse = reinterpret_cast<float*>(smem + off.lse);
+  float2* s_stats = reinterpret_cast<float2*>(smem + off.stats);
   float* s_delta = reinterpret_cast<float*>(smem + off.delta);
   int* s_rows = reinterpret_cast<int*>(smem + off.rows);
-  uint32_t* s_places = reinterpret_cast<uint32_t*>(smem + off.places);
   int* s_krows = reinterpret_cast<int*>(smem + off.krows);
   float* s_bias = reinterpret_cast<float*>(smem + off.bias);
   uint8_t* s_buckets = reinterpret_cast<uint8_t*>(smem + off.buckets);
   float* s_pts = reinterpret_cast<float*>(smem + off.pts);
   float4* s_kpts = reinterpret_cast<float4*>(smem + off.kpts);  // negated
   BucketTable& s_table = *reinterpret_cast<BucketTable*>(smem + off.table);
-  const uint32_t rs = row_bytes<T, CP>(a.kv_cta);
+  const uint32_t rs = row_bytes<T, CP>(1);
   const uint32_t stage = kTileQueries * rs;
 
   const int64_t begin = a.plan.query_begin[block];
@@ -95,7 +91,7 @@ __global__ void __launch_bounds__(128 * kKvHeads, CP <= 32 && sizeof(T) == 2 ? 4
   const uint32_t* list = a.plan.list + begin;
   const int64_t leaf0 = (block - c.b0) * kBlockLeaves;
   const int valid = c.n - leaf0 < kBlockLeaves ? int(c.n - leaf0) : kBlockLeaves;
-  // Steps: every chunk once for each query head that shares a key/value head.
+  // Steps: every chunk once for each query head that shares the key/value head.
   const int group = a.group;
   const int64_t steps = int64_t(chunks) * group;
   const Units units(a.scale);
@@ -111,8 +107,6 @@ __global__ void __launch_bounds__(128 * kKvHeads, CP <= 32 && sizeof(T) == 2 ? 4
   // three chunks ahead, for their rows and points two chunks ahead (one query a
   // lane), and copies the rows one step ahead.
   const bool whole = a.width == 16 && a.channels == CP;
-  // Heads that lie side by side are copied as one; those of shared keys lie `group` apart.
-  const int runs = group == 1 ? 1 : kvs, columns = kvs / runs * CP * int(SIZE) / 16;
   const int row_words = a.heads * CP * int(SIZE) / 16;
   const int warps = int(blockDim.x) / 32;
   uint32_t next_slot = 0;
@@ -135,30 +129,27 @@ __global__ void __launch_bounds__(128 * kKvHeads, CP <= 32 && sizeof(T) == 2 ? 4
   auto copy = [&](int64_t step, int e, int member) {  // step = e * group + member, by one warp (or all)
     const int slot = int(step & 1);
     const int* rows = s_rows + (e & 1) * kTileQueries;
-    const int first = kv0 * group + member;  // query heads kv * group + member, one a key/value head
+    const int head = kv * group + member;
     const uint32_t to = base + slot * stage;
     if (whole) {
-      for (int h = 0; h < runs; ++h) {
-        const int64_t begin = int64_t(first + h * group) * CP * SIZE;
-        copy_words<32>(to + off.q + h * CP * SIZE, to + off.d + h * CP * SIZE, static_cast<const char*>(a.q) + begin,
-                       static_cast<const char*>(a.grad_out) + begin, uint32_t(rows[lane]) * row_words, columns, rs, lane);
-      }
+      const int64_t begin = int64_t(head) * CP * SIZE;
+      copy_words(to + off.q, to + off.d, static_cast<const char*>(a.q) + begin,
+                 static_cast<const char*>(a.grad_out) + begin, uint32_t(rows[lane]) * row_words, CP * int(SIZE) / 16, rs,
+                 lane);
     } else {
       auto row_of = [&](int r) { return rows[r]; };
-      const Rows<T, CP> q{static_cast<const T*>(a.q), a.heads, a.channels, first, kvs, group, a.width, rs};
-      const Rows<T, CP> d{static_cast<const T*>(a.grad_out), a.heads, a.channels, first, kvs, group, a.width, rs};
+      const Rows<T, CP> q{static_cast<const T*>(a.q), a.heads, a.channels, head, 1, a.width, rs};
+      const Rows<T, CP> d{static_cast<const T*>(a.grad_out), a.heads, a.channels, head, 1, a.width, rs};
       q.copy(to + off.q, kTileQueries, row_of, crew);
       d.copy(to + off.d, kTileQueries, row_of, crew);
       if (warp != 0) return;
     }
-    for (int h = 0; h < kvs; ++h) {
-      const int64_t at = int64_t(rows[lane]) * a.heads + (kv0 + h) * group + member;
-      float* lse = s_lse + (slot * a.kv_cta + h) * kTileQueries + lane;
-      // Past the list's end the sum is infinite: p = 0.
-      if (e * kTileQueries + lane < listed) cp_async<4>(smem_u32(lse), a.lse_in + at, true);
-      else *lse = INFINITY;
-      cp_async<4>(smem_u32(s_delta + (slot * a.kv_cta + h) * kTileQueries + lane), a.delta + at, true);
-    }
+    const int64_t at = int64_t(rows[lane]) * a.heads + head;
+    float2* stats = s_stats + slot * kTileQueries + lane;
+    // Past the list's end the sum is infinite: p = 0.
+    if (e * kTileQueries + lane < listed) cp_async<8>(smem_u32(stats), a.stats_in + at, true);
+    else *stats = make_float2(0.0f, INFINITY);
+    cp_async<4>(smem_u32(s_delta + slot * kTileQueries + lane), a.delta + at, true);
   };
   auto sort_pairs = [&](int e) {  // distance buckets of chunk e
     if (bias && e < chunks) {
@@ -170,13 +161,13 @@ __global__ void __launch_bounds__(128 * kKvHeads, CP <= 32 && sizeof(T) == 2 ? 4
     }
   };
 
-  clear_padding<T, CP>(smem + off.k, rs, kBlockLeaves, a.kv_cta, a.channels, crew);
-  clear_padding<T, CP>(smem + off.v, rs, kBlockLeaves, a.kv_cta, a.channels, crew);
-  clear_padding<T, CP>(smem + off.q, rs, 2 * kTileQueries, a.kv_cta, a.channels, crew);
-  clear_padding<T, CP>(smem + off.d, rs, 2 * kTileQueries, a.kv_cta, a.channels, crew);
+  clear_padding<T, CP>(smem + off.k, rs, kBlockLeaves, 1, a.channels, crew);
+  clear_padding<T, CP>(smem + off.v, rs, kBlockLeaves, 1, a.channels, crew);
+  clear_padding<T, CP>(smem + off.q, rs, 2 * kTileQueries, 1, a.channels, crew);
+  clear_padding<T, CP>(smem + off.d, rs, 2 * kTileQueries, 1, a.channels, crew);
   if (bias)
-    for (int i = tid; i < kvs * group * a.buckets; i += blockDim.x)
-      s_bias[(i / a.buckets) * kMaxBuckets + i % a.buckets] = a.table[int64_t(kv0) * group * a.buckets + i] * units.bias;
+    for (int i = tid; i < group * a.buckets; i += blockDim.x)
+      s_bias[(i / a.buckets) * kMaxBuckets + i % a.buckets] = units.of_bias(a.table[int64_t(kv) * group * a.buckets + i]);
   if (warp < 2 && warp < chunks) {
     ask_list(warp);
     ask_rows();
@@ -186,8 +177,8 @@ __global__ void __launch_bounds__(128 * kKvHeads, CP <= 32 && sizeof(T) == 2 ? 4
   __syncthreads();
   {
     auto row_of = [&](int r) { return s_krows[r]; };
-    const Rows<T, CP> keys{static_cast<const T*>(a.k), a.kv_heads, a.channels, kv0, kvs, 1, a.width, rs};
-    const Rows<T, CP> values{static_cast<const T*>(a.v), a.kv_heads, a.channels, kv0, kvs, 1, a.width, rs};
+    const Rows<T, CP> keys{static_cast<const T*>(a.k), a.kv_heads, a.channels, kv, 1, a.width, rs};
+    const Rows<T, CP> values{static_cast<const T*>(a.v), a.kv_heads, a.channels, kv, 1, a.width, rs};
     keys.copy(base + off.k, kBlockLeaves, row_of, crew);
     values.copy(base + off.v, kBlockLeaves, row_of, crew);
   }
@@ -201,14 +192,12 @@ __global__ void __launch_bounds__(128 * kKvHeads, CP <= 32 && sizeof(T) == 2 ? 4
   cp_wait<0>();
   __syncthreads();
 
-  const int kv = warp >> 2, quarter = warp & 3;
-  const bool mine = kv < kvs && quarter * 16 < valid;
+  const bool mine = warp * 16 < valid;
   const int g = lane >> 2, t = lane & 3;
   // Byte addresses with the lane's offset; query tiles of stage 0.
-  const uint32_t head_at = base + kv * CP * SIZE;
-  const uint32_t k_at = head_at + off.k + quarter * 16 * rs + F::lane_a(rs, lane), v_at = k_at + (off.v - off.k);
+  const uint32_t k_at = base + off.k + warp * 16 * rs + F::lane_a(rs, lane), v_at = k_at + (off.v - off.k);
   const uint32_t nk = F::lane_nk(rs, lane), kn = F::lane_kn(rs, lane);
-  const uint8_t* near0 = s_buckets + (quarter * 16 + g) * kKeyBucketRow + 8 * t;
+  const uint8_t* near0 = s_buckets + (warp * 16 + g) * kKeyBucketRow + 8 * t;
   const float lift = gradient_lift<T>(a), unit = units.unit;
   typename F::A held_k[HOLD], held_v[HOLD];
   if constexpr (HELD) {
@@ -233,10 +222,10 @@ __global__ void __launch_bounds__(128 * kKvHeads, CP <= 32 && sizeof(T) == 2 ? 4
     if (last && e + 3 < chunks && warp == (e + 3) % warps) ask_list(e + 3);
     if (mine) {
       const int slot = int(step & 1);
-      const uint32_t q_at = head_at + off.q + slot * stage, d_at = head_at + off.d + slot * stage;
-      const float* lse = s_lse + (slot * a.kv_cta + kv) * kTileQueries + 2 * t;
-      const float* delta = s_delta + (slot * a.kv_cta + kv) * kTileQueries + 2 * t;
-      const uint32_t head_bias = base + off.bias + (kv * group + member) * kMaxBuckets * 4;
+      const uint32_t q_at = base + off.q + slot * stage, d_at = base + off.d + slot * stage;
+      const float2* stats = s_stats + slot * kTileQueries + 2 * t;
+      const float* delta = s_delta + slot * kTileQueries + 2 * t;
+      const uint32_t head_bias = base + off.bias + member * kMaxBuckets * 4;
       float s[NT][4], ds[NT][4];
       const uint8_t* near = near0 + (e & 1) * kBlockLeaves * kKeyBucketRow;
       if (bias)
@@ -248,12 +237,13 @@ __global__ void __launch_bounds__(128 * kKvHeads, CP <= 32 && sizeof(T) == 2 ? 4
       multiply_nk<T, CP, NT, HELD, true>(ds, held_v, v_at, rs, d_at + nk, rs);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float2 l = *reinterpret_cast<const float2*>(lse + n * 8);
+        const float4 m = *reinterpret_cast<const float4*>(stats + n * 8);
         const float2 d = *reinterpret_cast<const float2*>(delta + n * 8);
-        const Pair minus_l = pair(-l.x, -l.y), minus_d = pair(-d.x, -d.y);
+        const Pair minus_top = pair(-m.x, -m.z), minus_logsum = pair(-m.y, -m.w), minus_d = pair(-d.x, -d.y);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float2 x = unpair(fma2(pair(s[n][2 * r], s[n][2 * r + 1]), both(unit), minus_l));
+          const Pair z = add2(pair(s[n][2 * r], s[n][2 * r + 1]), minus_top);
+          const float2 x = unpair(fma2(z, both(unit), minus_logsum));
           s[n][2 * r] = exp2_fast(x.x);
           s[n][2 * r + 1] = exp2_fast(x.y);
           Pair y = add2(pair(ds[n][2 * r], ds[n][2 * r + 1]), minus_d);
@@ -324,9 +314,9 @@ __global__ void __launch_bounds__(128 * kKvHeads, CP <= 32 && sizeof(T) == 2 ? 4
     const float back = a.scale / lift;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int row = s_krows[quarter * 16 + g + 8 * r];
+      const int row = s_krows[warp * 16 + g + 8 * r];
       if (row < 0) continue;
-      const int64_t at = (int64_t(row) * a.kv_heads + kv0 + kv) * a.channels;
+      const int64_t at = (int64_t(row) * a.kv_heads + kv) * a.channels;
       T* out_k = static_cast<T*>(a.grad_k) + at;
       T* out_v = static_cast<T*>(a.grad_v) + at;
 #pragma unroll
@@ -339,17 +329,12 @@ __global__ void __launch_bounds__(128 * kKvHeads, CP <= 32 && sizeof(T) == 2 ? 4
 }
 
 template <typename T, int CP>
-cudaError_t run_key_block(AttendArgs a, cudaStream_t stream) {
-  a.kv_cta = a.kv_heads < kKvHeads ? a.kv_heads : kKvHeads;
-  KeyBlockSmem s = key_block_smem(sizeof(T), CP, a.kv_cta, a.group, a.table != nullptr);
-  if (s.total > 200 * 1024 && a.kv_cta > 1) {
-    a.kv_cta = 1;
-    s = key_block_smem(sizeof(T), CP, a.kv_cta, a.group, a.table != nullptr);
-  }
+cudaError_t run_key_block(const AttendArgs& a, cudaStream_t stream) {
+  const KeyBlockSmem s = key_block_smem(sizeof(T), CP, a.group, a.table != nullptr);
   const cudaError_t e = allow_smem(k_key_block<T, CP>, s.total);
   if (e != cudaSuccess) return e;
-  const dim3 grid(unsigned(a.map.num_blocks), unsigned((a.kv_heads + a.kv_cta - 1) / a.kv_cta));
-  k_key_block<T, CP><<<grid, a.kv_cta * 128, s.total, stream>>>(a);
+  const dim3 grid(unsigned(a.map.num_blocks), unsigned(a.kv_heads));
+  k_key_block<T, CP><<<grid, 128, s.total, stream>>>(a);
   return cudaGetLastError();
 }
 

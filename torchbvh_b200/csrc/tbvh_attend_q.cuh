@@ -13,7 +13,7 @@
 //
 //   forward    m, l: running maximum and sum (32 bits); o: sum of p V
 //              o <- o 2^(m_old - m) + p V in one pass over the keys
-//   backward   p = 2^(z - lse), dS = p (dO V^T - <dO, O>)
+//   backward   p = 2^(z - m - log2 l), dS = p (dO V^T - <dO, O>)
 //              dQ = scale sum dS K;  dT[h][bucket] += dS
 //
 // EXACT (forward, 16-bit features whose bias table trains): the parts of the
@@ -33,10 +33,10 @@
 namespace tbvh {
 
 constexpr int kStepLeaves = 32;
-#ifndef V_NS
-#define V_NS 2
-#endif
-constexpr int kStages = V_NS;  // steps whose rows are in shared memory or on their way
+// Steps whose rows are in shared memory or on their way. Three take the memory of
+// a third thread block an SM: 16,384 queries, 8 heads of 32, bf16, with bias, the
+// whole training pass 1.23 ms for three and 1.09 for two.
+constexpr int kStages = 2;
 constexpr int kBucketRow = kStepLeaves + 8;  // bytes of a query's row of buckets
 
 struct QueryTileSmem {
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   };
   auto copy = [&](int i) {  // by the warp that fetched step i
     const uint32_t at = base + i % kStages * stage;
-    copy_words<32>(at + off.k, at + off.v, k_rows, v_rows, checked_row(a, c, next_index) * row_words, columns, kv_rs, lane);
+    copy_words(at + off.k, at + off.v, k_rows, v_rows, checked_row(a, c, next_index) * row_words, columns, kv_rs, lane);
   };
   // Other shapes: the rows go through shared memory to all threads.
   auto publish = [&](int i) { s_places[i % kStages * kStepLeaves + lane] = checked_row(a, c, next_index); };
@@ -149,8 +149,8 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
     const uint32_t at = base + i % kStages * stage;
     const uint32_t* places = s_places + i % kStages * kStepLeaves;
     auto row_of = [&](int r) { return int(places[r]); };
-    const Rows<T, CP> keys{static_cast<const T*>(a.k), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
-    const Rows<T, CP> values{static_cast<const T*>(a.v), a.kv_heads, a.channels, span.kv0, span.kvs, 1, a.width, kv_rs};
+    const Rows<T, CP> keys{static_cast<const T*>(a.k), a.kv_heads, a.channels, span.kv0, span.kvs, a.width, kv_rs};
+    const Rows<T, CP> values{static_cast<const T*>(a.v), a.kv_heads, a.channels, span.kv0, span.kvs, a.width, kv_rs};
     keys.copy(at + off.k, kStepLeaves, row_of, crew);
     values.copy(at + off.v, kStepLeaves, row_of, crew);
   };
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   if (bias) {
     float* s_bias = reinterpret_cast<float*>(smem + off.bias);
     for (int i = tid; i < span.heads * a.buckets; i += blockDim.x)
-      s_bias[(i / a.buckets) * kMaxBuckets + i % a.buckets] = a.table[int64_t(span.h0) * a.buckets + i] * units.bias;
+      s_bias[(i / a.buckets) * kMaxBuckets + i % a.buckets] = units.of_bias(a.table[int64_t(span.h0) * a.buckets + i]);
     // Rows that a step leaves unsorted are still looked up (and dropped): they must hold offsets.
     for (int i = tid; i < 2 * kTileQueries * kBucketRow / 4; i += blockDim.x)
       reinterpret_cast<uint32_t*>(s_buckets)[i] = 0;
@@ -196,10 +196,10 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   __syncthreads();
   {
     auto row_of = [&](int r) { return s_rows[r]; };
-    const Rows<T, CP> q{static_cast<const T*>(a.q), a.heads, a.channels, span.h0, span.heads, 1, a.width, q_rs};
+    const Rows<T, CP> q{static_cast<const T*>(a.q), a.heads, a.channels, span.h0, span.heads, a.width, q_rs};
     q.copy(base + off.q, kTileQueries, row_of, crew);
     if constexpr (BACK) {
-      const Rows<T, CP> d{static_cast<const T*>(a.grad_out), a.heads, a.channels, span.h0, span.heads, 1, a.width, q_rs};
+      const Rows<T, CP> d{static_cast<const T*>(a.grad_out), a.heads, a.channels, span.h0, span.heads, a.width, q_rs};
       d.copy(base + off.d, kTileQueries, row_of, crew);
     }
   }
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   Pair acc[CP / 8][2] = {};  // rows g and g + 8
   Pair fine[EXACT ? CP / 8 : 1][2] = {};
   float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};  // forward: running maximum, sum
-  float lse[2] = {INFINITY, INFINITY}, delta[2] = {0.0f, 0.0f};  // backward
+  float logsum[2] = {INFINITY, INFINITY}, delta[2] = {0.0f, 0.0f};  // backward
   float lift = 1.0f;  // float16: power of two that brings the gradients to order 1
   if constexpr (BACK) {
     lift = gradient_lift<T>(a);
@@ -242,7 +242,9 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
     for (int r = 0; r < 2; ++r) {
       const int row = s_rows[half * 16 + g + 8 * r];
       if (mine && row >= 0) {
-        lse[r] = a.lse_in[int64_t(row) * a.heads + span.h0 + head];
+        const float2 stats = a.stats_in[int64_t(row) * a.heads + span.h0 + head];
+        top[r] = stats.x;
+        logsum[r] = stats.y;
         delta[r] = a.delta[int64_t(row) * a.heads + span.h0 + head];
       }
     }
@@ -279,132 +281,136 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
     // instructions overlap; the rare forms (the cloud's last leaves, scales that are
     // not folded) have their own copy.
     auto work = [&](auto biased, auto plain) {
-    constexpr bool BIASED = decltype(biased)::value, PLAIN = decltype(plain)::value;
-    float s[NT][4];
-    logits<T, CP, HELD, BIASED, PLAIN>(s, held_q, q_at, q_rs, k_at + nk, kv_rs, head_bias, near, 8 * kBucketRow,
-                                       a.scale * kLog2e, units.folded);
-    if constexpr (!PLAIN) {
+      constexpr bool BIASED = decltype(biased)::value, PLAIN = decltype(plain)::value;
+      float s[NT][4];
+      logits<T, CP, HELD, BIASED, PLAIN>(s, held_q, q_at, q_rs, k_at + nk, kv_rs, head_bias, near, 8 * kBucketRow,
+                                         a.scale * kLog2e, units.folded);
+      if constexpr (!PLAIN) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n * 8 + 2 * t + (j & 1) >= left) s[n][j] = -INFINITY;
-    }
-    if constexpr (!BACK) {
-      Pair shrink[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float most = top[r];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) most = max3(most, s[n][2 * r], s[n][2 * r + 1]);
-        most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
-        const float from_top = most == -INFINITY ? 0.0f : -most * unit;  // nothing yet: all p are 0
-        const float fade = exp2_fast(fmaf(top[r], unit, from_top));
-        Pair add;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const float2 x = unpair(fma2(pair(s[n][2 * r], s[n][2 * r + 1]), both(unit), both(from_top)));
-          s[n][2 * r] = exp2_fast(x.x);
-          s[n][2 * r + 1] = exp2_fast(x.y);
-          const Pair p = pair(s[n][2 * r], s[n][2 * r + 1]);
-          add = n == 0 ? p : add2(add, p);
-        }
-        const float grown = fmaf(sum[r], fade, unpair(add).x + unpair(add).y);
-        top[r] = on[r] ? most : top[r];
-        sum[r] = on[r] ? grown : sum[r];
-        shrink[r] = both(fade);
+          for (int j = 0; j < 4; ++j)
+            if (n * 8 + 2 * t + (j & 1) >= left) s[n][j] = -INFINITY;
       }
+      if constexpr (!BACK) {
+        Pair shrink[2];
 #pragma unroll
-      for (int n0 = 0; n0 < CP / 8; n0 += kChannelGroup) {
-        float part[kChannelGroup][4], low[EXACT ? kChannelGroup : 1][4];
+        for (int r = 0; r < 2; ++r) {
+          float most = top[r];
 #pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-          typename F::A p, rest;
-          from_acc<T>(p, s, st);
-          if constexpr (EXACT) rest_of_acc<T>(rest, p, s, st);
+          for (int n = 0; n < NT; ++n) most = max3(most, s[n][2 * r], s[n][2 * r + 1]);
+          most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
+          most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
+          // Subtracted before the factor, which would round large logits apart.
+          const float down = most == -INFINITY ? 0.0f : -most;  // nothing yet: all p are 0
+          const float fade = exp2_fast((top[r] + down) * unit);
+          Pair add;
 #pragma unroll
-          for (int j = 0; j < kChannelGroup / 2; ++j) {
-            typename F::B b;
-            F::pair_kn(b, v_at + kn + st * F::STEP * kv_rs + (n0 + 2 * j) * 8 * SIZE, kv_rs);
-            if (st == 0) {
-              F::mma_first(part[2 * j], p, b[0], b[1]);
-              F::mma_first(part[2 * j + 1], p, b[2], b[3]);
-              if constexpr (EXACT) {
-                F::mma_first(low[2 * j], rest, b[0], b[1]);
-                F::mma_first(low[2 * j + 1], rest, b[2], b[3]);
+          for (int n = 0; n < NT; ++n) {
+            const float2 x = unpair(mul2(add2(pair(s[n][2 * r], s[n][2 * r + 1]), both(down)), both(unit)));
+            s[n][2 * r] = exp2_fast(x.x);
+            s[n][2 * r + 1] = exp2_fast(x.y);
+            const Pair p = pair(s[n][2 * r], s[n][2 * r + 1]);
+            add = n == 0 ? p : add2(add, p);
+          }
+          const float grown = fmaf(sum[r], fade, unpair(add).x + unpair(add).y);
+          top[r] = on[r] ? most : top[r];
+          sum[r] = on[r] ? grown : sum[r];
+          shrink[r] = both(fade);
+        }
+#pragma unroll
+        for (int n0 = 0; n0 < CP / 8; n0 += kChannelGroup) {
+          float part[kChannelGroup][4];
+          [[maybe_unused]] float low[EXACT ? kChannelGroup : 1][4];
+#pragma unroll
+          for (int st = 0; st < STEPS; ++st) {
+            typename F::A p;
+            [[maybe_unused]] typename F::A rest;
+            from_acc<T>(p, s, st);
+            if constexpr (EXACT) rest_of_acc<T>(rest, p, s, st);
+#pragma unroll
+            for (int j = 0; j < kChannelGroup / 2; ++j) {
+              typename F::B b;
+              F::pair_kn(b, v_at + kn + st * F::STEP * kv_rs + (n0 + 2 * j) * 8 * SIZE, kv_rs);
+              if (st == 0) {
+                F::mma_first(part[2 * j], p, b[0], b[1]);
+                F::mma_first(part[2 * j + 1], p, b[2], b[3]);
+                if constexpr (EXACT) {
+                  F::mma_first(low[2 * j], rest, b[0], b[1]);
+                  F::mma_first(low[2 * j + 1], rest, b[2], b[3]);
+                }
+              } else {
+                F::mma(part[2 * j], p, b[0], b[1]);
+                F::mma(part[2 * j + 1], p, b[2], b[3]);
+                if constexpr (EXACT) {
+                  F::mma(low[2 * j], rest, b[0], b[1]);
+                  F::mma(low[2 * j + 1], rest, b[2], b[3]);
+                }
               }
-            } else {
-              F::mma(part[2 * j], p, b[0], b[1]);
-              F::mma(part[2 * j + 1], p, b[2], b[3]);
-              if constexpr (EXACT) {
-                F::mma(low[2 * j], rest, b[0], b[1]);
-                F::mma(low[2 * j + 1], rest, b[2], b[3]);
-              }
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            keep_group(acc, n0, r, shrink[r], part, on[r]);
+            if constexpr (EXACT) keep_group(fine, n0, r, shrink[r], low, on[r]);
+          }
+        }
+      } else {
+        float ds[NT][4];
+        multiply_nk<T, CP, NT, HELD, true>(ds, held_d, d_at, q_rs, v_at + nk, kv_rs);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const Pair z = add2(pair(s[n][2 * r], s[n][2 * r + 1]), both(-top[r]));
+            const float2 x = unpair(fma2(z, both(unit), both(-logsum[r])));
+            Pair p = pair(exp2_fast(x.x), exp2_fast(x.y));
+            if constexpr (sizeof(T) == 2) p = mul2(p, both(lift));
+            p = mul2(p, add2(pair(ds[n][2 * r], ds[n][2 * r + 1]), both(-delta[r])));
+            ds[n][2 * r] = unpair(p).x;
+            ds[n][2 * r + 1] = unpair(p).y;
+          }
+        if constexpr (BIASED) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if (on[r]) {
+              const uint2 b = *reinterpret_cast<const uint2*>(near + r * 8 * kBucketRow);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {  // each thread has a column of its own
+                  const uint32_t at =
+                      hist + __byte_perm(n < 2 ? b.x : b.y, 0, 0x4440 + (n & 1) * 2 + j) * blockDim.x;
+                  const float x = lds_f32(at) + ds[n][2 * r + j];
+                  asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(x) : "memory");
+                }
             }
           }
         }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          keep_group(acc, n0, r, shrink[r], part, on[r]);
-          if constexpr (EXACT) keep_group(fine, n0, r, shrink[r], low, on[r]);
-        }
-      }
-    } else {
-      float ds[NT][4];
-      multiply_nk<T, CP, NT, HELD, true>(ds, held_d, d_at, q_rs, v_at + nk, kv_rs);
+        for (int n0 = 0; n0 < CP / 8; n0 += kChannelGroup) {
+          float part[kChannelGroup][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+          for (int st = 0; st < STEPS; ++st) {
+            typename F::A p;
+            from_acc<T>(p, ds, st);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float2 x = unpair(fma2(pair(s[n][2 * r], s[n][2 * r + 1]), both(unit), both(-lse[r])));
-          Pair p = pair(exp2_fast(x.x), exp2_fast(x.y));
-          if constexpr (sizeof(T) == 2) p = mul2(p, both(lift));
-          p = mul2(p, add2(pair(ds[n][2 * r], ds[n][2 * r + 1]), both(-delta[r])));
-          ds[n][2 * r] = unpair(p).x;
-          ds[n][2 * r + 1] = unpair(p).y;
-        }
-      if constexpr (BIASED) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if (on[r]) {
-            const uint2 b = *reinterpret_cast<const uint2*>(near + r * 8 * kBucketRow);
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {  // each thread has a column of its own
-                const uint32_t at =
-                    hist + __byte_perm(n < 2 ? b.x : b.y, 0, 0x4440 + (n & 1) * 2 + j) * blockDim.x;
-                const float x = lds_f32(at) + ds[n][2 * r + j];
-                asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(x) : "memory");
+            for (int j = 0; j < kChannelGroup / 2; ++j) {
+              typename F::B b;
+              F::pair_kn(b, k_at + kn + st * F::STEP * kv_rs + (n0 + 2 * j) * 8 * SIZE, kv_rs);
+              if (st == 0) {
+                F::mma_first(part[2 * j], p, b[0], b[1]);
+                F::mma_first(part[2 * j + 1], p, b[2], b[3]);
+              } else {
+                F::mma(part[2 * j], p, b[0], b[1]);
+                F::mma(part[2 * j + 1], p, b[2], b[3]);
               }
-          }
-        }
-      }
-#pragma unroll
-      for (int n0 = 0; n0 < CP / 8; n0 += kChannelGroup) {
-        float part[kChannelGroup][4];
-#pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-          typename F::A p;
-          from_acc<T>(p, ds, st);
-#pragma unroll
-          for (int j = 0; j < kChannelGroup / 2; ++j) {
-            typename F::B b;
-            F::pair_kn(b, k_at + kn + st * F::STEP * kv_rs + (n0 + 2 * j) * 8 * SIZE, kv_rs);
-            if (st == 0) {
-              F::mma_first(part[2 * j], p, b[0], b[1]);
-              F::mma_first(part[2 * j + 1], p, b[2], b[3]);
-            } else {
-              F::mma(part[2 * j], p, b[0], b[1]);
-              F::mma(part[2 * j + 1], p, b[2], b[3]);
             }
           }
-        }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) keep_group(acc, n0, r, both(1.0f), part, on[r]);
+          for (int r = 0; r < 2; ++r) keep_group(acc, n0, r, both(1.0f), part, on[r]);
+        }
       }
-    }
     };
     if (left >= kStepLeaves && units.folded) {
       if (bias) work(std::true_type{}, std::true_type{});
@@ -428,7 +434,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
                                    kTileQueries + q;
           float* part = a.part + slot * a.part_row;
           if (t == 0) {
-            part[0] = top[r] * unit;
+            part[0] = top[r];
             part[1] = sum[r];
           }
 #pragma unroll
@@ -457,9 +463,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
             store_pair(exact, n * 8 + 2 * t, a.channels, (unpair(acc[n][r]).x + unpair(fine[n][r]).x) * inv,
                        (unpair(acc[n][r]).y + unpair(fine[n][r]).y) * inv, false);
         }
-        // An empty row keeps +inf: its probabilities come out as 0 in the backward pass.
-        if (a.lse != nullptr && t == 0)
-          a.lse[int64_t(row) * a.heads + span.h0 + head] = sum[r] == 0.0f ? INFINITY : fmaf(top[r], unit, log2f(sum[r]));
+        if (a.stats != nullptr && t == 0) a.stats[int64_t(row) * a.heads + span.h0 + head] = row_stats(top[r], sum[r]);
       }
     } else if (a.grad_q != nullptr) {
       const float back = a.scale / lift;
@@ -500,10 +504,7 @@ cudaError_t run_query_tile(const AttendArgs& a, cudaStream_t stream) {
       query_tile_smem(sizeof(T), CP, a.kv_cta, a.heads_cta, BACK, a.table != nullptr, a.buckets);
   cudaError_t e = allow_smem(k_query_tile<T, CP, BACK, EXACT>, s.total);
   if (e != cudaSuccess) return e;
-  const unsigned groups = a.heads_cta >= a.group
-                              ? unsigned((a.kv_heads + a.kv_cta - 1) / a.kv_cta)
-                              : unsigned(a.kv_heads) * unsigned((a.group + a.heads_cta - 1) / a.heads_cta);
-  const dim3 grid(unsigned(a.map.num_tiles), groups, BACK ? 1 : unsigned(a.splits));
+  const dim3 grid(unsigned(a.map.num_tiles), unsigned(head_groups(a)), BACK ? 1 : unsigned(a.splits));
   k_query_tile<T, CP, BACK, EXACT><<<grid, a.heads_cta * 64, s.total, stream>>>(a);
   return cudaGetLastError();
 }
