@@ -226,6 +226,28 @@ __device__ __forceinline__ uint64_t score_key(float s, uint32_t block) {
   return (uint64_t(__float_as_uint(s)) << 32) | block;
 }
 
+// Inserts x into ascending keys from the top, kInsertGroup slots at a time: below
+// the group where no lane's x belongs nothing moves, and candidates come with
+// ascending bounds, so most belong near the end (16 x 65,536 points, 16 blocks:
+// 1.13 ms for groups of four, 1.12 of two, 1.18 of eight, 1.29 for all 16; 32
+// blocks of 4 x 65,536: 605, 643, 628 and 796 us).
+constexpr int kInsertGroup = 4;
+
+template <int CAP, int HI>
+__device__ __forceinline__ void insert_key(uint64_t (&key)[CAP], uint64_t x) {
+  constexpr int LO = HI > kInsertGroup ? HI - kInsertGroup : 0;
+#pragma unroll
+  for (int i = HI - 1; i > LO; --i) key[i] = x < key[i - 1] ? key[i - 1] : (x < key[i] ? x : key[i]);
+  if constexpr (LO == 0) {
+    key[0] = x < key[0] ? x : key[0];
+  } else if (x < key[LO - 1]) {
+    key[LO] = key[LO - 1];
+    insert_key<CAP, LO>(key, x);
+  } else {
+    key[LO] = x < key[LO] ? x : key[LO];
+  }
+}
+
 // One warp a tile. The warp walks the tree as a packet, two levels a step: the
 // (up to four) grandchildren of a node are scored by every lane, those that some
 // lane admits are pushed, the one nearest to most lanes last. A popped node is
@@ -300,9 +322,7 @@ __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
 
   auto insert = [&](uint64_t x) {
     if (x < bound) {
-#pragma unroll
-      for (int i = CAP - 1; i > 0; --i) key[i] = x < key[i - 1] ? key[i - 1] : (x < key[i] ? x : key[i]);
-      key[0] = x < key[0] ? x : key[0];
+      insert_key<CAP, CAP>(key, x);
       bound = key[CAP - 1];
     }
   };
@@ -585,6 +605,9 @@ __global__ void __launch_bounds__(kOrderThreads) k_block_order(BlockMap map, Blo
   if (count <= kOrderShort) {
     for (int i = tid; i < count; i += kOrderThreads) s_entry[i] = in[i];
     __syncthreads();
+    // Through shared memory where the list fits: whole lines to memory instead of words.
+    const int64_t queries = plan.query_begin[block + 1] - plan.query_begin[block];
+    const bool fits = queries <= kOrderWords;
     for (int i = tid; i < count; i += kOrderThreads) {
       const uint2 mine = s_entry[i];
       int before = 0;
@@ -592,8 +615,11 @@ __global__ void __launch_bounds__(kOrderThreads) k_block_order(BlockMap map, Blo
         const uint2 e = s_entry[k];
         before += e.x < mine.x ? __popc(e.y) : 0;
       }
-      write_slots(out + before, mine.x, mine.y);
+      write_slots((fits ? s_bits : out) + before, mine.x, mine.y);
     }
+    if (!fits) return;
+    __syncthreads();
+    for (int i = tid; i < queries; i += kOrderThreads) out[i] = s_bits[i];
     return;
   }
   const BlockCloud c = map.of_block(block);
