@@ -146,6 +146,7 @@ struct Frag16 {
 
 template <>
 struct Frag<__nv_bfloat16> : Frag16<__nv_bfloat16> {
+  static constexpr int PARTS = 3;  // that hold a float32
   // Probabilities and their gradients enter the second products in 16 bits: a
   // relative half step of 2^-8 each, the same as the values they multiply.
   __device__ static __forceinline__ uint32_t pack(float x, float y) {
@@ -175,6 +176,7 @@ struct Frag<__nv_bfloat16> : Frag16<__nv_bfloat16> {
 
 template <>
 struct Frag<__half> : Frag16<__half> {
+  static constexpr int PARTS = 2;  // that hold a float32 of [0, 1] to 2^-22 or 2^-25
   // As above with 2^-11; the backward pass scales by a power of two so that
   // small gradients stay normal numbers.
   __device__ static __forceinline__ uint32_t pack(float x, float y) {
@@ -287,16 +289,23 @@ __device__ __forceinline__ void from_acc(typename Frag<T>::A& a, const float (&a
   }
 }
 
-// What from_acc's 16-bit rounding leaves of the same elements, as an A operand.
+// What from_acc's 16-bit rounding leaves of the same elements, as A operands: in one
+// part (float16: 2^-22 of them is left), and for bfloat16 in another (2^-24; one part
+// would leave 2^-16).
 template <typename T, int N>
-__device__ __forceinline__ void rest_of_acc(typename Frag<T>::A& rest, const typename Frag<T>::A& a,
-                                            const float (&acc)[N][4], int s) {
+__device__ __forceinline__ void rest_of_acc(typename Frag<T>::A& rest, typename Frag<T>::A& last,
+                                            const typename Frag<T>::A& a, const float (&acc)[N][4], int s) {
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 near = Frag<T>::unpack(a[i]);
       const float* x = acc[2 * s + (i >> 1)] + 2 * (i & 1);
-      rest[i] = Frag<T>::pack(x[0] - near.x, x[1] - near.y);
+      const float left[2] = {x[0] - near.x, x[1] - near.y};
+      rest[i] = Frag<T>::pack(left[0], left[1]);
+      if constexpr (Frag<T>::PARTS == 3) {
+        const float2 second = Frag<T>::unpack(rest[i]);
+        last[i] = Frag<T>::pack(left[0] - second.x, left[1] - second.y);
+      }
     }
   }
 }
@@ -329,7 +338,18 @@ __device__ __forceinline__ void multiply_nk(float (&acc)[NT][4], const typename 
     for (int j = 0; j < NT / 2; ++j) {
       typename Frag<T>::B y;
       Frag<T>::pair_nk(y, b + j * 16 * b_rs + depth, b_rs);
-      if (FRESH && s == 0) {
+      if constexpr (sizeof(T) == 4) {
+        // The matrix pipe truncates as it adds, all to one side: each depth step is summed by
+        // itself and added with rounding.
+        float part[2][4];
+        Frag<T>::mma_first(part[0], x, y[0], y[1]);
+        Frag<T>::mma_first(part[1], x, y[2], y[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[2 * j][i] = FRESH && s == 0 ? part[0][i] : acc[2 * j][i] + part[0][i];
+          acc[2 * j + 1][i] = FRESH && s == 0 ? part[1][i] : acc[2 * j + 1][i] + part[1][i];
+        }
+      } else if (FRESH && s == 0) {
         Frag<T>::mma_first(acc[2 * j], x, y[0], y[1]);
         Frag<T>::mma_first(acc[2 * j + 1], x, y[2], y[3]);
       } else {

@@ -17,9 +17,9 @@
 //              dQ = scale sum dS K;  dT[h][bucket] += dS
 //
 // EXACT (forward, 16-bit features whose bias table trains): the parts of the
-// probabilities that 16 bits do not hold go through a second product of their
-// own, kept apart, so that the output's bits do not depend on it; both sums
-// together are the float32 output that <dO, O> is taken from.
+// probabilities that 16 bits do not hold go through products of their own, kept
+// apart, so that the output's bits do not depend on them; both sums together are
+// the float32 output that <dO, O> is taken from.
 //
 // A row that did not select the entry keeps its sums by selection, not by
 // masking its scores: what it computes there is dropped, so non-finite keys and
@@ -325,9 +325,9 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
 #pragma unroll
           for (int st = 0; st < STEPS; ++st) {
             typename F::A p;
-            [[maybe_unused]] typename F::A rest;
+            [[maybe_unused]] typename F::A rest, last;
             from_acc<T>(p, s, st);
-            if constexpr (EXACT) rest_of_acc<T>(rest, p, s, st);
+            if constexpr (EXACT) rest_of_acc<T>(rest, last, p, s, st);
 #pragma unroll
             for (int j = 0; j < kChannelGroup / 2; ++j) {
               typename F::B b;
@@ -338,6 +338,10 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
                 if constexpr (EXACT) {
                   F::mma_first(low[2 * j], rest, b[0], b[1]);
                   F::mma_first(low[2 * j + 1], rest, b[2], b[3]);
+                  if constexpr (F::PARTS == 3) {
+                    F::mma(low[2 * j], last, b[0], b[1]);
+                    F::mma(low[2 * j + 1], last, b[2], b[3]);
+                  }
                 }
               } else {
                 F::mma(part[2 * j], p, b[0], b[1]);
@@ -345,6 +349,10 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
                 if constexpr (EXACT) {
                   F::mma(low[2 * j], rest, b[0], b[1]);
                   F::mma(low[2 * j + 1], rest, b[2], b[3]);
+                  if constexpr (F::PARTS == 3) {
+                    F::mma(low[2 * j], last, b[0], b[1]);
+                    F::mma(low[2 * j + 1], last, b[2], b[3]);
+                  }
                 }
               }
             }
