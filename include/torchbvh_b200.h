@@ -285,6 +285,8 @@ int tbvh_widen_indices(int device, const int32_t* src, int64_t* dst, int64_t cou
  * of those blocks, with an optional learned bias by distance bucket.
  */
 
+enum { TBVH_SMALL_QUERIES = 16384 };
+
 /* Geometry of a selection. points_per_cloud > 0: num_clouds clouds of that
  * size with queries_per_cloud queries each, tables NULL. Else ragged: the
  * table of tbvh_block_table, on the host and on the device. */
@@ -301,7 +303,9 @@ typedef struct tbvh_block_geometry {
   const float* node_aabbs;        /* of tbvh_build */
   const int64_t* sorted_indices;  /* of tbvh_build */
   const float* query_points;      /* [total_queries][dim]; read by tbvh_select_blocks only */
-  const int64_t* order;           /* of tbvh_sort_queries; NULL: the given order; read by the same only */
+  const int64_t* order;           /* of tbvh_sort_queries; read by the same only. NULL: clouds of at most
+                                   * TBVH_SMALL_QUERIES queries each are put in order by the call, larger
+                                   * ones keep the given order */
   void* plan;                     /* tbvh_block_plan_size() bytes, kept with the selection */
   size_t plan_bytes;
 } tbvh_block_geometry;

@@ -82,6 +82,32 @@ def test_selection_matches_the_definition(name, n):
     assert torchbvh.device_status() == 0
 
 
+@pytest.mark.parametrize("queries, dim", [
+    ([33], 2), ([1024], 3), ([1025], 2), ([4096], 3), ([4097], 2), ([8193], 3), ([12289], 2), ([16384], 3), ([16385], 3),
+    ([16384, 2, 5, 40], 3), ([1, 16385, 33], 2),
+])
+def test_queries_of_every_order_are_all_served(queries, dim):
+    scene = Scene("ragged" if len(queries) > 1 else "single", [900] * len(queries), queries, dim, seed=16)
+    for q in scene.qpts:  # some beyond the cloud's box, some equal, one not a number
+        q[::3] = q[::3] * 4 - 2
+        q[1::7] = q[:1]
+    scene.qpts[0][len(scene.qpts[0]) // 2, 0] = np.nan
+    got = scene.select(3)
+    blocks = scene.split(got["block_indices"], scene.queries)
+    for b, order in enumerate(scene.orders):
+        want, _ = oracle.select(scene.points[b], order, scene.qpts[b], 3)
+        assert np.array_equal(blocks[b].cpu().numpy(), want)
+    # Every query has one place in the plan: all rows of an attention are written.
+    q = scene.tensor([np.zeros((m, 1, 8), np.float32) for m in queries])
+    k = scene.tensor([np.ones((900, 1, 8), np.float32)] * len(queries))
+    out = torchbvh.attend_blocks(got, q, k, k)
+    empty = (got["block_indices"] < 0).all(-1)
+    assert int(empty.sum()) == 1
+    # A mean of ones: 1 but for the sums' roundings, of at most 192 terms.
+    assert bool(((out - (~empty)[..., None, None].float()).abs() <= 192 * 2.0**-23).all())
+    assert torchbvh.device_status() == 0
+
+
 @pytest.mark.parametrize("kind", ["same", "clusters"])
 def test_selection_ties_go_to_the_lowest_block(kind):
     scene = Scene("single", [5000], [100], 3, kind=kind)

@@ -52,7 +52,7 @@ from ._validation import (
 
 __all__ = ["BlockSelection", "select_blocks", "attend_blocks", "distance_bias"]
 
-_TILE = 32  # queries of one tile: within one tile the query order does not matter
+_SMALL = 16384  # queries of one cloud up to which the selection puts them in order itself
 
 
 class BlockSelection(_Handle):
@@ -141,8 +141,10 @@ def select_blocks(bvh: BVHHandle | BatchedBVHHandle | RaggedBVHHandle, query_poi
         table_dev = torch.tensor(list(table), dtype=torch.int64, device=device)
         geometry.num_clouds, geometry.table_host, geometry.table_dev = (
             len(host) - 1, ctypes.cast(table, ctypes.c_void_p), table_dev.data_ptr())
-        order = _C.morton_sort_queries_ragged(queries, query_offsets, int(queries.size(0)), tree["scene_min"],
-                                              tree["scene_max"])
+        order = None
+        if max(b - a for a, b in zip(host, host[1:])) > _SMALL:
+            order = _C.morton_sort_queries_ragged(queries, query_offsets, int(queries.size(0)), tree["scene_min"],
+                                                  tree["scene_max"])
         keep = (table, table_dev)
         key_shape = (tree["point_offsets"][-1],)
     else:
@@ -158,7 +160,7 @@ def select_blocks(bvh: BVHHandle | BatchedBVHHandle | RaggedBVHHandle, query_poi
         geometry.num_clouds, geometry.points_per_cloud, geometry.queries_per_cloud = (
             clouds, tree["num_leaves"], per_cloud)
         order = None
-        if per_cloud > _TILE:
+        if per_cloud > _SMALL:
             lift = (lambda t: t) if batched else (lambda t: t.unsqueeze(0))
             order = _C.morton_sort_queries_narrow(lift(queries), lift(tree["scene_min"]), lift(tree["scene_max"]))
         keep = ()

@@ -45,6 +45,7 @@ struct BlockMap {
   __device__ __forceinline__ BlockCloud uniform(int64_t b) const {
     return BlockCloud{b * n, n, b * rows, b * m, m, b * tiles_of(m), b * blocks_of(n)};
   }
+  __device__ __forceinline__ BlockCloud of_cloud(int64_t b) const { return table == nullptr ? uniform(b) : table[b]; }
   __device__ __forceinline__ BlockCloud of_tile(int64_t t) const {
     if (table == nullptr) return uniform(num_clouds == 1 ? 0 : t / tiles_of(m));
     int lo = 0, hi = num_clouds - 1;
@@ -84,7 +85,7 @@ struct BlockPlan {
 struct BlockSetup {
   BlockMap map;
   BlockPlan plan;
-  int64_t total_points, total_queries;
+  int64_t total_points, total_queries, most_queries;  // most: of one cloud
 };
 
 // Checks the sizes and fills everything of `s` but the pointers.
