@@ -651,13 +651,18 @@ __global__ void __launch_bounds__(1024) k_block_begin(BlockPlan plan, int64_t bl
   int64_t carry = 0;
   for (int64_t at = 0; at < blocks; at += 8 * 1024) {
     int64_t sum = 0;
-    int v[8];
+    int v[8] = {};
+    const int64_t mine = at + tid * 8;
+    const bool full = mine + 8 <= blocks;
+    if (full) {
+      *reinterpret_cast<int4*>(v) = *reinterpret_cast<const int4*>(counts + mine);
+      *reinterpret_cast<int4*>(v + 4) = *reinterpret_cast<const int4*>(counts + mine + 4);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t j = at + tid * 8 + i;
-      v[i] = j < blocks ? counts[j] : 0;
-      sum += v[i];
+      for (int i = 0; i < 8; ++i) v[i] = mine + i < blocks ? counts[mine + i] : 0;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += v[i];
     int64_t x = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -673,14 +678,23 @@ __global__ void __launch_bounds__(1024) k_block_begin(BlockPlan plan, int64_t bl
       total += s_warp[w];
     }
     before += x - sum;
+    if (full) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t j = at + tid * 8 + i;
-      if (j < blocks) {
-        begin[j] = before;
-        if (blockIdx.x == 0) counts[j] = 0;
+      for (int i = 0; i < 8; i += 2) {
+        *reinterpret_cast<longlong2*>(begin + mine + i) = make_longlong2(before, before + v[i]);
+        before += v[i] + v[i + 1];
       }
-      before += v[i];
+      if (blockIdx.x == 0)
+        for (int i = 0; i < 8; i += 4) *reinterpret_cast<int4*>(counts + mine + i) = make_int4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (mine + i < blocks) {
+          begin[mine + i] = before;
+          if (blockIdx.x == 0) counts[mine + i] = 0;
+        }
+        before += v[i];
+      }
     }
     carry += total;
     __syncthreads();
