@@ -3,12 +3,13 @@
 //
 // Products run on warp-level matrix instructions (mma.sync m16n8) with
 // accumulators in registers. Every score costs more than its products: mask,
-// bucket lookup, bias, exponential, rounding. At 32 channels a score is 128
-// multiply-adds' worth of flops in the matrix pipe, one exponential (16 a clock
-// an SM) and about a dozen other instructions (128 a clock an SM), so the issue
-// slots bound these kernels, not the matrix pipe; and a 16-row instruction lets
-// a warp skip a block that none of its 16 queries selected, which a 128-row
-// tensor-memory tile could not.
+// bucket lookup, bias, exponential, rounding. With 32 channels and a bias the
+// forward pass issues 44 thread instructions a selected score (184 M warp
+// instructions for 134 M scores), 64 multiply-adds of which would take a
+// tensor-memory instruction a twentieth of that time: the issue slots bound these
+// kernels, not the matrix pipe (14 % busy). And a 16-row instruction lets a warp
+// skip a block that none of its 16 queries selected, which a 128-row tile in tensor
+// memory could not.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -378,7 +378,10 @@ __device__ __forceinline__ void insert_key(uint64_t (&key)[CAP], uint64_t x) {
 // queries, a lower bound for all of them; the boxes go to shared memory in
 // ascending order of that bound, so that near blocks enter the lists first, few
 // are displaced again, and the scan ends at the first block no query can want.
-// Bound by issue: an insertion shifts a list of 64-bit keys in registers.
+// Bound by issue: an insertion shifts a list of 64-bit keys in registers (16 x
+// 65,536 queries, 16 blocks: 0.85 of the 1.05 ms of the call with its lists, issue
+// slots 73 % and the integer pipe 64 % busy, DRAM 3 %). One block at a time instead of
+// bunches in order took 1.2 times as long.
 template <int D, int CAP>
 __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
   __shared__ uint32_t s_stack[kSelectStack];
