@@ -108,6 +108,23 @@ def test_queries_of_every_order_are_all_served(queries, dim):
     assert torchbvh.device_status() == 0
 
 
+@pytest.mark.parametrize("n", [1, 4, 7, 16, 31])
+@pytest.mark.parametrize("points, queries, kind", [
+    (1025, 1, "uniform"), (1089, 40, "same"), (20000, 300, "clusters"), (5000, 18943, "uniform"), (5000, 18945, "uniform"),
+])
+def test_selection_by_several_warps_or_one(points, queries, kind, n):
+    # 592 tiles of 32 queries, and clouds of 16 blocks, are where a tile's warps change.
+    scene = Scene("single", [points], [queries], 3, seed=17, kind=kind)
+    some = scene.qpts[0][::5]
+    some[:] = scene.points[0][np.arange(len(some)) % points]  # on the points: many scores of 0
+    scene.qpts[0][-1] = np.inf
+    got = scene.select(n)
+    want_b, want_d = oracle.select(scene.points[0], scene.orders[0], scene.qpts[0], n)
+    assert np.array_equal(got["block_indices"].cpu().numpy(), want_b)
+    assert np.array_equal(got["squared_distances"].cpu().numpy().view(np.int32), want_d.view(np.int32))
+    assert torchbvh.device_status() == 0
+
+
 @pytest.mark.parametrize("kind", ["same", "clusters"])
 def test_selection_ties_go_to_the_lowest_block(kind):
     scene = Scene("single", [5000], [100], 3, kind=kind)

@@ -85,7 +85,7 @@ struct BlockPlan {
 struct BlockSetup {
   BlockMap map;
   BlockPlan plan;
-  int64_t total_points, total_queries, most_queries;  // most: of one cloud
+  int64_t total_points, total_queries, most_queries, most_blocks;  // most: of one cloud
 };
 
 // Checks the sizes and fills everything of `s` but the pointers.

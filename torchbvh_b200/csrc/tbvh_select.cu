@@ -14,6 +14,7 @@
 #include <climits>
 #include <cstdarg>
 #include <cstdio>
+#include <type_traits>
 
 #include "tbvh_blocks.h"
 #include "tbvh_kernels.h"
@@ -119,6 +120,7 @@ int measure_blocks(const char* op, const tbvh_block_geometry* g, BlockSetup& s) 
     s.total_queries = want.q0;
   }
   s.most_queries = most_queries;
+  s.most_blocks = most_blocks;
   s.plan.capacity = (most_queries < kTileQueries ? most_queries : kTileQueries) * g->num_blocks;
   if (s.plan.capacity > most_blocks) s.plan.capacity = most_blocks;
   return TBVH_OK;
@@ -370,7 +372,33 @@ __device__ __forceinline__ void insert_key(uint64_t (&key)[CAP], uint64_t x) {
   }
 }
 
-// One warp a tile. The warp walks the tree as a packet, two levels a step: the
+// Ascending: the lowest CAP of this lane's keys and of `other`, both ascending.
+template <int CAP>
+__device__ __forceinline__ void merge_keys(uint64_t (&key)[CAP], const uint64_t* other) {
+#pragma unroll
+  for (int i = 0; i < CAP; ++i) {  // the lower of each pair from opposite ends: a bitonic sequence
+    const uint64_t x = other[CAP - 1 - i];
+    key[i] = x < key[i] ? x : key[i];
+  }
+#pragma unroll
+  for (int d = CAP / 2; d > 0; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < CAP; ++i)
+      if ((i & d) == 0) {
+        const uint64_t a = key[i], b = key[i + d];
+        key[i] = a < b ? a : b;
+        key[i + d] = a < b ? b : a;
+      }
+}
+
+// WARPS warps a tile: one where tiles fill the GPU, four where they do not and the
+// time is one warp's. Each then takes every fourth bunch of the tree (below) into
+// lists of its own, which are merged at the end; all prune by the least of a query's
+// k-th keys, which the k-th best of all cannot exceed. Whole calls of 8 (32) blocks,
+// one warp / four: 22 tiles 168 / 101 us (353 / 208), 313 tiles 75 / 62 (118 / 111),
+// 512 tiles 91 / 81 (152 / 148), 1,024 tiles 98 / 91 (173 / 236).
+//
+// A warp walks the tree as a packet, two levels a step: the
 // (up to four) grandchildren of a node are scored by every lane, those that some
 // lane admits are pushed, the one nearest to most lanes last. A popped node is
 // scored again against the meanwhile lower k-th keys. At a bunch each of 16
@@ -382,14 +410,18 @@ __device__ __forceinline__ void insert_key(uint64_t (&key)[CAP], uint64_t x) {
 // 65,536 queries, 16 blocks: 0.85 of the 1.05 ms of the call with its lists, issue
 // slots 73 % and the integer pipe 64 % busy, DRAM 3 %). One block at a time instead of
 // bunches in order took 1.2 times as long.
-template <int D, int CAP>
-__global__ void __launch_bounds__(32) k_select(SelectArgs a) {
-  __shared__ uint32_t s_stack[kSelectStack];
-  __shared__ int64_t s_row[32];
-  __shared__ uint64_t s_keys[32 * CAP];
+template <int D, int CAP, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) k_select(SelectArgs a) {
+  __shared__ uint32_t s_stacks[WARPS][kSelectStack];
+  __shared__ int64_t s_rows[WARPS][32];
+  __shared__ uint64_t s_keys[WARPS * 32 * CAP];
   __shared__ int64_t s_query[32];
-  __shared__ float4 s_lo[kBunch], s_hi[kBunch];  // w: lower bound, block
-  const int lane = threadIdx.x;
+  __shared__ float4 s_los[WARPS][kBunch], s_his[WARPS][kBunch];  // w: lower bound, block
+  __shared__ unsigned long long s_bound[32];                     // WARPS > 1: least k-th key of each query
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t* s_stack = s_stacks[warp];
+  int64_t* s_row = s_rows[warp];
+  float4 *s_lo = s_los[warp], *s_hi = s_his[warp];
   const int64_t tile = blockIdx.x;
   const BlockCloud c = a.map.of_tile(tile);
   const int64_t pos = (tile - c.t0) * kTileQueries + lane;
@@ -421,8 +453,11 @@ __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
       query = c.q0 + local;
     }
   }
-  s_query[lane] = query;
-  a.plan.query_row[tile * kTileQueries + lane] = int(query);
+  if constexpr (WARPS > 1) __syncthreads();  // all have read the row
+  if (warp == 0) {
+    s_query[lane] = query;
+    a.plan.query_row[tile * kTileQueries + lane] = int(query);
+  }
   float q[D];
   bool searching = active;
 #pragma unroll
@@ -432,7 +467,7 @@ __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
   }
 #pragma unroll
   for (int x = 0; x < 3; ++x)
-    a.plan.query_point[(tile * 3 + x) * kTileQueries + lane] = x < D ? q[x < D ? x : 0] : 0.0f;
+    if (warp == 0) a.plan.query_point[(tile * 3 + x) * kTileQueries + lane] = x < D ? q[x < D ? x : 0] : 0.0f;
   // Ascending keys; the first CAP - num slots hold 0 and stay, so the last slot
   // is the num-th best. Admission: key < last slot.
   const uint64_t empty = uint64_t(__float_as_uint(kFar)) << 32;
@@ -445,12 +480,16 @@ __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
   }
   // A lane that does not search admits nothing: its bound is 0.
   uint64_t bound = searching ? empty : 0;
+  if constexpr (WARPS > 1) {
+    if (warp == 0) s_bound[lane] = bound;
+    __syncthreads();
+  }
   __syncwarp();
 
   auto insert = [&](uint64_t x) {
     if (x < bound) {
       insert_key<CAP, CAP>(key, x);
-      bound = key[CAP - 1];
+      bound = key[CAP - 1] < bound ? key[CAP - 1] : bound;
     }
   };
 
@@ -501,6 +540,10 @@ __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
       s_hi[place] = make_float4(box.hi[0], box.hi[1], D == 3 ? box.hi[D - 1] : 0.0f, __uint_as_float(base + lane));
     }
     __syncwarp();
+    if constexpr (WARPS > 1) {  // the other warps' progress
+      const uint64_t shared = *static_cast<volatile unsigned long long*>(s_bound + lane);
+      bound = shared < bound ? shared : bound;
+    }
     float reach = worst();
     for (int k = 0; k < blocks; ++k) {
       const float4 lo = s_lo[k], hi = s_hi[k];
@@ -514,11 +557,12 @@ __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
         reach = worst();
       }
     }
+    if constexpr (WARPS > 1) atomicMin(s_bound + lane, static_cast<unsigned long long>(bound));
   };
 
   int depth = 0;
   if (bunch_level == 0) {
-    scan_bunch(0);
+    if (warp == 0) scan_bunch(0);
   } else {
     if (lane == 0) s_stack[0] = 0;
     depth = 1;
@@ -555,7 +599,8 @@ __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
     unsigned admitted = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const bool ok = k < children && score_key(score[k], (base + k) << (last - child_level)) < bound;
+      const bool here = WARPS == 1 || child_level < bunch_level || int(base + k) % WARPS == warp;
+      const bool ok = here && k < children && score_key(score[k], (base + k) << (last - child_level)) < bound;
       if (__any_sync(kFullMask, ok)) admitted |= 1u << k;
       if (ok && score[k] < least) {
         least = score[k];
@@ -588,10 +633,31 @@ __global__ void __launch_bounds__(32) k_select(SelectArgs a) {
     __syncwarp();
   }
 
-  // Rows of the result, written a row at a time: slot s of lane r by lane s.
+  uint64_t* own = s_keys + threadIdx.x * CAP;
 #pragma unroll
-  for (int i = 0; i < CAP; ++i) s_keys[lane * CAP + i] = key[i];
+  for (int i = 0; i < CAP; ++i) own[i] = key[i];
+  if constexpr (WARPS > 1) {
+    // The slots in use to the front: lists that ascend throughout. Then warp w takes in
+    // the lists of warp w + 1, and so on by doubles.
+#pragma unroll
+    for (int i = 0; i < CAP; ++i) key[i] = i < a.num ? own[CAP - a.num + i] : ~uint64_t(0);
+#pragma unroll
+    for (int d = 1; d < WARPS; d *= 2) {
+#pragma unroll
+      for (int i = 0; i < CAP; ++i) own[i] = key[i];
+      __syncthreads();
+      if (warp % (2 * d) == 0) merge_keys(key, own + d * 32 * CAP);
+      __syncthreads();
+    }
+    if (warp != 0) return;
+#pragma unroll
+    for (int i = 0; i < CAP; ++i)
+      if (i < a.num) own[CAP - a.num + i] = key[i];
+#pragma unroll
+    for (int i = 0; i < CAP; ++i) key[i] = i < CAP - a.num ? 0 : own[i];
+  }
   __syncwarp();
+  // Rows of the result, written a row at a time: slot s of lane r by lane s.
   {
     int r = lane / a.num, slot = lane % a.num;
     const int dr = 32 / a.num, ds = 32 % a.num;
@@ -803,6 +869,8 @@ __global__ void __launch_bounds__(kOrderThreads) k_block_order(BlockMap map, Blo
   }
 }
 
+constexpr int64_t kFewTiles = 4 * 148;  // below four tiles an SM a tile has four warps
+
 template <int D, int ITEMS>
 cudaError_t launch_order(const SelectArgs& a, cudaStream_t stream) {
   constexpr size_t smem = order_queries_smem(ITEMS);
@@ -818,7 +886,7 @@ cudaError_t launch_order(const SelectArgs& a, cudaStream_t stream) {
 }
 
 template <int D>
-cudaError_t launch_select(SelectArgs a, int64_t most_queries, cudaStream_t stream) {
+cudaError_t launch_select(SelectArgs a, int64_t most_queries, int64_t most_blocks, cudaStream_t stream) {
   a.ordered = a.order == nullptr && most_queries > kTileQueries && most_queries <= kSmallQueries;
   if (a.ordered) {
     const int items = int((most_queries + kOrderQueriesThreads - 1) / kOrderQueriesThreads);
@@ -830,10 +898,16 @@ cudaError_t launch_select(SelectArgs a, int64_t most_queries, cudaStream_t strea
     if (e != cudaSuccess) return e;
   }
   const unsigned grid = unsigned(a.map.num_tiles);
-  if (a.num <= 4) k_select<D, 4><<<grid, 32, 0, stream>>>(a);
-  else if (a.num <= 8) k_select<D, 8><<<grid, 32, 0, stream>>>(a);
-  else if (a.num <= 16) k_select<D, 16><<<grid, 32, 0, stream>>>(a);
-  else k_select<D, 32><<<grid, 32, 0, stream>>>(a);
+  const bool few = a.map.num_tiles < kFewTiles && most_blocks > kBunch;
+  auto go = [&](auto cap) {
+    constexpr int CAP = decltype(cap)::value;
+    if (few) k_select<D, CAP, 4><<<grid, 128, 0, stream>>>(a);
+    else k_select<D, CAP, 1><<<grid, 32, 0, stream>>>(a);
+  };
+  if (a.num <= 4) go(std::integral_constant<int, 4>{});
+  else if (a.num <= 8) go(std::integral_constant<int, 8>{});
+  else if (a.num <= 16) go(std::integral_constant<int, 16>{});
+  else go(std::integral_constant<int, 32>{});
   count_launches(1);
   return cudaGetLastError();
 }
@@ -897,7 +971,8 @@ int tbvh_select_blocks(const tbvh_block_geometry* g, int64_t* out_blocks, float*
     a.out_dist = out_distances;
     a.num = g->num_blocks;
     a.status = device_status_ptr();
-    e = g->dim == 3 ? launch_select<3>(a, s.most_queries, st) : launch_select<2>(a, s.most_queries, st);
+    e = g->dim == 3 ? launch_select<3>(a, s.most_queries, s.most_blocks, st)
+                    : launch_select<2>(a, s.most_queries, s.most_blocks, st);
   }
   if (e == cudaSuccess && s.plan.entry_count) {
     k_block_begin<<<2, 1024, 0, st>>>(s.plan, s.map.num_blocks);
