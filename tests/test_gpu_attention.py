@@ -343,6 +343,22 @@ def test_half_gradients_of_large_values_stay_in_range():
     _check(scene, selection, f, _run(scene, selection, f))
 
 
+@pytest.mark.parametrize("grad", [2.0**-14, 1.0, 2.0**8])
+def test_half_gradients_beside_an_outlying_value(grad):
+    # A value that no query sees leaves room for the gradients of the others: 2 * 32 * 4 * 2^10
+    # of it are lifted to 2^15, a typical dS of 6 / 256 then to 2^-9, four powers of two above
+    # float16's subnormal numbers, whose half step is 2^-4.5 of the rounding that is counted.
+    scene = Scene("single", [2000], [64], 3, seed=18)
+    scene.qpts[0] *= 0.1
+    selection = scene.select(4)
+    f = _features(scene, F16, 2, 2, 32, 5, seed=18)
+    seen = set(selection["block_indices"].unique().tolist())
+    hidden = next(j for j in range(31) if j not in seen)
+    f["v"][0][scene.orders[0][64 * hidden]] = 1024.0
+    f["grad"][0] = (f["grad"][0].float() * grad).to(F16)
+    _check(scene, selection, f, _run(scene, selection, f))
+
+
 def test_half_gradients_without_queries():
     scene = Scene("single", [100], [0], 3, seed=13)
     selection = scene.select(4)

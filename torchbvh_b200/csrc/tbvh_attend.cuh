@@ -702,14 +702,14 @@ __host__ __device__ inline int head_groups(const AttendArgs& a) {
                                 : a.kv_heads * ((a.group + a.heads_cta - 1) / a.heads_cta);
 }
 
-// float16: the power of two that brings the product of the largest |grad_out| and
-// |value| to [1, 2), so that dS, at most 2 * 2 * 128 of it, stays in float16's range
-// and its small numbers stay normal; taken out again at the end.
+// float16: the power of two that brings the most that |dS| can be, 2 * channels times
+// the largest |grad_out| and |value|, to [2^14, 2^15): it stays in float16's range, and
+// as many of its small numbers as can be stay normal. Taken out again at the end.
 template <typename T>
 __device__ __forceinline__ float gradient_lift(const AttendArgs& a) {
   if (a.largest == nullptr) return 1.0f;
-  const float most = __uint_as_float(a.largest[0]) * __uint_as_float(a.largest[1]);
-  return most > 0.0f ? exp2f(-floorf(log2f(most))) : 1.0f;
+  const float most = 2.0f * float(a.channels) * __uint_as_float(a.largest[0]) * __uint_as_float(a.largest[1]);
+  return most > 0.0f ? exp2f(14.0f - floorf(log2f(most))) : 1.0f;
 }
 
 // What the backward pass keeps of a row's softmax: the largest logit, in units of
