@@ -306,7 +306,7 @@ typedef struct tbvh_block_geometry {
   const int64_t* order;           /* of tbvh_sort_queries; read by the same only. NULL: clouds of at most
                                    * TBVH_SMALL_QUERIES queries each are put in order by the call, larger
                                    * ones keep the given order */
-  void* plan;                     /* tbvh_block_plan_size() bytes, kept with the selection */
+  void* plan;                     /* tbvh_block_plan_size() bytes on a multiple of 16, kept with the selection */
   size_t plan_bytes;
 } tbvh_block_geometry;
 

@@ -270,6 +270,43 @@ def test_attend_entries_reject(native_lib, change, text):
         assert rc == _native.TBVH_ERR_BAD_ARG and text in native_lib.tbvh_last_error().decode()
 
 
+@pytest.mark.parametrize("change, text", [
+    ({"scale": float("nan")}, "scale must be finite"),
+    ({"scale": float("inf")}, "scale must be finite"),
+    ({"queries": 18}, "not aligned to its type"),
+    ({"keys": 18}, "not aligned to its type"),
+    ({"values": 17, "dtype": 2}, "not aligned to its type"),
+    ({"bias_table": 18, "bias_edges": 16, "num_buckets": 4}, "not aligned to its type"),
+])
+def test_attend_entries_reject_scales_and_misaligned_features(native_lib, change, text):
+    g, f = _geometry(), _features(**change)
+    for rc in (native_lib.tbvh_attend_blocks(ctypes.byref(g), ctypes.byref(f), 16, None, None, None, 0, None),
+               native_lib.tbvh_attend_blocks_backward(ctypes.byref(g), ctypes.byref(f), 16, None, 16, 16, 16, None, None,
+                                                      None, 16, 2**40, None)):
+        assert rc == _native.TBVH_ERR_BAD_ARG and text in native_lib.tbvh_last_error().decode()
+
+
+@pytest.mark.parametrize("out, stats, exact", [(18, 16, None), (16, 20, None), (16, 16, 18)])
+def test_attend_entry_rejects_misaligned_outputs(native_lib, out, stats, exact):
+    g = _geometry(node_aabbs=16, sorted_indices=16, plan=256, plan_bytes=2**40)
+    f = _features(dtype=0 if exact is None else 1)
+    rc = native_lib.tbvh_attend_blocks(ctypes.byref(g), ctypes.byref(f), out, stats, exact, 16, 2**40, None)
+    assert rc == _native.TBVH_ERR_BAD_ARG and "not aligned to its type" in native_lib.tbvh_last_error().decode()
+    g.plan = 264
+    rc = native_lib.tbvh_attend_blocks(ctypes.byref(g), ctypes.byref(f), 16, 16, None, 16, 2**40, None)
+    assert rc == _native.TBVH_ERR_BAD_ARG and "multiple of 16 bytes" in native_lib.tbvh_last_error().decode()
+
+
+@pytest.mark.parametrize("at", range(7))
+def test_backward_entry_rejects_misaligned_pointers(native_lib, at):
+    g = _geometry(node_aabbs=16, sorted_indices=16, plan=256, plan_bytes=2**40, backward=1)
+    f = _features(num_buckets=4, bias_table=16, bias_edges=16)
+    pointers = [16, 16, 16, 16, 16, 16, 16, 16]  # out, out_exact, stats, grad_out, grad of q, k, v, table
+    pointers[at] = 18
+    rc = native_lib.tbvh_attend_blocks_backward(ctypes.byref(g), ctypes.byref(f), *pointers, 16, 2**40, None)
+    assert rc == _native.TBVH_ERR_BAD_ARG and "not aligned to its type" in native_lib.tbvh_last_error().decode()
+
+
 def test_backward_entry_rejects(native_lib):
     g = _geometry(node_aabbs=16, sorted_indices=16, plan=256, plan_bytes=2**40)
     call = lambda *a: native_lib.tbvh_attend_blocks_backward(ctypes.byref(g), ctypes.byref(_features()), *a)

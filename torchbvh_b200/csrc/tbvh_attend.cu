@@ -1,7 +1,9 @@
 // C entries of block attention: argument checks, launch plans, and the small
 // kernels around the two backward passes.
 #include <algorithm>
+#include <cfloat>
 #include <climits>
+#include <cmath>
 #include <type_traits>
 
 #include "tbvh_attend_q.cuh"
@@ -171,6 +173,16 @@ void plan_heads(AttendArgs& a, int size, bool back) {
   }
 }
 
+// Whether every pointer (NULL or not) lies on a multiple of `size`.
+template <typename... P>
+bool aligned(size_t size, P... pointers) {
+  return ((uintptr_t(pointers) % size == 0) && ...);
+}
+
+int element_size(int dtype) { return dtype == TBVH_F32 ? 4 : 2; }
+
+int misaligned(const char* op) { return blocks_fail(TBVH_ERR_BAD_ARG, "%s: a pointer is not aligned to its type", op); }
+
 int check_features(const char* op, const tbvh_attend_features* f, bool pointers) {
   if (f == nullptr) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: features are NULL", op);
   if (f->dtype != TBVH_F32 && f->dtype != TBVH_F16 && f->dtype != TBVH_BF16)
@@ -183,14 +195,16 @@ int check_features(const char* op, const tbvh_attend_features* f, bool pointers)
     return blocks_fail(TBVH_ERR_BAD_ARG, "%s: channels must be 1 to 128", op);
   if (f->num_buckets < 0 || f->num_buckets > kMaxBuckets)
     return blocks_fail(TBVH_ERR_BAD_ARG, "%s: the bias has 1 to %d buckets", op, kMaxBuckets);
+  if (!(fabsf(f->scale) <= FLT_MAX)) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: scale must be finite", op);
   if (!pointers) return TBVH_OK;
   if (f->num_buckets > 0 && (!f->bias_table || (!f->bias_edges && f->num_buckets > 1)))
     return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL bias pointer", op);
   if (!f->keys || !f->values) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL input pointer", op);
+  if (!aligned(element_size(f->dtype), f->queries, f->keys, f->values) ||
+      (f->num_buckets > 0 && !aligned(4, f->bias_table, f->bias_edges)))
+    return misaligned(op);
   return TBVH_OK;
 }
-
-int element_size(int dtype) { return dtype == TBVH_F32 ? 4 : 2; }
 
 AttendArgs common_args(const tbvh_block_geometry* g, const tbvh_attend_features* f, const BlockSetup& s,
                        bool back) {
@@ -255,6 +269,7 @@ int tbvh_attend_blocks(const tbvh_block_geometry* g, const tbvh_attend_features*
   if (out_exact && f->dtype == TBVH_F32)
     return blocks_fail(TBVH_ERR_BAD_ARG, "%s: out_exact is for 16-bit features (out is float32 already)", op);
   if (!f->queries || !out) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL query or output pointer", op);
+  if (!aligned(element_size(f->dtype), out) || !aligned(8, stats) || !aligned(4, out_exact, workspace)) return misaligned(op);
   AttendArgs a = common_args(g, f, s, false);
   a.splits = forward_splits(s, a);
   const size_t need = tbvh_attend_blocks_workspace_size(g, f);
@@ -301,6 +316,9 @@ int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_
     return blocks_fail(TBVH_ERR_BAD_ARG, "%s: grad_table needs a bias", op);
   if (s.total_queries > 0 && (!f->queries || (!out && !out_exact) || !stats || !grad_out))
     return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL query, output or gradient pointer", op);
+  if (!aligned(element_size(f->dtype), out, grad_out, grad_queries, grad_keys, grad_values) ||
+      !aligned(8, stats, workspace) || !aligned(4, out_exact, grad_table))
+    return misaligned(op);
   const BackwardSizes b = backward_sizes(s, f);
   if (workspace == nullptr || workspace_bytes < b.total())
     return blocks_fail(TBVH_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the required %zu", op,

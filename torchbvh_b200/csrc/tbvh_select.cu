@@ -140,6 +140,8 @@ int setup_blocks(const char* op, const tbvh_block_geometry* g, BlockSetup& s) {
   if (g->plan == nullptr || g->plan_bytes < need)
     return blocks_fail(TBVH_ERR_WORKSPACE, "%s: plan of %zu bytes is smaller than the required %zu", op, g->plan_bytes,
                        need);
+  if (uintptr_t(g->plan) % 16 != 0)
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: the plan must lie on a multiple of 16 bytes", op);
   char* at = static_cast<char*>(g->plan);
   s.plan.query_row = reinterpret_cast<int*>(at);
   at += p.rows;
