@@ -124,25 +124,9 @@ cudaError_t run_delta(const void* grad, const void* out, const float* exact, flo
 
 size_t pad256(size_t v) { return (v + 255) / 256 * 256; }
 
-struct BackwardSizes {
-  size_t delta, most, part, rows;
-  size_t total() const { return delta + most + part + rows; }
-};
-
-BackwardSizes backward_sizes(const BlockSetup& s, const tbvh_attend_features* f) {
-  BackwardSizes b{};
-  b.delta = pad256(size_t(s.total_queries) * f->heads * 4);
-  b.most = 256;
-  if (f->num_buckets > 0) {
-    b.part = pad256(size_t(s.map.num_tiles) * f->heads * f->num_buckets * 4);
-    b.rows = pad256(size_t(kTableRows) * f->heads * f->num_buckets * 8);
-  }
-  return b;
-}
-
-// Splits of the forward pass: enough thread blocks for two an SM when the tiles
-// alone are fewer, never more than a tile can have entries.
-int forward_splits(const BlockSetup& s, const AttendArgs& a) {
+// Splits of the kernels by query tile: enough thread blocks for two an SM when the
+// tiles alone are fewer, never more than a tile can have entries.
+int tile_splits(const BlockSetup& s, const AttendArgs& a) {
   const int64_t blocks = s.map.num_tiles * head_groups(a);
   if (blocks <= 0 || blocks >= 148) return 1;
   int64_t want = (296 + blocks - 1) / blocks;
@@ -231,6 +215,24 @@ AttendArgs common_args(const tbvh_block_geometry* g, const tbvh_attend_features*
   return a;
 }
 
+struct BackwardSizes {
+  size_t delta, most, part, rows, queries;
+  size_t total() const { return delta + most + part + rows + queries; }
+};
+
+BackwardSizes backward_sizes(const BlockSetup& s, const tbvh_attend_features* f, int splits) {
+  BackwardSizes b{};
+  b.delta = pad256(size_t(s.total_queries) * f->heads * 4);
+  b.most = 256;
+  if (f->num_buckets > 0) {
+    b.part = pad256(size_t(splits) * s.map.num_tiles * f->heads * f->num_buckets * 4);
+    b.rows = pad256(size_t(kTableRows) * f->heads * f->num_buckets * 8);
+  }
+  if (splits > 1)
+    b.queries = size_t(splits) * s.map.num_tiles * f->heads * kTileQueries * padded_channels(f->channels) * 4;
+  return b;
+}
+
 // Row copies place rows by 32-bit counts of 16-byte words; tensors past 64 GB
 // take the narrower copies, which count in 64 bits.
 bool words_fit(const BlockSetup& s, const tbvh_attend_features* f) {
@@ -251,7 +253,7 @@ size_t tbvh_attend_blocks_workspace_size(const tbvh_block_geometry* g, const tbv
   BlockSetup s;
   if (measure_blocks("attend_blocks", g, s) || check_features("attend_blocks", f, false)) return 0;
   const AttendArgs a = common_args(g, f, s, false);
-  const int splits = forward_splits(s, a);
+  const int splits = tile_splits(s, a);
   if (splits == 1) return 256;
   return size_t(splits) * s.map.num_tiles * f->heads * kTileQueries * (2 * padded_channels(f->channels) + 2) * 4;
 }
@@ -271,7 +273,7 @@ int tbvh_attend_blocks(const tbvh_block_geometry* g, const tbvh_attend_features*
   if (!f->queries || !out) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL query or output pointer", op);
   if (!aligned(element_size(f->dtype), out) || !aligned(8, stats) || !aligned(4, out_exact, workspace)) return misaligned(op);
   AttendArgs a = common_args(g, f, s, false);
-  a.splits = forward_splits(s, a);
+  a.splits = tile_splits(s, a);
   const size_t need = tbvh_attend_blocks_workspace_size(g, f);
   if (a.splits > 1 && (workspace == nullptr || workspace_bytes < need))
     return blocks_fail(TBVH_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the required %zu", op,
@@ -294,7 +296,7 @@ size_t tbvh_attend_blocks_backward_workspace_size(const tbvh_block_geometry* g, 
   using namespace tbvh;
   BlockSetup s;
   if (measure_blocks("attend_blocks_backward", g, s) || check_features("attend_blocks_backward", f, false)) return 0;
-  return backward_sizes(s, f).total();
+  return backward_sizes(s, f, tile_splits(s, common_args(g, f, s, true))).total();
 }
 
 int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_features* f, const void* out,
@@ -319,11 +321,12 @@ int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_
   if (!aligned(element_size(f->dtype), out, grad_out, grad_queries, grad_keys, grad_values) ||
       !aligned(8, stats, workspace) || !aligned(4, out_exact, grad_table))
     return misaligned(op);
-  const BackwardSizes b = backward_sizes(s, f);
+  AttendArgs a = common_args(g, f, s, true);
+  a.splits = tile_splits(s, a);
+  const BackwardSizes b = backward_sizes(s, f, a.splits);
   if (workspace == nullptr || workspace_bytes < b.total())
     return blocks_fail(TBVH_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the required %zu", op,
                        workspace_bytes, b.total());
-  AttendArgs a = common_args(g, f, s, true);
   char* at = static_cast<char*>(workspace);
   a.delta = reinterpret_cast<float*>(at);
   at += b.delta;
@@ -332,6 +335,9 @@ int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_
   float* part = reinterpret_cast<float*>(at);
   at += b.part;
   double* rows = reinterpret_cast<double*>(at);
+  at += b.rows;
+  a.part = reinterpret_cast<float*>(at);
+  a.part_row = padded_channels(f->channels);
   a.stats_in = reinterpret_cast<const float2*>(stats);
   a.grad_out = grad_out;
   a.grad_q = grad_queries;
@@ -367,7 +373,7 @@ int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_
     if (s.total_queries == 0) {
       e = cudaMemsetAsync(grad_table, 0, size_t(values) * 4, st);
     } else {
-      e = launch_table_sum(part, rows, grad_table, s.map.num_tiles, values, st);
+      e = launch_table_sum(part, rows, grad_table, a.splits * s.map.num_tiles, values, st);
     }
   }
   if (e == cudaSuccess && grad_keys) e = launch_attend_grad_kv(a, f->dtype, st);

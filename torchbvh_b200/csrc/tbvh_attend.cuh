@@ -673,7 +673,7 @@ struct AttendArgs {
   float* delta;    // [total_queries][heads] <grad_out, out>
   const unsigned* largest;  // float bits of the largest finite |grad_out| and |value| (float16 only)
   void *grad_q, *grad_k, *grad_v;
-  float* table_part;  // [tiles][heads][buckets], nullable
+  float* table_part;  // [split][tiles][heads][buckets], nullable
 };
 
 // First query head, count, first key/value head and count of blockIdx.y.
@@ -761,7 +761,7 @@ constexpr int kTableRows = 64;
 cudaError_t launch_attend_forward(const AttendArgs& a, int dtype, cudaStream_t stream);
 cudaError_t launch_attend_forward_exact(const AttendArgs& a, int dtype, cudaStream_t stream);
 cudaError_t launch_attend_merge(const AttendArgs& a, int dtype, cudaStream_t stream);
-cudaError_t launch_attend_grad_q(const AttendArgs& a, int dtype, cudaStream_t stream);
+cudaError_t launch_attend_grad_q(const AttendArgs& a, int dtype, cudaStream_t stream);  // joins its splits too
 cudaError_t launch_attend_grad_kv(const AttendArgs& a, int dtype, cudaStream_t stream);
 // grad_table[values] = sum of part[rows][values] in a fixed order; scratch of kTableRows * values doubles.
 cudaError_t launch_table_sum(const float* part, double* scratch, float* grad_table, int64_t rows, int values,

@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
   const int warps = int(blockDim.x) / 32;
 
   const int all = a.plan.tile_count[tile];
-  const int splits = BACK ? 1 : a.splits;
+  const int splits = a.splits;
   const int from = int(int64_t(all) * blockIdx.z / splits);
   const int steps = 2 * (int(int64_t(all) * (blockIdx.z + 1) / splits) - from);
   const uint2* entries = a.plan.entries + tile * a.plan.capacity + from;
@@ -486,8 +486,19 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
       const float back = a.scale / lift;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int row = s_rows[half * 16 + g + 8 * r];
+        const int q = half * 16 + g + 8 * r, row = s_rows[q];
         if (row < 0) continue;
+        if (splits > 1) {
+          float* part = a.part + (((int64_t(blockIdx.z) * a.map.num_tiles + tile) * a.heads + span.h0 + head) *
+                                      kTileQueries + q) * a.part_row;
+#pragma unroll
+          for (int n = 0; n < CP / 8; ++n) {
+            const float2 x = unpair(acc[n][r]);
+            part[n * 8 + 2 * t] = x.x;
+            part[n * 8 + 2 * t + 1] = x.y;
+          }
+          continue;
+        }
         T* out = static_cast<T*>(a.grad_q) + (int64_t(row) * a.heads + span.h0 + head) * a.channels;
 #pragma unroll
         for (int n = 0; n < CP / 8; ++n)
@@ -509,7 +520,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
       for (int i = tid; i < span.heads * a.buckets; i += blockDim.x) {
         const int h = i / a.buckets, b = i % a.buckets;
         const float x = s_hist[b * blockDim.x + h * 64] + s_hist[b * blockDim.x + h * 64 + 32];
-        a.table_part[(tile * a.heads + span.h0) * a.buckets + i] = x / lift;
+        a.table_part[((int64_t(blockIdx.z) * a.map.num_tiles + tile) * a.heads + span.h0) * a.buckets + i] = x / lift;
       }
     }
   }
@@ -521,7 +532,7 @@ cudaError_t run_query_tile(const AttendArgs& a, cudaStream_t stream) {
       query_tile_smem(sizeof(T), CP, a.kv_cta, a.heads_cta, BACK, a.table != nullptr, a.buckets);
   cudaError_t e = allow_smem(k_query_tile<T, CP, BACK, EXACT>, s.total);
   if (e != cudaSuccess) return e;
-  const dim3 grid(unsigned(a.map.num_tiles), unsigned(head_groups(a)), BACK ? 1 : unsigned(a.splits));
+  const dim3 grid(unsigned(a.map.num_tiles), unsigned(head_groups(a)), unsigned(a.splits));
   k_query_tile<T, CP, BACK, EXACT><<<grid, a.heads_cta * 64, s.total, stream>>>(a);
   return cudaGetLastError();
 }
