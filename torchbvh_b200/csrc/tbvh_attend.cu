@@ -124,12 +124,14 @@ cudaError_t run_delta(const void* grad, const void* out, const float* exact, flo
 
 size_t pad256(size_t v) { return (v + 255) / 256 * 256; }
 
-// Splits of the kernels by query tile: enough thread blocks for two an SM when the
-// tiles alone are fewer, never more than a tile can have entries.
+// Splits of the kernels by query tile: enough thread blocks for four an SM when the
+// tiles alone are fewer than two, never more than a tile can have entries (189 thread
+// blocks, float32 training: 622 us, 645 when only fewer than 148 were split; 64 as
+// one: 1,773 us, split 664).
 int tile_splits(const BlockSetup& s, const AttendArgs& a) {
   const int64_t blocks = s.map.num_tiles * head_groups(a);
-  if (blocks <= 0 || blocks >= 148) return 1;
-  int64_t want = (296 + blocks - 1) / blocks;
+  if (blocks <= 0 || blocks >= 2 * 148) return 1;
+  int64_t want = (4 * 148 + blocks - 1) / blocks;
   if (want > s.plan.capacity) want = s.plan.capacity;
   return int(want < 1 ? 1 : want > 32 ? 32 : want);
 }
