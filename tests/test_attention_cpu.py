@@ -69,6 +69,56 @@ def test_select_rejects_a_destroyed_handle():
         torchbvh.select_blocks(handle, torch.zeros(4, 3), 4)
 
 
+class _Streams:
+    """The allocator's stream calls, kept: a fake current stream, and what was recorded on which."""
+
+    def __init__(self, monkeypatch):
+        self.current, self.capturing, self.recorded = 0, False, []
+        monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+        monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: self.recorded.append((t.data_ptr(), s)))
+        monkeypatch.setattr(_native, "raw_stream", lambda device: self.current)
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: self.current)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: self.capturing)
+
+        def select(geometry, total, device):
+            n = geometry.num_blocks
+            return torch.zeros(total, n, dtype=torch.int64), torch.zeros(total, n), torch.zeros(256, dtype=torch.uint8)
+
+        monkeypatch.setattr(_native, "select_blocks", select)
+        monkeypatch.setattr(_native.BlockGeometry, "device", property(lambda g: 0, lambda g, v: None))
+
+    def take(self):
+        got, self.recorded = set(self.recorded), []
+        return got
+
+
+@pytest.mark.parametrize("built_on", [1, None])
+@pytest.mark.parametrize("batched", [False, True])
+def test_the_tree_s_memory_is_recorded_on_the_stream_that_selects(monkeypatch, batched, built_on):
+    # Its memory goes back to the stream that built it as soon as the caller drops it, while the
+    # selection's stream, and later the attention's, may still have to read it.
+    streams = _Streams(monkeypatch)
+    handle, queries = (_batched(), torch.zeros(2, 5, 3)) if batched else (_handle(), torch.zeros(5, 3))
+    handle._fields.update(scene_min=torch.zeros(3), scene_max=torch.ones(3))
+    handle._built_on = built_on
+    tree = {handle[x].data_ptr() for x in ("node_aabbs", "sorted_indices", "scene_min", "scene_max")}
+    streams.current = 2
+    selection = torchbvh.select_blocks(handle, queries, 4)
+    assert streams.take() == {(p, 2) for p in tree}
+    selection._stream = 2  # (a device tensor's)
+    selection._used_here()
+    assert not streams.take()
+    streams.current = 1  # the tree's own stream: the selection's memory is what it reads of others
+    selection._used_here()
+    assert streams.take() >= {(selection._keep[2].data_ptr(), 1)}
+    if built_on is not None:
+        torchbvh.select_blocks(handle, queries, 4)
+        assert not streams.take()
+    streams.current, streams.capturing = 3, True
+    torchbvh.select_blocks(handle, queries, 4)
+    assert not streams.take()
+
+
 def _selection(query_shape=(5,), key_shape=(100,), backward=1):
     fields = {"block_indices": torch.zeros(*query_shape, 4, dtype=torch.int64), "num_blocks": 4}
     return BlockSelection(fields, _native.BlockGeometry(backward=backward), (), key_shape, query_shape)

@@ -575,6 +575,35 @@ def test_on_another_stream():
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+@pytest.mark.parametrize("queries", [200, 20000])  # put in order by the call, and by the sort that reads the tree's box
+@pytest.mark.parametrize("layout", ["single", "ragged"])
+def test_a_tree_of_another_stream_may_be_dropped_while_it_is_read(layout, queries):
+    scene = Scene(layout, [3000], [queries], 3, seed=24)
+    points, qpts, offsets, query_offsets = (scene.tensor(scene.points), scene.tensor(scene.qpts), scene.offsets([3000]),
+                                            scene.offsets([queries]))
+    f = _features(scene, F32, 2, 2, 16, 0, seed=24)
+    q, k, v = (scene.tensor(f[x]) for x in "qkv")
+    first = torchbvh.select_blocks(scene.bvh, qpts, 4, query_offsets=query_offsets)
+    want = first["block_indices"], torchbvh.attend_blocks(first, q, k, v)
+    builder, reader = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(builder):
+        tree = torchbvh.build_bvh(points, batch_offsets=offsets)
+        sizes = [t.numel() * t.element_size() for t in (scene.bvh._packed if layout == "ragged" else scene.bvh).values()
+                 if isinstance(t, torch.Tensor)]
+    reader.wait_stream(builder)
+    with torch.cuda.stream(reader):
+        torch.cuda._sleep(100_000_000)  # some 50 ms
+        selection = torchbvh.select_blocks(tree, qpts, 4, query_offsets=query_offsets)
+        torch.cuda._sleep(100_000_000)
+        got = selection["block_indices"], torchbvh.attend_blocks(selection, q, k, v)
+        del tree, selection
+    with torch.cuda.stream(builder):
+        over = [torch.zeros(n, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(8)]
+    torch.cuda.synchronize()
+    assert len(over) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_captured_and_replayed():
     """Forward and backward in one CUDA graph, replayed on new inputs; then a second graph."""
     scene = Scene("single", [1000], [500], 3, seed=21)

@@ -85,12 +85,20 @@ class BlockSelection(_Handle):
         super().destroy()
 
     def _used_here(self) -> None:
-        """Tells the allocator that the current stream reads the selection's memory."""
-        if _native.raw_stream(self._device) != self._stream and not torch.cuda.is_current_stream_capturing():
-            stream = torch.cuda.current_stream(self._device)
-            for item in self._keep:
-                if isinstance(item, torch.Tensor) and item.is_cuda:
-                    item.record_stream(stream)
+        """Tells the allocator that the current stream reads the selection's memory. (The stream
+        that made the selection is known to it: ``select_blocks`` recorded the tree's memory.)"""
+        _record_use(self._keep, self._stream, self._device)
+
+
+def _record_use(items, known: int | None, device: torch.device) -> None:
+    """Tells the allocator that the current stream reads the tensors of ``items``, which lie in
+    memory of the stream ``known`` (None: not known). A captured graph outlives any such record:
+    there the memory has to be kept."""
+    if _native.raw_stream(device) != known and not torch.cuda.is_current_stream_capturing():
+        stream = torch.cuda.current_stream(device)
+        for item in items:
+            if isinstance(item, torch.Tensor) and item.is_cuda:
+                item.record_stream(stream)
 
 
 # The messages are put together only for a call that is refused.
@@ -166,6 +174,8 @@ def select_blocks(bvh: BVHHandle | BatchedBVHHandle | RaggedBVHHandle, query_poi
         keep = ()
         key_shape = ((clouds,) if batched else ()) + (tree["num_leaves"],)
     nodes, leaves = tree["node_aabbs"], tree["sorted_indices"]
+    # The caller may drop the tree as soon as this returns, and with it memory of the stream that built it.
+    _record_use((nodes, leaves, tree["scene_min"], tree["scene_max"]), bvh._built_on, device)
     geometry.device, geometry.dim = device.index, tree["dim"]
     geometry.node_aabbs, geometry.sorted_indices = nodes.data_ptr(), leaves.data_ptr()
     geometry.query_points = queries.data_ptr()

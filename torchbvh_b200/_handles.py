@@ -35,6 +35,7 @@ class _Deferred:
 class _Handle(Mapping):
     kind_message = "BVH handle has been destroyed"
     marker: str | None = None
+    _built_on: int | None = None  # stream whose memory the payload lies in; None: not known
 
     def __init__(self, fields: Mapping):
         self._fields = dict(fields)

@@ -32,7 +32,7 @@ from ._handles import (
     _bvh_data,
     _ragged_bvh_data,
 )
-from ._native import _C
+from ._native import _C, raw_stream
 from ._validation import (
     _as_contiguous,
     _as_contiguous_int64,
@@ -137,17 +137,23 @@ def _checked_build_points(layout: str, points: torch.Tensor) -> torch.Tensor:
     return points
 
 
+def _built_here(handle, device: torch.device):
+    handle._built_on = raw_stream(device)
+    return handle
+
+
 def _build_bvh_single(points: torch.Tensor) -> BVHHandle:
     points = _checked_build_points(_SINGLE, points)
     payload = _C.build_bvh_batched_cooperative(points.unsqueeze(0))
     # One cloud is a batch of one: drop the batch dimension of the per-cloud fields.
     fields = {key: (value[0] if key in ("node_aabbs", "sorted_indices", "scene_min", "scene_max") else value)
               for key, value in payload.items() if key != "batch_size"}
-    return BVHHandle(fields)
+    return _built_here(BVHHandle(fields), points.device)
 
 
 def _build_bvh_batched(points: torch.Tensor) -> BatchedBVHHandle:
-    return BatchedBVHHandle(_C.build_bvh_batched_cooperative(_checked_build_points(_BATCHED, points)))
+    points = _checked_build_points(_BATCHED, points)
+    return _built_here(BatchedBVHHandle(_C.build_bvh_batched_cooperative(points)), points.device)
 
 
 def _sample_payload(packed: Mapping, batch: int) -> dict:
@@ -180,7 +186,7 @@ def _build_bvh_ragged(points: torch.Tensor, batch_offsets: torch.Tensor) -> Ragg
         "batch_size": len(offsets) - 1,
         "dim": int(points.size(1)),
     }
-    return RaggedBVHHandle(meta, samples, packed)
+    return _built_here(RaggedBVHHandle(meta, samples, packed), points.device)
 
 
 def build_bvh(
