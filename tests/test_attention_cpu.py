@@ -6,6 +6,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import torchbvh_b200 as torchbvh
 from torchbvh_b200 import _native
@@ -229,6 +230,39 @@ def test_distance_bias_rejects_bad_arguments(monkeypatch):
         torchbvh.distance_bias(d2[:, :, 0], torch.zeros(0, 3), edges)
     with pytest.raises(ValueError, match="edges must have shape"):
         torchbvh.distance_bias(d2, table, torch.zeros(3))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("dual", range(4))
+def test_forward_mode_derivatives_are_refused_not_dropped(monkeypatch, dual, grad):
+    # A dual tensor need not require a gradient; its tangent must not be lost on the way.
+    _Streams(monkeypatch)
+    monkeypatch.setattr(_native, "attend_blocks", lambda geometry, q, *rest: (q.clone(), None, None))
+    inputs = [*_qkv(), torch.zeros(2, 4)]
+    edges = torch.zeros(3)
+    with forward_ad.dual_level():
+        assert torchbvh.attend_blocks(_selection(), *inputs[:3], bias_table=inputs[3], bias_edges=edges) is not None
+        t = inputs[dual].requires_grad_(grad)
+        inputs[dual] = forward_ad.make_dual(t, torch.ones_like(t))
+        for x in inputs:
+            if x is not inputs[dual]:
+                x.requires_grad_(grad)
+        with pytest.raises(NotImplementedError, match="attend_blocks: forward-mode derivatives"):
+            torchbvh.attend_blocks(_selection(), *inputs[:3], bias_table=inputs[3], bias_edges=edges)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="attend_blocks: forward-mode derivatives"):
+            torchbvh.attend_blocks(_selection(), *inputs[:3], bias_table=inputs[3], bias_edges=edges)
+
+
+def test_distance_bias_refuses_forward_mode_derivatives(monkeypatch):
+    _Streams(monkeypatch)
+    monkeypatch.setattr(_native, "distance_bias", lambda d2, heads, *rest: torch.zeros(1, 10, heads, 4))
+    d2, edges = torch.zeros(1, 10, 4), torch.zeros(2)
+    with forward_ad.dual_level():
+        # Buckets do not change with the distances: their derivative is zero.
+        assert torchbvh.distance_bias(forward_ad.make_dual(d2, torch.ones_like(d2)), torch.zeros(2, 3), edges) is not None
+        table = forward_ad.make_dual(torch.zeros(2, 3), torch.ones(2, 3))
+        with pytest.raises(NotImplementedError, match="distance_bias: forward-mode derivatives"):
+            torchbvh.distance_bias(d2, table, edges)
 
 
 # ---- C ABI ----------------------------------------------------------------------------------

@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from ._constants import (
@@ -202,6 +203,12 @@ def _check_bias(prefix: str, table: torch.Tensor, edges: torch.Tensor, heads: in
         raise ValueError(f"{prefix}: {table_name} and {edges_name} must be on the same device as the other inputs")
 
 
+def _refuse_tangents(prefix: str, *tensors: torch.Tensor | None) -> None:
+    """Forward-mode derivatives would be dropped: a dual tensor need not require a gradient."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{prefix}: forward-mode derivatives are not implemented")
+
+
 class _AttendBlocks(torch.autograd.Function):
     """Attention with the backward pass of the native library. Keeps its inputs,
     its output and two numbers a row (its softmax's maximum and sum). Where a bias
@@ -252,7 +259,7 @@ def attend_blocks(selection: BlockSelection, queries: torch.Tensor, keys: torch.
     no point to attend to gets zeros.
 
     Differentiable in ``queries``, ``keys``, ``values`` and ``bias_table`` (the
-    selection must have been made with ``backward=True``). Results and gradients
+    selection must have been made with ``backward=True``), in reverse mode. Results and gradients
     of equal inputs are equal bit for bit: nothing is summed in changing order.
     Products of 16-bit features are summed in float32; the softmax is float32.
     """
@@ -292,6 +299,7 @@ def attend_blocks(selection: BlockSelection, queries: torch.Tensor, keys: torch.
     scale = channels**-0.5 if scale is None else float(scale)
     if not abs(scale) <= torch.finfo(torch.float32).max:
         raise ValueError(f"{prefix}: scale must be finite in float32")
+    _refuse_tangents(prefix, queries, keys, values, bias_table)
     queries, keys, values = _as_contiguous(queries), _as_contiguous(keys), _as_contiguous(values)
     selection._used_here()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (queries, keys, values, bias_table)):
@@ -326,8 +334,8 @@ def distance_bias(squared_distances: torch.Tensor, table: torch.Tensor, edges: t
     ``query_displaced_knn``) or ``(B, N, k)`` (as from ``query_knn``, shared by
     the heads) float32; ``table (H, num_buckets)`` float32 with 1 to 64 buckets;
     ``edges (num_buckets - 1,)`` float32, in any order. Returns
-    ``(B, N, H, k)`` float32, differentiable in ``table``; its gradient is summed
-    in a fixed order.
+    ``(B, N, H, k)`` float32, differentiable in ``table``, in reverse mode; its
+    gradient is summed in a fixed order.
     """
     prefix = "distance_bias"
     rank = squared_distances.dim()
@@ -340,6 +348,7 @@ def distance_bias(squared_distances: torch.Tensor, table: torch.Tensor, edges: t
         raise ValueError(f"{prefix}: squared_distances head dimension must match table")
     if not 1 <= heads <= MAX_BLOCK_HEADS:
         raise ValueError(f"{prefix}: table must have at least one head, and at most {MAX_BLOCK_HEADS}")
+    _refuse_tangents(prefix, table)
     squared_distances = _as_contiguous(squared_distances.detach())
     table, edges = _as_contiguous(table), _as_contiguous(edges.detach())
     if torch.is_grad_enabled() and table.requires_grad:
