@@ -33,6 +33,12 @@ def test_select_rejects_bad_block_counts(n):
         torchbvh.select_blocks(torchbvh.BVHHandle({}), torch.zeros(4, 3), n)
 
 
+@pytest.mark.parametrize("n", [True, False])
+def test_select_rejects_a_truth_value_as_a_block_count(n):
+    with pytest.raises(ValueError, match="num_blocks must be 1 to 32"):
+        torchbvh.select_blocks(torchbvh.BVHHandle({}), torch.zeros(4, 3), n)
+
+
 def test_select_rejects_what_is_no_handle():
     with pytest.raises(TypeError, match="must be a BVHHandle returned by build_bvh"):
         torchbvh.select_blocks({}, torch.zeros(4, 3), 4)

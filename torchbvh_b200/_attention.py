@@ -135,7 +135,7 @@ def select_blocks(bvh: BVHHandle | BatchedBVHHandle | RaggedBVHHandle, query_poi
     ``attend_blocks`` needs, for inference. Carries no gradient.
     """
     prefix = "select_blocks"
-    if not (isinstance(num_blocks, int) and 1 <= num_blocks <= MAX_SELECTED_BLOCKS):
+    if not (isinstance(num_blocks, int) and not isinstance(num_blocks, bool) and 1 <= num_blocks <= MAX_SELECTED_BLOCKS):
         raise ValueError(f"{prefix}: num_blocks must be 1 to {MAX_SELECTED_BLOCKS}")
     geometry = _native.BlockGeometry(num_blocks=num_blocks, backward=1 if backward else 0)
     if isinstance(bvh, RaggedBVHHandle):
