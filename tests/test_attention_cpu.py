@@ -3,6 +3,7 @@ bias: everything that is checked before any device work."""
 from __future__ import annotations
 
 import ctypes
+import re
 
 import pytest
 import torch
@@ -272,6 +273,21 @@ def test_distance_bias_refuses_forward_mode_derivatives(monkeypatch):
 
 
 # ---- C ABI ----------------------------------------------------------------------------------
+
+def test_python_s_limits_are_the_library_s():
+    from torchbvh_b200 import _attention, _build_lib, _constants
+
+    def value(path, pattern):
+        (found,) = re.findall(pattern, path.read_text())
+        return int(found)
+
+    header, blocks = _build_lib.INCLUDE / "torchbvh_b200.h", _build_lib.CSRC / "tbvh_blocks.h"
+    # Were the first lower in the library, larger clouds would keep the caller's order of queries.
+    assert _attention._SMALL == value(header, r"TBVH_SMALL_QUERIES = (\d+)")
+    assert _constants.MAX_SELECTED_BLOCKS == value(blocks, r"kMaxSelect = (\d+)")
+    assert _constants.MAX_BIAS_BUCKETS == value(blocks, r"kMaxBuckets = (\d+)")
+    assert _constants.BLOCK_SIZE == 1 << value(blocks, r"kBlockLevels = (\d+)")
+
 
 def test_block_table(native_lib):
     table = list(_native.block_table([0, 64, 65, 1000], [0, 10, 10, 75]))
