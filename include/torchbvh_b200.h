@@ -294,7 +294,8 @@ typedef struct tbvh_block_geometry {
   int device;
   int dim;                        /* 2 or 3 */
   int num_blocks;                 /* blocks per query, 1..32 */
-  int backward;                   /* 1: the plan also serves the backward pass */
+  int backward;                   /* 1: the plan also serves the backward pass (at most 2^27 tiles: a cloud has
+                                   * one for every 32 queries or part of them) */
   int64_t num_clouds;
   int64_t points_per_cloud;
   int64_t queries_per_cloud;

@@ -330,6 +330,16 @@ def test_plan_size(native_lib):
     assert size(points_per_cloud=2**30, queries_per_cloud=2**30, num_clouds=1, num_blocks=32) > 2**36
 
 
+def test_plan_rejects_more_tiles_than_the_backward_lists_can_number(native_lib):
+    # Query slots of the lists are 32 bits: at most 2^27 tiles, of which each small cloud has its own.
+    size = lambda **kw: native_lib.tbvh_block_plan_size(
+        ctypes.byref(_geometry(points_per_cloud=1, queries_per_cloud=1, **kw)))
+    assert size(num_clouds=2**27, backward=1) > 0
+    assert size(num_clouds=2**27 + 1) > 0
+    assert size(num_clouds=2**27 + 1, backward=1) == 0
+    assert "too many clouds" in native_lib.tbvh_last_error().decode()
+
+
 @pytest.mark.parametrize("change, text", [
     ({"dim": 4}, "D must be 2 or 3"),
     ({"num_blocks": 0}, "num_blocks must be 1 to 32"),

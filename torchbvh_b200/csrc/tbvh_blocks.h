@@ -23,6 +23,7 @@ namespace tbvh {
 constexpr int kBlockLevels = 6;
 constexpr int kBlockLeaves = 1 << kBlockLevels;
 constexpr int kTileQueries = 32;
+constexpr int64_t kMostListTiles = (int64_t(1) << 32) / kTileQueries;  // of the backward lists, whose slots are 32 bits
 constexpr int kMaxSelect = 32;
 constexpr int kMaxBuckets = 64;
 

@@ -119,6 +119,10 @@ int measure_blocks(const char* op, const tbvh_block_geometry* g, BlockSetup& s) 
     s.total_points = want.p0;
     s.total_queries = want.q0;
   }
+  // Small clouds have a tile each: more tiles than 32-bit query slots reach are fewer than 2^31 queries.
+  if (g->backward && map.num_tiles > kMostListTiles)
+    return blocks_fail(TBVH_ERR_BAD_ARG, "%s: too many clouds for the backward lists (at most 2^27 tiles of %d queries)",
+                       op, kTileQueries);
   s.most_queries = most_queries;
   s.most_blocks = most_blocks;
   s.plan.capacity = (most_queries < kTileQueries ? most_queries : kTileQueries) * g->num_blocks;
