@@ -4,7 +4,9 @@
  * Plain pointers and sizes only. Every device pointer must live on `device`;
  * every call enqueues work on `stream` (a cudaStream_t passed as void*) and
  * returns without synchronising. Outputs and workspace are caller-allocated
- * (the Python layer uses the PyTorch caching allocator). Return value 0 is
+ * (the Python layer uses the PyTorch caching allocator). An entry leaves
+ * `device` the thread's current device (the Python calls of block selection,
+ * block attention and the distance bias put the caller's back). Return value 0 is
  * success; otherwise one of TBVH_ERR_* with a message in tbvh_last_error().
  *
  * Each entry point names the reference interface it replaces (paths inside

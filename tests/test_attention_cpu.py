@@ -127,6 +127,56 @@ def test_the_tree_s_memory_is_recorded_on_the_stream_that_selects(monkeypatch, b
     assert not streams.take()
 
 
+@pytest.mark.parametrize("fails", [False, True])
+@pytest.mark.parametrize("name", ["select_blocks", "sorted", "ragged", "attend_blocks", "attend_blocks_backward",
+                                  "distance_bias", "distance_bias_backward"])
+def test_the_current_device_stays_the_caller_s(monkeypatch, name, fails):
+    # A library whose entries make another device the current one, as they do for tensors there.
+    current = [0]
+
+    class Library:
+        def __getattr__(self, entry):
+            def call(*args):
+                current[0] = 1
+                return 256 if entry.endswith("_size") else _native.TBVH_ERR_BAD_ARG if fails else 0
+            return (lambda: b"refused") if entry == "tbvh_last_error" else call
+
+    monkeypatch.setattr(_native, "load_library", Library)
+    monkeypatch.setattr(_native, "raw_stream", lambda device: 0)
+    monkeypatch.setattr(_native, "_stream", lambda device: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "set_device", lambda d: current.__setitem__(0, d))
+    q, k, v = _qkv()
+    table, edges, stats, d2 = torch.zeros(2, 4), torch.zeros(3), torch.zeros(5, 2, 2), torch.zeros(1, 10, 4)
+    if name in ("sorted", "ragged"):
+        monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        monkeypatch.setattr(_native.BlockGeometry, "device", property(lambda g: 0, lambda g, x: None))
+        monkeypatch.setattr(_native, "block_table", lambda *a: (ctypes.c_int64 * 7)())
+        monkeypatch.setattr(_native, "select_blocks", lambda g, m, d: (torch.zeros(m, 4), torch.zeros(m, 4), None))
+        handle, m, offsets = _handle(), 16385, None
+        handle._fields.update(scene_min=torch.zeros(3), scene_max=torch.ones(3))
+        if name == "ragged":
+            offsets = torch.tensor([0, m])
+            handle = torchbvh.RaggedBVHHandle({"batch_size": 1}, [], {**handle._fields, "point_offsets": [0, 100]})
+        call = lambda: torchbvh.select_blocks(handle, torch.zeros(m, 3), 4, query_offsets=offsets)
+    else:
+        call = {
+            "select_blocks": lambda: _native.select_blocks(_geometry(), 5, torch.device("cpu")),
+            "attend_blocks": lambda: _native.attend_blocks(_geometry(), q, k, v, table, edges, 1.0, True, False),
+            "attend_blocks_backward": lambda: _native.attend_blocks_backward(
+                _geometry(), q, k, v, table, edges, 1.0, q, None, stats, q, True, True, True),
+            "distance_bias": lambda: _native.distance_bias(d2, 2, False, table, edges),
+            "distance_bias_backward": lambda: _native.distance_bias_backward(d2, 2, False, edges, torch.zeros(1, 10, 2, 4)),
+        }[name]
+    if fails:
+        with pytest.raises(RuntimeError, match="refused"):
+            call()
+    else:
+        call()
+    assert current[0] == 0
+
+
 def _selection(query_shape=(5,), key_shape=(100,), backward=1):
     fields = {"block_indices": torch.zeros(*query_shape, 4, dtype=torch.int64), "num_blocks": 4}
     return BlockSelection(fields, _native.BlockGeometry(backward=backward), (), key_shape, query_shape)

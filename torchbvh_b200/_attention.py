@@ -152,8 +152,8 @@ def select_blocks(bvh: BVHHandle | BatchedBVHHandle | RaggedBVHHandle, query_poi
             len(host) - 1, ctypes.cast(table, ctypes.c_void_p), table_dev.data_ptr())
         order = None
         if max(b - a for a, b in zip(host, host[1:])) > _SMALL:
-            order = _C.morton_sort_queries_ragged(queries, query_offsets, int(queries.size(0)), tree["scene_min"],
-                                                  tree["scene_max"])
+            order = _native.keeps_device(_C.morton_sort_queries_ragged)(
+                queries, query_offsets, int(queries.size(0)), tree["scene_min"], tree["scene_max"])
         keep = (table, table_dev)
         key_shape = (tree["point_offsets"][-1],)
     else:
@@ -171,7 +171,8 @@ def select_blocks(bvh: BVHHandle | BatchedBVHHandle | RaggedBVHHandle, query_poi
         order = None
         if per_cloud > _SMALL:
             lift = (lambda t: t) if batched else (lambda t: t.unsqueeze(0))
-            order = _C.morton_sort_queries_narrow(lift(queries), lift(tree["scene_min"]), lift(tree["scene_max"]))
+            order = _native.keeps_device(_C.morton_sort_queries_narrow)(
+                lift(queries), lift(tree["scene_min"]), lift(tree["scene_max"]))
         keep = ()
         key_shape = ((clouds,) if batched else ()) + (tree["num_leaves"],)
     nodes, leaves = tree["node_aabbs"], tree["sorted_indices"]

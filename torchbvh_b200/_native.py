@@ -18,6 +18,7 @@ reference's per-sample Python loop (torchbvh/_query.py:68-85,299-366).
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 import types
@@ -580,6 +581,20 @@ def raw_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def keeps_device(call):
+    """Native entries make the inputs' device the current one; this puts the caller's back."""
+    @functools.wraps(call)
+    def kept(*args):
+        before = torch._C._cuda_getDevice()
+        try:
+            return call(*args)
+        finally:
+            if torch._C._cuda_getDevice() != before:
+                torch.cuda.set_device(before)
+
+    return kept
+
+
 def block_table(point_offsets: list[int], query_offsets: list[int]):
     """Host table of a ragged selection: seven int64 a cloud (tbvh_block_table)."""
     clouds = len(point_offsets) - 1
@@ -590,6 +605,7 @@ def block_table(point_offsets: list[int], query_offsets: list[int]):
     return table
 
 
+@keeps_device
 def select_blocks(geometry: BlockGeometry, total_queries: int, device: torch.device):
     """(block_indices, squared_distances, plan) of ``geometry``, whose plan pointer it sets."""
     lib = load_library()
@@ -611,6 +627,7 @@ def _attend_features(queries, keys, values, table, edges, scale: float) -> Atten
                           values.data_ptr(), _data(table), _data(edges))
 
 
+@keeps_device
 def attend_blocks(geometry: BlockGeometry, queries, keys, values, table, edges, scale: float, keep_stats: bool,
                   keep_exact: bool):
     """(out, softmax statistics, out before its rounding to 16 bits); the latter two None unless kept."""
@@ -627,6 +644,7 @@ def attend_blocks(geometry: BlockGeometry, queries, keys, values, table, edges, 
     return out, stats, exact
 
 
+@keeps_device
 def attend_blocks_backward(geometry: BlockGeometry, queries, keys, values, table, edges, scale: float, out,
                            exact, stats, grad_out, need_queries: bool, need_keys: bool, need_table: bool):
     """(grad_queries, grad_keys, grad_values, grad_table), None where not needed."""
@@ -645,6 +663,7 @@ def attend_blocks_backward(geometry: BlockGeometry, queries, keys, values, table
     return grad_q, grad_k, grad_v, grad_t
 
 
+@keeps_device
 def distance_bias(squared_distances: torch.Tensor, heads: int, per_head: bool, table, edges) -> torch.Tensor:
     """Bias (..., heads, k) of contiguous squared distances (..., heads, k) or (..., k)."""
     device = squared_distances.device
@@ -658,6 +677,7 @@ def distance_bias(squared_distances: torch.Tensor, heads: int, per_head: bool, t
     return out
 
 
+@keeps_device
 def distance_bias_backward(squared_distances, heads: int, per_head: bool, edges, grad_out) -> torch.Tensor:
     """Gradient (heads, buckets) of the bias table."""
     device = squared_distances.device

@@ -192,6 +192,7 @@ int check_features(const char* op, const tbvh_attend_features* f, bool pointers)
   return TBVH_OK;
 }
 
+// All but the status word, which is the current device's.
 AttendArgs common_args(const tbvh_block_geometry* g, const tbvh_attend_features* f, const BlockSetup& s,
                        bool back) {
   AttendArgs a{};
@@ -211,7 +212,6 @@ AttendArgs common_args(const tbvh_block_geometry* g, const tbvh_attend_features*
   a.table = f->num_buckets > 0 ? f->bias_table : nullptr;
   a.edges = f->bias_edges;
   a.buckets = f->num_buckets;
-  a.status = device_status_ptr();
   a.splits = 1;
   plan_heads(a, element_size(f->dtype), back);
   return a;
@@ -275,6 +275,7 @@ int tbvh_attend_blocks(const tbvh_block_geometry* g, const tbvh_attend_features*
   if (!f->queries || !out) return blocks_fail(TBVH_ERR_BAD_ARG, "%s: NULL query or output pointer", op);
   if (!aligned(element_size(f->dtype), out) || !aligned(8, stats) || !aligned(4, out_exact, workspace)) return misaligned(op);
   AttendArgs a = common_args(g, f, s, false);
+  a.status = device_status_ptr();
   a.splits = tile_splits(s, a);
   const size_t need = tbvh_attend_blocks_workspace_size(g, f);
   if (a.splits > 1 && (workspace == nullptr || workspace_bytes < need))
@@ -324,6 +325,7 @@ int tbvh_attend_blocks_backward(const tbvh_block_geometry* g, const tbvh_attend_
       !aligned(8, stats, workspace) || !aligned(4, out_exact, grad_table))
     return misaligned(op);
   AttendArgs a = common_args(g, f, s, true);
+  a.status = device_status_ptr();
   a.splits = tile_splits(s, a);
   const BackwardSizes b = backward_sizes(s, f, a.splits);
   if (workspace == nullptr || workspace_bytes < b.total())
