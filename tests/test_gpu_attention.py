@@ -359,6 +359,41 @@ def test_half_gradients_beside_an_outlying_value(grad):
     _check(scene, selection, f, _run(scene, selection, f))
 
 
+@pytest.mark.parametrize("num_buckets", [0, 3])  # 3: with the output kept in float32
+@pytest.mark.parametrize("points, queries, n", [(64, 64, 1), (640, 40, 10)])  # 10: tiles are split
+def test_half_weights_far_below_the_largest_keep_their_bits(points, queries, n, num_buckets):
+    # One point takes nearly all of every row's weight and has no value: what is left are sums of
+    # weights of about 2^-26, which float16 could not hold as they are, times values of 2^8.
+    scene = Scene("single", [points], [queries], 3, seed=25)
+    selection = scene.select(n)
+    f = _features(scene, F16, 2, 2, 32, num_buckets, seed=25)
+    q, k, v, grad = (f[x][0] for x in ("q", "k", "v", "grad"))
+    q *= 0.25
+    q[..., 0], k[..., 0] = 8, 0
+    k[5, :, 0] = 12.75  # 8 * 12.75 / 32^0.5 = 18.03
+    v *= 256
+    v[5] = 0
+    grad *= 256
+    if num_buckets:
+        f["table"].zero_()
+    got = _run(scene, selection, f)
+    chosen = selection["block_indices"].cpu()
+    want = oracle.Attention(torch.as_tensor(scene.points[0]), scene.orders[0], torch.as_tensor(scene.qpts[0]), chosen, q, k, v,
+                            f["table"], f["edges"], None, grad)
+    others = want.p[:, :, torch.arange(points) != 5]
+    assert 2.0**-29 < float(others.min()) and float(others.max()) < 2.0**-22
+    # dS is lifted to float16's range by the largest that it could be; below 2^-14 of that range it has
+    # half a step of 2^-24 instead of a relative one.
+    most = 2 * 32 * float(grad.abs().max()) * float(v.abs().max())
+    step = 2.0**-25 / 2.0 ** (14 - np.floor(np.log2(most))) * 32**-0.5
+    oracle.within(got[0], want.out, want.out_bound, "out")
+    oracle.within(got[1], want.dq, want.dq_bound + step * k.double().abs().sum(0), "grad of queries")
+    oracle.within(got[2], want.dk, want.dk_bound + step * q.double().abs().sum(0), "grad of keys")
+    oracle.within(got[3], want.dv, want.dv_bound, "grad of values")
+    if num_buckets:
+        oracle.within(got[4], want.dt, want.dt_bound, "grad of table")
+
+
 def test_half_gradients_without_queries():
     scene = Scene("single", [100], [0], 3, seed=13)
     selection = scene.select(4)

@@ -120,6 +120,7 @@ __device__ __forceinline__ float lds_f32(uint32_t addr) {
 //  pair_kn     B for two neighbouring n-tiles from a tile stored [depth][n]
 //  from_acc    A from an accumulator tile whose columns are the depth
 //  mma_first   mma into zeros
+// PEAK: probabilities enter their products times this, and the sums leave without it.
 template <typename T>
 struct Frag;
 
@@ -148,6 +149,7 @@ struct Frag16 {
 template <>
 struct Frag<__nv_bfloat16> : Frag16<__nv_bfloat16> {
   static constexpr int PARTS = 3;  // that hold a float32
+  static constexpr float PEAK = 1.0f;
   // Probabilities and their gradients enter the second products in 16 bits: a
   // relative half step of 2^-8 each, the same as the values they multiply.
   __device__ static __forceinline__ uint32_t pack(float x, float y) {
@@ -178,8 +180,11 @@ struct Frag<__nv_bfloat16> : Frag16<__nv_bfloat16> {
 template <>
 struct Frag<__half> : Frag16<__half> {
   static constexpr int PARTS = 2;  // that hold a float32 of [0, 1] to 2^-22 or 2^-25
-  // As above with 2^-11; the backward pass scales by a power of two so that
-  // small gradients stay normal numbers.
+  // As above with 2^-11 for normal numbers, which begin at 2^-14. A probability of 1 is
+  // therefore taken as 2^15, so that it has this relative error down to 2^-29 and 2^-40
+  // outright below; dS is scaled by a power of two of its own (gradient_lift): 2^-11
+  // relative down to 2^-29 of the most that it can be, 2^-40 of that below.
+  static constexpr float PEAK = 0x1p15f;
   __device__ static __forceinline__ uint32_t pack(float x, float y) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
@@ -212,6 +217,7 @@ struct Frag<__half> : Frag16<__half> {
 template <>
 struct Frag<float> {
   static constexpr int STEP = 8;
+  static constexpr float PEAK = 1.0f;
   struct A {
     uint32_t hi[4], lo[4];
   };

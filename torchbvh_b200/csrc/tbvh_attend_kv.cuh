@@ -251,9 +251,13 @@ __global__ void __launch_bounds__(128, CP <= 32 && sizeof(T) == 2 ? 4 : CP <= 64
           s[n][2 * r + 1] = exp2_fast(x.y);
           Pair y = add2(pair(ds[n][2 * r], ds[n][2 * r + 1]), minus_d);
           if constexpr (SIZE == 2) y = mul2(y, both(lift));
-          y = mul2(pair(s[n][2 * r], s[n][2 * r + 1]), y);
+          Pair p = pair(s[n][2 * r], s[n][2 * r + 1]);
+          y = mul2(p, y);
           ds[n][2 * r] = unpair(y).x;
           ds[n][2 * r + 1] = unpair(y).y;
+          if constexpr (F::PEAK != 1.0f) p = mul2(p, both(F::PEAK));
+          s[n][2 * r] = unpair(p).x;
+          s[n][2 * r + 1] = unpair(p).y;
         }
       }
       constexpr int STEPS = kTileQueries / F::STEP;
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(128, CP <= 32 && sizeof(T) == 2 ? 4 : CP <= 64
 #pragma unroll
       for (int n = 0; n < CP / 8; ++n) {
         store_pair(out_k, n * 8 + 2 * t, a.channels, dk[n][2 * r] * back, dk[n][2 * r + 1] * back, a.wide_out);
-        store_pair(out_v, n * 8 + 2 * t, a.channels, dv[n][2 * r], dv[n][2 * r + 1], a.wide_out);
+        store_pair(out_v, n * 8 + 2 * t, a.channels, dv[n][2 * r] / F::PEAK, dv[n][2 * r + 1] / F::PEAK, a.wide_out);
       }
     }
   }
