@@ -394,6 +394,37 @@ def test_half_weights_far_below_the_largest_keep_their_bits(points, queries, n, 
         oracle.within(got[4], want.dt, want.dt_bound, "grad of table")
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["fp32", "fp16", "bf16"])
+def test_infinite_values_are_infinite_results(dtype):
+    scene = Scene("single", [300], [70], 3, seed=26)
+    selection = scene.select(5)  # all blocks
+    f = _features(scene, dtype, 2, 2, 40, 0, seed=26)
+    clean = _run(scene, selection, f, train=False)[0]
+    f["v"][0][7, :, 3], f["v"][0][9, :, 30], f["v"][0][8, :, 12] = torch.inf, -torch.inf, torch.nan
+    got = _run(scene, selection, f, train=False)[0]
+    assert bool((got[..., 3] == torch.inf).all()) and bool((got[..., 30] == -torch.inf).all())
+    assert bool(got[..., 12].isnan().all())
+    rest = [c for c in range(40) if c not in (3, 12, 30)]
+    assert torch.equal(got[..., rest], clean[..., rest])
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["fp32", "fp16", "bf16"])
+def test_a_key_that_makes_a_logit_minus_infinity_is_masked(dtype, sign):
+    # As one whose logit is so low that its weight is zero: the same bits.
+    scene = Scene("single", [300], [70], 3, seed=27)
+    selection = scene.select(5)
+    f = _features(scene, dtype, 2, 2, 40, 4, seed=27)
+    f["q"][0][..., 2] = sign * (f["q"][0][..., 2].abs() + 0.5)
+    runs = []
+    for low in (-torch.inf, -3e4):
+        f["k"][0][11, :, 2] = sign * low
+        runs.append(_run(scene, selection, f))
+    for i in (0, 3, 4):  # output, gradients of values and table (0 times the key itself is not a number)
+        assert bool(runs[0][i].isfinite().all()) and torch.equal(runs[0][i], runs[1][i])
+    assert not runs[0][3][11].any()
+
+
 def test_half_gradients_without_queries():
     scene = Scene("single", [100], [0], 3, seed=13)
     selection = scene.select(4)

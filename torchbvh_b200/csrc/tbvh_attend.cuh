@@ -213,7 +213,11 @@ struct Frag<__half> : Frag16<__half> {
 // float32 features: each operand is split into two TF32 numbers (11 + 11 bits)
 // and the product taken as hi hi + hi lo + lo hi; what is dropped is 2^-22 of
 // it. Three TF32 products cost six bf16 ones and still twice the plain
-// multiply-add rate.
+// multiply-add rate. An infinity is a high part of the largest TF32 number and an
+// infinite low part, so that the only term with an infinity is its low part times
+// the other operand's high part, which has the product's sign (an infinite high part
+// would meet low parts of either sign). Times more than 2^11 the term with the other's
+// low part may overflow too, to the other side: such a product can be NaN.
 template <>
 struct Frag<float> {
   static constexpr int STEP = 8;
@@ -224,11 +228,9 @@ struct Frag<float> {
   using B = float[4];  // two n-tiles
 
   __device__ static __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    const float rest = x - __uint_as_float(hi);
+    asm("cvt.rna.satfinite.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    const float rest = x - __uint_as_float(hi);  // of an infinity, itself; of a NaN, NaN
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
-    // An infinity or NaN is carried by the high part alone.
-    if (!(fabsf(x) <= FLT_MAX)) lo = 0;
   }
   __device__ static __forceinline__ uint32_t lane_a(uint32_t rs, int lane) {
     return (lane >> 2) * rs + (lane & 3) * 4;
