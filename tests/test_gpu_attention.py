@@ -425,6 +425,38 @@ def test_a_key_that_makes_a_logit_minus_infinity_is_masked(dtype, sign):
     assert not runs[0][3][11].any()
 
 
+def test_float32_values_up_to_the_type_s_largest():
+    scene = Scene("single", [100], [40], 3, seed=28)
+    selection = scene.select(2)
+    f = _features(scene, F32, 1, 1, 16, 0, seed=28)
+    most = torch.finfo(F32).max
+    for row, x in enumerate((most, -most, most * (1 - 2.0**-12), most * (1 - 2.0**-11), most / 2)):
+        f["v"][0][row, 0, row] = x
+    got = _run(scene, selection, f, train=False)
+    _check(scene, selection, f, got, train=False)
+
+
+@pytest.mark.parametrize("train", [False, True])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("points, queries, n", [(2048, 3, 32), (2048, 400, 32), (64, 5, 1)])
+def test_means_of_the_type_s_largest_values(points, queries, n, dtype, train):
+    # All weights are equal: the mean of equal values is the value, though their sum is far above
+    # the type's largest. Half of the largest, which leaves room for the result's own roundings.
+    scene = Scene("single", [points], [queries], 3, seed=31)
+    selection = scene.select(n)
+    f = _features(scene, dtype, 2, 2, 16, 3, seed=31)
+    f["q"][0].zero_()
+    f["table"].zero_()
+    most = torch.finfo(dtype).max / 2
+    f["v"][0][..., 0], f["v"][0][..., 1] = most, -most
+    f["grad"][0][..., :2] = 0
+    out = _run(scene, selection, f, train=train)[0]
+    # Sums of up to 2,048 equal terms, each rounded once as it is added, and the type's rounding.
+    bound = (2100 * 2.0**-23 + oracle.HALF_STEP[dtype]) * most
+    for c, x in ((0, most), (1, -most)):
+        assert bool(((out[..., c].double() - x).abs() <= bound).all()), c
+
+
 def test_half_gradients_without_queries():
     scene = Scene("single", [100], [0], 3, seed=13)
     selection = scene.select(4)

@@ -120,7 +120,10 @@ __device__ __forceinline__ float lds_f32(uint32_t addr) {
 //  pair_kn     B for two neighbouring n-tiles from a tile stored [depth][n]
 //  from_acc    A from an accumulator tile whose columns are the depth
 //  mma_first   mma into zeros
-// PEAK: probabilities enter their products times this, and the sums leave without it.
+// Probabilities enter their products times a power of two, and the sums leave without
+// it: PEAK where a row's probabilities sum to 1, PEAK_OUT where the largest of them is 1.
+// A sum over the 2,048 keys that a row can have is then less than the type's largest
+// value, if its result is.
 template <typename T>
 struct Frag;
 
@@ -149,7 +152,7 @@ struct Frag16 {
 template <>
 struct Frag<__nv_bfloat16> : Frag16<__nv_bfloat16> {
   static constexpr int PARTS = 3;  // that hold a float32
-  static constexpr float PEAK = 1.0f;
+  static constexpr float PEAK = 1.0f, PEAK_OUT = 0x1p-12f;
   // Probabilities and their gradients enter the second products in 16 bits: a
   // relative half step of 2^-8 each, the same as the values they multiply.
   __device__ static __forceinline__ uint32_t pack(float x, float y) {
@@ -184,7 +187,7 @@ struct Frag<__half> : Frag16<__half> {
   // therefore taken as 2^15, so that it has this relative error down to 2^-29 and 2^-40
   // outright below; dS is scaled by a power of two of its own (gradient_lift): 2^-11
   // relative down to 2^-29 of the most that it can be, 2^-40 of that below.
-  static constexpr float PEAK = 0x1p15f;
+  static constexpr float PEAK = 0x1p15f, PEAK_OUT = 0x1p15f;
   __device__ static __forceinline__ uint32_t pack(float x, float y) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
@@ -221,7 +224,7 @@ struct Frag<__half> : Frag16<__half> {
 template <>
 struct Frag<float> {
   static constexpr int STEP = 8;
-  static constexpr float PEAK = 1.0f;
+  static constexpr float PEAK = 1.0f, PEAK_OUT = 0x1p-12f;
   struct A {
     uint32_t hi[4], lo[4];
   };

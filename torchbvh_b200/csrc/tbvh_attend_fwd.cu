@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(256) k_merge(AttendArgs a, int cp) {
         }
       }
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / Frag<T>::PEAK_OUT / sum;
     T* out = static_cast<T*>(a.out) + (int64_t(row) * a.heads + head) * a.channels;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
             const float2 x = unpair(mul2(add2(pair(s[n][2 * r], s[n][2 * r + 1]), both(down)), both(unit)));
             Pair p = pair(exp2_fast(x.x), exp2_fast(x.y));
             add = n == 0 ? p : add2(add, p);
-            if constexpr (F::PEAK != 1.0f) p = mul2(p, both(F::PEAK));
+            p = mul2(p, both(F::PEAK_OUT));
             s[n][2 * r] = unpair(p).x;
             s[n][2 * r + 1] = unpair(p).y;
           }
@@ -457,11 +457,11 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
           }
 #pragma unroll
           for (int n = 0; n < CP / 8; ++n) {
-            const float2 o = unpair(mul2(acc[n][r], both(1.0f / F::PEAK)));
+            const float2 o = unpair(acc[n][r]);
             part[2 + n * 8 + 2 * t] = o.x;
             part[2 + n * 8 + 2 * t + 1] = o.y;
             if constexpr (EXACT) {
-              const float2 f = unpair(mul2(fine[n][r], both(1.0f / F::PEAK)));
+              const float2 f = unpair(fine[n][r]);
               part[2 + CP + n * 8 + 2 * t] = f.x;
               part[2 + CP + n * 8 + 2 * t + 1] = f.y;
             }
@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(256, CP <= 32 ? (BACK || EXACT || sizeof(T) ==
           continue;
         }
         if (row < 0) continue;
-        const float inv = sum[r] == 0.0f ? 0.0f : 1.0f / F::PEAK / sum[r];
+        const float inv = sum[r] == 0.0f ? 0.0f : 1.0f / F::PEAK_OUT / sum[r];
         T* out = static_cast<T*>(a.out) + (int64_t(row) * a.heads + span.h0 + head) * a.channels;
 #pragma unroll
         for (int n = 0; n < CP / 8; ++n)
