@@ -564,6 +564,46 @@ def test_many_tiles_on_one_block():
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("points, n", [(60, 1), (130, 2)])
+def test_lists_of_more_tiles_than_one_window(points, n):
+    """More than 2,048 tiles on a block: the long path of the backward lists takes them in windows."""
+    queries = 70001
+    scene = Scene("single", [points], [queries], 2, seed=29)
+    selection = scene.select(n)
+    f = _features(scene, F32, 1, 1, 8, 0, seed=29)
+    got = _run(scene, selection, f)
+    chosen = selection["block_indices"].cpu()
+    counts = torch.bincount(chosen.reshape(-1))
+    assert int(counts.max()) > 66000  # (so that some block's entries lie in two windows)
+    want = oracle.Attention(torch.as_tensor(scene.points[0]), scene.orders[0], torch.as_tensor(scene.qpts[0]), chosen,
+                            f["q"][0], f["k"][0], f["v"][0], None, None, None, f["grad"][0])
+    oracle.within(got[0], want.out, want.out_bound, "out")
+    oracle.within(got[1], want.dq, want.dq_bound, "grad of queries")
+    # Sums over queries: a step of 32 is summed by itself and added to at most 2,188 others, each a half
+    # step of partial sums that are at most the sum of the terms' sizes; 2^-18 relative for each term of dV.
+    p, do = want.p[0], f["grad"][0][:, 0].double()
+    bound = (2220 * 2.0**-24 + 2.0**-18) * (p.T @ do.abs())
+    oracle.within(got[3][:, 0], want.dv[:, 0], bound, "grad of values")
+    oracle.within(got[2], want.dk, want.dk_bound, "grad of keys")
+    again = _run(scene, scene.select(n), f)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["fp32", "fp16", "bf16"])
+def test_a_cloud_alone_and_in_a_batch_that_is_split_otherwise(dtype):
+    """How often tiles are split goes by the whole call's tiles: results then differ by roundings,
+    each within its bound."""
+    scene = Scene("batched", [500] * 3, [2500] * 3, 3, seed=30)
+    f = _features(scene, dtype, 4, 4, 32, 9, seed=30)
+    one = Scene("single", [500], [2500], 3, seed=30)
+    one.points, one.qpts = [scene.points[1]], [scene.qpts[1]]
+    one.bvh = torchbvh.build_bvh(one.tensor(one.points))
+    g = {x: [f[x][1]] if x in ("q", "k", "v", "grad") else f[x] for x in f}
+    for s, features, tiles in ((scene, f, 3 * 79), (one, g, 79)):
+        selection = s.select(8)
+        _check(s, selection, features, _run(s, selection, features))
+
+
 def test_strides_orders_and_alignment():
     scene = Scene("single", [333], [90], 3, seed=14)
     selection = scene.select(4)
