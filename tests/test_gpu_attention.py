@@ -2,6 +2,10 @@
 float64 oracle (attention_oracle.py)."""
 from __future__ import annotations
 
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -602,6 +606,36 @@ def test_a_cloud_alone_and_in_a_batch_that_is_split_otherwise(dtype):
     for s, features, tiles in ((scene, f, 3 * 79), (one, g, 79)):
         selection = s.select(8)
         _check(s, selection, features, _run(s, selection, features))
+
+
+FIRST_CALLS = """
+import torch, torchbvh_b200 as t
+heads, kv, types, buckets, train = {}
+selection = t.select_blocks(t.build_bvh(torch.rand(90, 3, device="cuda")), torch.rand(40, 3, device="cuda"), 2)
+table, edges = torch.zeros(heads, buckets, device="cuda"), torch.zeros(buckets - 1, device="cuda")
+for dtype, channels in types:
+    q = torch.randn(40, heads, channels, device="cuda").to(dtype)
+    k = torch.randn(90, kv, channels, device="cuda").to(dtype).requires_grad_(train)
+    out = t.attend_blocks(selection, q, k, k, bias_table=table, bias_edges=edges)
+    if train:
+        out.sum().backward()
+torch.cuda.synchronize()
+"""
+
+
+@pytest.mark.parametrize("call", [
+    # Shared memory of the forward pass: 49,040 bytes beside 256 static ones, where 49,152 are the default.
+    (4, 1, [(F32, 20), (F16, 40), (BF16, 64)], 8, False),
+    (5, 1, [(F32, 32), (F16, 64), (BF16, 33)], 1, False),
+    # The same of the gradients of keys: 48,912 bytes.
+    (46, 1, [(F16, 32), (BF16, 8)], 8, True),
+])
+def test_the_first_call_of_a_process(call):
+    """A kernel's limit of shared memory is raised for the process: what an earlier call of other
+    shapes may have raised is not there yet."""
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(call)], capture_output=True, text=True, timeout=300,
+                          cwd=Path(__file__).resolve().parents[1])
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_strides_orders_and_alignment():
