@@ -256,13 +256,23 @@ def attend_blocks(selection: BlockSelection, queries: torch.Tensor, keys: torch.
     ``C ** -0.5``), plus ``bias_table[h, b]`` where ``b`` is the number of
     ``bias_edges`` not above the squared distance of the two points (float32).
     ``bias_table (H, num_buckets)`` and ``bias_edges (num_buckets - 1,)`` are
-    float32, with 1 to 64 buckets; a bias of -inf masks its bucket. A query with
-    no point to attend to gets zeros.
+    float32, with 1 to 64 buckets; a bias of -inf masks its bucket, whose points
+    still have to be finite (they enter with a weight of zero). A query with no
+    point to attend to gets zeros.
 
     Differentiable in ``queries``, ``keys``, ``values`` and ``bias_table`` (the
     selection must have been made with ``backward=True``), in reverse mode. Results and gradients
     of equal inputs are equal bit for bit: nothing is summed in changing order.
-    Products of 16-bit features are summed in float32; the softmax is float32.
+    (A call of more queries, or a larger batch, may split its sums otherwise.)
+
+    All sums and the softmax are float32. With 16-bit features the weights are
+    rounded to 16 bits before their product with the values, and so are the
+    logits' gradients before theirs with keys and queries: one more half step of
+    the type, relative to each (float16: of weights down to 2^-29, and of
+    gradients down to 2^-29 of the largest that they could be; below, 2^-40 of
+    it). Products of float32 features keep all but 2^-22 of themselves. The
+    table's gradient is summed in float32 within a thread block, in float64
+    across them.
     """
     prefix = "attend_blocks"
     if not isinstance(selection, BlockSelection):

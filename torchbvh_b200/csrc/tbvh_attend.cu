@@ -125,9 +125,9 @@ cudaError_t run_delta(const void* grad, const void* out, const float* exact, flo
 size_t pad256(size_t v) { return (v + 255) / 256 * 256; }
 
 // Splits of the kernels by query tile: enough thread blocks for four an SM when the
-// tiles alone are fewer than two, never more than a tile can have entries (189 thread
-// blocks, float32 training: 622 us, 645 when only fewer than 148 were split; 64 as
-// one: 1,773 us, split 664).
+// tiles alone are fewer than two, never more than a tile can have entries (training
+// passes, float32: 189 thread blocks 564 us, 613 when only fewer than 148 were split;
+// 64 of one head of 96 over 12 blocks 811 us, 1,351 as one).
 int tile_splits(const BlockSetup& s, const AttendArgs& a) {
   const int64_t blocks = s.map.num_tiles * head_groups(a);
   if (blocks <= 0 || blocks >= 2 * 148) return 1;

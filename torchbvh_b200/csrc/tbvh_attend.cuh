@@ -4,12 +4,13 @@
 // Products run on warp-level matrix instructions (mma.sync m16n8) with
 // accumulators in registers. Every score costs more than its products: mask,
 // bucket lookup, bias, exponential, rounding. With 32 channels and a bias the
-// forward pass issues 44 thread instructions a selected score (184 M warp
-// instructions for 134 M scores), 64 multiply-adds of which would take a
-// tensor-memory instruction a twentieth of that time: the issue slots bound these
-// kernels, not the matrix pipe (14 % busy). And a 16-row instruction lets a warp
-// skip a block that none of its 16 queries selected, which a 128-row tile in tensor
-// memory could not.
+// forward pass issues 44 thread instructions a selected score (187 M warp instructions
+// for 134 M scores), 33 a computed one: a warp computes all 16 rows of a block that any
+// of them selected, 1.3 to 1.9 scores for one. The 64 multiply-adds of a score would take
+// a tensor-memory instruction a twentieth of that time: issue (58 % of its slots) and the
+// waits between a step's barriers bound these kernels, not the matrix pipe (14 % busy).
+// And a 16-row instruction lets a warp skip a block that none of its 16 queries selected,
+// which a 128-row tile in tensor memory could not.
 #pragma once
 
 #include <cuda_bf16.h>

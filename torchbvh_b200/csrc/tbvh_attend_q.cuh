@@ -26,10 +26,10 @@
 // values reach only the rows that attend to them.
 //
 // Bound by issue and by the latencies between a step's barriers, not by bytes or
-// products. 4 x 16,384 queries over 8 blocks, 4 heads of 32, bf16, 32 buckets: 0.33
-// ms, 4e11 scores a second (52 TFLOP/s of products), issue slots 58 % busy, matrix
-// pipe 14 %, exponentials 17 %, DRAM 2 %; without a bias 0.22 ms. In a training pass
-// of 16,384 queries with 8 heads: forward (EXACT) 0.35 ms, backward 0.35 ms.
+// products. 4 x 16,384 queries over 8 blocks, 4 heads of 32, bf16, 32 buckets: 0.34
+// ms, 4e11 scores a second (51 TFLOP/s of products), issue slots 58 % busy, matrix
+// pipe 14 %, exponentials 17 %, DRAM 2 %; without a bias 0.24 ms. In a training pass
+// of 16,384 queries with 8 heads: forward (EXACT) 0.36 ms, backward 0.35 ms.
 // Measured and left: rows by bulk copies of one thread (a step 1.7 times as long);
 // two warps that share four heads' scores of 16 rows (1.25 to 1.5 times); 32 rows a
 // warp (0.35 ms with, 0.24 without a bias).
