@@ -2,8 +2,10 @@
 float64 oracle (attention_oracle.py)."""
 from __future__ import annotations
 
+import ctypes
 import subprocess
 import sys
+import threading
 from pathlib import Path
 
 import numpy as np
@@ -11,6 +13,7 @@ import pytest
 import torch
 
 import torchbvh_b200 as torchbvh
+from torchbvh_b200 import _native
 from tests import attention_oracle as oracle
 
 pytestmark = pytest.mark.gpu
@@ -636,6 +639,54 @@ def test_the_first_call_of_a_process(call):
     done = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(call)], capture_output=True, text=True, timeout=300,
                           cwd=Path(__file__).resolve().parents[1])
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("op", ["attend", "bias"])
+def test_two_threads_at_once(op):
+    """Entries whose kernel is the same but needs different amounts of shared memory, each in a loop
+    of its own thread and stream: no launch may find the limit that the other one needs."""
+    lib = _native.load_library()
+    scene = Scene("single", [65], [3], 3, seed=32)
+    selection = scene.select(1)
+    calls, results = [], []
+    for heads, buckets in ((4, 64), (2, 42)):
+        table, edges = torch.randn((heads, buckets), device="cuda"), torch.logspace(-4, 0, buckets - 1, device="cuda")
+        if op == "attend":
+            f = _features(scene, F32, heads, heads, 32, 0, seed=32)
+            q, k, v = (scene.tensor(f[x]) for x in "qkv")
+            out, keep = torch.empty_like(q), (q, k, v, table, edges)
+            features = _native._attend_features(*keep, 0.2)
+            want = torchbvh.attend_blocks(selection, q, k, v, bias_table=table, bias_edges=edges, scale=0.2)
+            size = lib.tbvh_attend_blocks_workspace_size(ctypes.byref(selection._geometry), ctypes.byref(features))
+            ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+            args = (ctypes.byref(selection._geometry), ctypes.byref(features), out.data_ptr(), None, None, ws.data_ptr(), size)
+            calls.append((lib.tbvh_attend_blocks, args, keep, ws))
+        else:
+            d2, grad = torch.rand((1, 5, 8), device="cuda"), torch.randn((1, 5, heads, 8), device="cuda")
+            out = torch.empty_like(table)
+            want, = torch.autograd.grad(torchbvh.distance_bias(d2, table.requires_grad_(), edges), table, grad)
+            size = lib.tbvh_distance_bias_backward_workspace_size(5, heads, 8, buckets)
+            ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+            args = (0, d2.data_ptr(), 5, heads, 8, 0, edges.data_ptr(), buckets, grad.data_ptr(), out.data_ptr(),
+                    ws.data_ptr(), size)
+            calls.append((lib.tbvh_distance_bias_backward, args, (d2, grad, edges), ws))
+        results.append((out, want))
+    torch.cuda.synchronize()
+    start, codes = threading.Barrier(len(calls)), []
+
+    def repeat(entry, args, *keep):
+        stream = torch.cuda.Stream()
+        start.wait(30)
+        codes.append({entry(*args, stream.cuda_stream) for _ in range(20000)})
+        stream.synchronize()
+
+    threads = [threading.Thread(target=repeat, args=call) for call in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert codes == [{0}, {0}]
+    assert all(torch.equal(out, want) for out, want in results)
 
 
 def test_strides_orders_and_alignment():

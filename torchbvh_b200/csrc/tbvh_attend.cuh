@@ -782,13 +782,14 @@ cudaError_t launch_table_sum(const float* part, double* scratch, float* grad_tab
 inline int padded_channels(int channels) { return channels <= 32 ? 32 : channels <= 64 ? 64 : channels <= 96 ? 96 : 128; }
 
 // Raises a kernel's dynamic shared-memory limit where the launch needs it: 48 KB hold the
-// kernel's static arrays too.
-constexpr size_t kStaticSmem = 1024;  // at least those of any kernel this is called for
+// kernel's static arrays too. Always to the same size, which leaves them room in an SM's
+// 227 KB: with the launch's own, a call in another thread could lower it in between.
+constexpr size_t kStaticSmem = 11 * 1024;  // at least those of any kernel this is called for
 template <typename K>
 cudaError_t allow_smem(K kernel, size_t bytes) {
-  return bytes + kStaticSmem > 48 * 1024
-             ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes))
-             : cudaSuccess;
+  return bytes + kStaticSmem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                                227 * 1024 - int(kStaticSmem))
+                                         : cudaSuccess;
 }
 
 }  // namespace tbvh

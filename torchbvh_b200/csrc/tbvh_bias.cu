@@ -265,7 +265,8 @@ int tbvh_distance_bias_backward(int device, const float* squared_distances, int6
   BiasArgs a{squared_distances, nullptr, edges, grad_out, part, rows, k, heads, num_buckets, per_head != 0};
   const size_t smem = size_t(num_buckets) * kBiasThreads * 4;
   const bool four = by_four(k, squared_distances, grad_out);
-  e = four ? allow_smem(k_bias_grad<4>, smem + sizeof(BucketTable)) : allow_smem(k_bias_grad<1>, smem + sizeof(BucketTable));
+  static_assert(sizeof(BucketTable) + 4 * kMaxBuckets <= kStaticSmem, "static arrays of k_bias_grad");
+  e = four ? allow_smem(k_bias_grad<4>, smem) : allow_smem(k_bias_grad<1>, smem);
   if (e != cudaSuccess) return blocks_cuda_fail(e, op);
   const dim3 grid{unsigned(blocks), unsigned(heads)};
   if (four) k_bias_grad<4><<<grid, kBiasThreads, smem, st>>>(a);
