@@ -123,8 +123,8 @@ __device__ __forceinline__ float lds_f32(uint32_t addr) {
 //  mma_first   mma into zeros
 // Probabilities enter their products times a power of two, and the sums leave without
 // it: PEAK where a row's probabilities sum to 1, PEAK_OUT where the largest of them is 1.
-// A sum over the 2,048 keys that a row can have is then less than the type's largest
-// value, if its result is.
+// A sum over the 2,048 keys that a row can have then stays below the type's largest
+// value; with 2^-12, what is below 2^-114 of a row's largest may be flushed to zero.
 template <typename T>
 struct Frag;
 
